@@ -15,7 +15,7 @@ DION_BF16 = 0
 DION_F32 = 1
 DION_NS_GRAM = 1
 DION_NS_STATIC_SCRATCH_BYTES = 64 << 20
-ABI_VERSION = 14  # dion_abi_version() of the library these signatures describe
+ABI_VERSION = 15  # dion_abi_version() of the library these signatures describe
 
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _i64p = ctypes.POINTER(ctypes.c_int64)
@@ -104,6 +104,11 @@ SIGNATURES = {
                                        c_void_p]),
     "dion_adamw_step": (c_int, [_u64p, _u64p, c_int, _u64p, _u64p, c_int, _u64p, _i64p, c_int, c_void_p, c_float,
                                 c_float, c_float, c_void_p, c_float, c_int, c_void_p]),
+    "dion_adamw_fp32_state_step": (c_int, [_u64p, c_int, _u64p, c_int, _u64p, _u64p, _u64p, _i64p, c_int, c_void_p,
+                                           c_float, c_float, c_float, c_void_p, c_float, c_int, c_void_p]),
+    "dion_adamw8_step": (c_int, [_u64p, c_int, _u64p, c_int, _u64p, _u64p, _u64p, _u64p, _u64p, _i64p, c_int, c_void_p,
+                                 c_float, c_float, c_float, c_void_p, c_float, c_int, c_int, c_void_p]),
+    "dion_state8_values": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p]),
     "dion_lion_step": (c_int, [_u64p, _u64p, c_int, _u64p, c_int, _i64p, c_int, c_void_p, c_float, c_float,
                                c_void_p, c_float, c_int, c_void_p]),
 }

@@ -37,7 +37,7 @@ static inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 static inline bool aligned16(uint64_t p) { return (p & 15) == 0; }
 
 extern "C" const char* dion_last_error(void) { return g_err; }
-extern "C" int dion_abi_version(void) { return 14; }
+extern "C" int dion_abi_version(void) { return 15; }
 
 // ---------------------------------------------------------------------------------------------
 // Kernel-level GEMMs
@@ -1782,35 +1782,98 @@ static int check_mta(const char* who, const uint64_t* X, const uint64_t* G, int 
   return DION_OK;
 }
 
+// One step counter may serve several tensors; a counter shared ACROSS launch chunks would be
+// advanced once per chunk, so every chunk must own its counters.
+static int check_step_counters(const char* who, const uint64_t* step_ptrs, int n) {
+  if (!step_ptrs) return fail(DION_E_INVALID, "%s: null argument", who);
+  for (int i = 0; i < n; ++i)
+    if (!step_ptrs[i]) return fail(DION_E_INVALID, "%s: tensor %d has a null state pointer", who, i);
+  for (int i = kMtaTensors; i < n; ++i)
+    for (int j = 0; j < i / kMtaTensors * kMtaTensors; ++j)
+      if (step_ptrs[i] == step_ptrs[j])
+        return fail(DION_E_INVALID,
+                    "%s: step counter of tensor %d is shared with tensor %d of an earlier chunk of %d tensors", who, i, j,
+                    kMtaTensors);
+  return DION_OK;
+}
+
+static int adamw_step(const char* who, const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype,
+                      const uint64_t* M_ptrs, const uint64_t* V_ptrs, int s_dtype, const uint64_t* step_ptrs,
+                      const int64_t* numels, int n, const float* lr_dev, float beta1, float beta2, float eps,
+                      const float* wd_dev, float wd_host, int cautious, void* stream) {
+  if (int rc = check_state_dtype(who, "s_dtype", s_dtype)) return rc;
+  if (int rc = check_state_dtype(who, "x_dtype", x_dtype)) return rc;
+  if (x_dtype != s_dtype && x_dtype != DION_BF16)
+    return fail(DION_E_INVALID, "%s: moments are kept in the parameters' type or in fp32", who);
+  if (int rc = check_mta(who, X_ptrs, G_ptrs, g_dtype, M_ptrs, numels, n, lr_dev)) return rc;
+  if (n == 0) return DION_OK;
+  if (!V_ptrs) return fail(DION_E_INVALID, "%s: null argument", who);
+  for (int i = 0; i < n; ++i)
+    if (numels[i] > 0 && !V_ptrs[i]) return fail(DION_E_INVALID, "%s: tensor %d has a null state pointer", who, i);
+  if (int rc = check_step_counters(who, step_ptrs, n)) return rc;
+  for (int i0 = 0; i0 < n; i0 += kMtaTensors) {
+    const int c = (n - i0) < kMtaTensors ? (n - i0) : kMtaTensors;
+    HIP_TRY(launch_adamw_mt(X_ptrs + i0, dt(x_dtype), G_ptrs + i0, dt(g_dtype), M_ptrs + i0, V_ptrs + i0, dt(s_dtype),
+                            step_ptrs + i0, numels + i0, c, lr_dev, beta1, beta2, eps, wd_dev, wd_host, cautious,
+                            (hipStream_t)stream),
+            who);
+  }
+  return DION_OK;
+}
+
 extern "C" int dion_adamw_step(const uint64_t* X_ptrs, const uint64_t* G_ptrs, int g_dtype,
                                const uint64_t* M_ptrs, const uint64_t* V_ptrs, int s_dtype,
                                const uint64_t* step_ptrs, const int64_t* numels, int n,
                                const float* lr_dev, float beta1, float beta2, float eps,
                                const float* wd_dev, float wd_host, int cautious, void* stream) {
-  if (int rc = check_state_dtype("dion_adamw_step", "s_dtype", s_dtype)) return rc;
-  if (int rc = check_mta("dion_adamw_step", X_ptrs, G_ptrs, g_dtype, M_ptrs, numels, n, lr_dev)) return rc;
+  return adamw_step("dion_adamw_step", X_ptrs, s_dtype, G_ptrs, g_dtype, M_ptrs, V_ptrs, s_dtype, step_ptrs, numels, n,
+                    lr_dev, beta1, beta2, eps, wd_dev, wd_host, cautious, stream);
+}
+
+extern "C" int dion_adamw_fp32_state_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype,
+                                          const uint64_t* M_ptrs, const uint64_t* V_ptrs, const uint64_t* step_ptrs,
+                                          const int64_t* numels, int n, const float* lr_dev, float beta1, float beta2,
+                                          float eps, const float* wd_dev, float wd_host, int cautious, void* stream) {
+  return adamw_step("dion_adamw_fp32_state_step", X_ptrs, x_dtype, G_ptrs, g_dtype, M_ptrs, V_ptrs, DION_F32, step_ptrs,
+                    numels, n, lr_dev, beta1, beta2, eps, wd_dev, wd_host, cautious, stream);
+}
+
+extern "C" int dion_adamw8_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype,
+                                const uint64_t* M_ptrs, const uint64_t* M_scale_ptrs, const uint64_t* V_ptrs,
+                                const uint64_t* V_scale_ptrs, const uint64_t* step_ptrs, const int64_t* numels, int n,
+                                const float* lr_dev, float beta1, float beta2, float eps, const float* wd_dev,
+                                float wd_host, int cautious, int seed, void* stream) {
+  const char* who = "dion_adamw8_step";
+  if (int rc = check_state_dtype(who, "x_dtype", x_dtype)) return rc;
+  if (int rc = check_mta(who, X_ptrs, G_ptrs, g_dtype, M_ptrs, numels, n, lr_dev)) return rc;
   if (n == 0) return DION_OK;
-  if (!V_ptrs || !step_ptrs) return fail(DION_E_INVALID, "dion_adamw_step: null argument");
-  for (int i = 0; i < n; ++i)
-    if (!step_ptrs[i] || (numels[i] > 0 && !V_ptrs[i]))
-      return fail(DION_E_INVALID, "dion_adamw_step: tensor %d has a null state pointer", i);
-  // One step counter may serve several tensors; a counter shared ACROSS launch chunks would be
-  // advanced once per chunk, so every chunk must own its counters.
+  if (!M_scale_ptrs || !V_ptrs || !V_scale_ptrs) return fail(DION_E_INVALID, "%s: null argument", who);
+  for (int i = 0; i < n; ++i) {
+    if (numels[i] > 0 && (!M_scale_ptrs[i] || !V_ptrs[i] || !V_scale_ptrs[i]))
+      return fail(DION_E_INVALID, "%s: tensor %d has a null state pointer", who, i);
+    if ((M_scale_ptrs[i] | V_scale_ptrs[i]) & 3)
+      return fail(DION_E_INVALID, "%s: the scales of tensor %d are not 4-byte aligned", who, i);
+    if (numels[i] > (int64_t(1) << 34)) return fail(DION_E_INVALID, "%s: tensor %d has more than 2^34 elements", who, i);
+  }
+  if (int rc = check_step_counters(who, step_ptrs, n)) return rc;
   for (int i0 = 0; i0 < n; i0 += kMtaTensors) {
     const int c = (n - i0) < kMtaTensors ? (n - i0) : kMtaTensors;
-    for (int i = i0; i < i0 + c; ++i)
-      for (int j = 0; j < i0; ++j)
-        if (step_ptrs[i] == step_ptrs[j])
-          return fail(DION_E_INVALID,
-                      "dion_adamw_step: step counter of tensor %d is shared with tensor %d of an earlier "
-                      "chunk of %d tensors",
-                      i, j, kMtaTensors);
-    HIP_TRY(launch_adamw_mt(X_ptrs + i0, G_ptrs + i0, dt(g_dtype), M_ptrs + i0, V_ptrs + i0, dt(s_dtype),
-                            step_ptrs + i0,
-                            numels + i0, c, lr_dev, beta1, beta2, eps, wd_dev, wd_host, cautious,
-                            (hipStream_t)stream),
-            "dion_adamw_step");
+    HIP_TRY(launch_adamw8(X_ptrs + i0, dt(x_dtype), G_ptrs + i0, dt(g_dtype), M_ptrs + i0, M_scale_ptrs + i0, V_ptrs + i0,
+                          V_scale_ptrs + i0, step_ptrs + i0, numels + i0, c, lr_dev, beta1, beta2, eps, wd_dev, wd_host,
+                          cautious, (uint32_t)seed, (hipStream_t)stream),
+            who);
   }
+  return DION_OK;
+}
+
+extern "C" int dion_state8_values(const void* codes, int squared, const float* scales, int64_t numel, void* out,
+                                  int out_dtype, void* stream) {
+  if (out_dtype != DION_BF16 && out_dtype != DION_F32) return fail(DION_E_INVALID, "dion_state8_values: out_dtype");
+  if (numel < 0) return fail(DION_E_INVALID, "dion_state8_values: negative size");
+  if (numel == 0) return DION_OK;
+  if (!codes || !scales || !out) return fail(DION_E_INVALID, "dion_state8_values: null argument");
+  HIP_TRY(launch_state8_values(codes, squared, scales, numel, out, dt(out_dtype), (hipStream_t)stream),
+          "dion_state8_values");
   return DION_OK;
 }
 

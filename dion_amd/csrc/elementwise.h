@@ -118,12 +118,21 @@ hipError_t launch_dion2_post_masked(const PtrTab& X, const PtrTab& M, int s_dtyp
 // Multi-tensor AdamW / Lion (scalar_opts.hip): n <= kMtaTensors tensors per launch, host arrays of
 // device pointers and element counts.
 constexpr int kMtaTensors = 48;
-hipError_t launch_adamw_mt(const uint64_t* X, const uint64_t* G, int g_dtype, const uint64_t* M,
+// (x_dtype is s_dtype, or bf16 beside fp32 moments)
+hipError_t launch_adamw_mt(const uint64_t* X, int x_dtype, const uint64_t* G, int g_dtype, const uint64_t* M,
                            const uint64_t* V, int s_dtype, const uint64_t* steps, const int64_t* numel, int n,
                            const float* lr_dev, float beta1, float beta2, float eps, const float* wd_dev,
                            float wd_host, int cautious, hipStream_t st);
 hipError_t launch_lion_mt(const uint64_t* X, const uint64_t* G, int g_dtype, const uint64_t* M, int s_dtype,
                           const int64_t* numel, int n, const float* lr_dev, float beta1, float beta2,
                           const float* wd_dev, float wd_host, int cautious, hipStream_t st);
+
+// AdamW with moments in 8 bits (adamw8.hip): n <= kMtaTensors tensors per launch.
+hipError_t launch_adamw8(const uint64_t* X, int x_dtype, const uint64_t* G, int g_dtype, const uint64_t* M,
+                         const uint64_t* MS, const uint64_t* V, const uint64_t* VS, const uint64_t* steps,
+                         const int64_t* numel, int n, const float* lr_dev, float beta1, float beta2, float eps,
+                         const float* wd_dev, float wd_host, int cautious, uint32_t seed, hipStream_t st);
+hipError_t launch_state8_values(const void* codes, int squared, const float* scales, int64_t numel, void* out,
+                                int out_dtype, hipStream_t st);
 
 }  // namespace dion

@@ -6,8 +6,8 @@
 // tensor: kMtaChunk of them (the tensor found by bisection in a table of first workgroups, a thread with the loads
 // of sixteen elements in flight at once), or in small launches a short run (mta_run; BRIEF).  All traffic is HBM streaming: AdamW reads X, G, M, V
 // and writes X, M, V (28 B/element with fp32 state and gradients, 26 with bf16 gradients), Lion 20 / 18
-// B/element.  The state tensors X, M, V of one launch share a dtype, fp32 or bf16 (half the bytes);
-// arithmetic is fp32 either way.
+// B/element.  The state tensors X, M, V of one launch share a dtype, fp32 or bf16 (half the bytes), or AdamW's
+// M and V are fp32 beside bf16 X; arithmetic is fp32 either way.
 // Bound by HBM.  2 x (50304 x 768) + norms, fp32 state, bf16 gradients: AdamW 580 us (3.5 TB/s) with a grid row per
 // tensor and one group of four elements in flight -> 394 us (5.1 TB/s) -> 356 us (5.65 TB/s) with non-temporal accesses;
 // Lion 295 -> 234 us (5.9 TB/s).  Device copy on the same card: 5.2-6.1 TB/s.
@@ -74,7 +74,8 @@ static __device__ __forceinline__ void adamw_one(float& x, float g, float& m, fl
   x = x - adj_lr * upd;
 }
 
-template <typename GT, typename ST, bool NT, bool BRIEF = false>
+// XT: the parameters' type, ST: the moments' (the same, or fp32 beside bf16 parameters)
+template <typename GT, typename XT, typename ST, bool NT, bool BRIEF = false>
 __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, const float* __restrict__ lr_dev,
                                                        const float* __restrict__ wd_dev,
                                                        AdamwScalars sc) {
@@ -82,12 +83,12 @@ __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, cons
   const int64_t first = (int64_t)(blockIdx.x - (BRIEF ? 0 : a.wg0[t])) * a.run;
   if (BRIEF && first >= a.numel[t]) return;
   const int64_t end = a.numel[t] < first + a.run ? a.numel[t] : first + a.run;
-  ST* __restrict__ x = (ST*)a.x[t];
+  XT* __restrict__ x = (XT*)a.x[t];
   const GT* __restrict__ g = (const GT*)a.g[t];
   ST* __restrict__ m = (ST*)a.m[t];
   ST* __restrict__ v = (ST*)a.v[t];
   // groups of 4 elements: 16-byte accesses to fp32 tensors, 8-byte accesses to bf16 ones
-  const bool vec = (((a.x[t] | a.m[t] | a.v[t]) & (sizeof(ST) == 2 ? 7 : 15)) == 0) &&
+  const bool vec = (((a.m[t] | a.v[t]) & (sizeof(ST) == 2 ? 7 : 15)) == 0) && ((a.x[t] & (sizeof(XT) == 2 ? 7 : 15)) == 0) &&
                    ((a.g[t] & (sizeof(GT) == 2 ? 7 : 15)) == 0);
   float w1, w2, inv_bc2_sqrt, adj_lr, coeff, aa;
   auto scalars = [&]() {
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, cons
       const int64_t q0 = (first + r * kMtaRound) / 4 + threadIdx.x;
 #pragma unroll
       for (int u = 0; u < kMtaGroups; ++u) {
-        st_load4<ST, NT>(x, q0 + u * 256, xv[u]);
+        st_load4<XT, NT>(x, q0 + u * 256, xv[u]);
         st_load4<ST, NT>(m, q0 + u * 256, mv[u]);
         st_load4<ST, NT>(v, q0 + u * 256, vv[u]);
         st_load4<GT, NT>(g, q0 + u * 256, gv[u]);
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, cons
         for (int e = 0; e < 4; ++e)
           adamw_one<GT>(xv[u][e], gv[u][e], mv[u][e], vv[u][e], w1, sc.beta2, w2, inv_bc2_sqrt, sc.eps, adj_lr, aa,
                         coeff, sc.cautious);
-        st_store4<ST, NT>(x, q0 + u * 256, xv[u]);
+        st_store4<XT, NT>(x, q0 + u * 256, xv[u]);
         st_store4<ST, NT>(m, q0 + u * 256, mv[u]);
         st_store4<ST, NT>(v, q0 + u * 256, vv[u]);
       }
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, cons
   float xv[4], mv[4], vv[4], gv[4];
   auto load = [&]() {
     if (q >= vend / 4) return;
-    st_load4<ST>(x, q, xv);
+    st_load4<XT>(x, q, xv);
     st_load4<ST>(m, q, mv);
     st_load4<ST>(v, q, vv);
     st_load4<GT>(g, q, gv);
@@ -147,15 +148,15 @@ __global__ __launch_bounds__(256) void adamw_mt_kernel(MtaTensors a, int n, cons
     for (int e = 0; e < 4; ++e)
       adamw_one<GT>(xv[e], gv[e], mv[e], vv[e], w1, sc.beta2, w2, inv_bc2_sqrt, sc.eps, adj_lr, aa, coeff,
                     sc.cautious);
-    st_store4<ST>(x, q, xv);
+    st_store4<XT>(x, q, xv);
     st_store4<ST>(m, q, mv);
     st_store4<ST>(v, q, vv);
   }
   for (int64_t i = vend + threadIdx.x; i < end; i += 256) {
-    float xs = st_load<ST>(x, i), ms = st_load<ST>(m, i), vs = st_load<ST>(v, i);
+    float xs = st_load<XT>(x, i), ms = st_load<ST>(m, i), vs = st_load<ST>(v, i);
     adamw_one<GT>(xs, st_load<GT>(g, i), ms, vs, w1, sc.beta2, w2, inv_bc2_sqrt, sc.eps, adj_lr, aa, coeff,
                   sc.cautious);
-    st_store<ST>(x, i, xs);
+    st_store<XT>(x, i, xs);
     st_store<ST>(m, i, ms);
     st_store<ST>(v, i, vs);
   }
@@ -276,7 +277,7 @@ static dim3 mta_grid(const MtaTensors& a, const int64_t* numel, int n) {
   return dim3((unsigned)((longest + a.run - 1) / a.run), n);
 }
 
-hipError_t launch_adamw_mt(const uint64_t* X, const uint64_t* G, int g_dtype, const uint64_t* M,
+hipError_t launch_adamw_mt(const uint64_t* X, int x_dtype, const uint64_t* G, int g_dtype, const uint64_t* M,
                            const uint64_t* V, int s_dtype, const uint64_t* steps, const int64_t* numel, int n,
                            const float* lr_dev, float beta1, float beta2, float eps, const float* wd_dev,
                            float wd_host, int cautious, hipStream_t st) {
@@ -284,20 +285,22 @@ hipError_t launch_adamw_mt(const uint64_t* X, const uint64_t* G, int g_dtype, co
   if (!fill(a, X, G, M, V, steps, numel, n)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(mta_advance_steps_kernel, dim3(1), dim3(64), 0, st, a, n);
   if (a.wg0[n] == 0) return hipGetLastError();
-  const bool nt = past_caches(numel, n, 3 * (s_dtype == 0 ? 2 : 4) + (g_dtype == 0 ? 2 : 4));
+  const bool nt = past_caches(numel, n, (x_dtype == 0 ? 2 : 4) + 2 * (s_dtype == 0 ? 2 : 4) + (g_dtype == 0 ? 2 : 4));
   AdamwScalars sc{beta1, beta2, eps, wd_host, cautious};
   const dim3 grid = mta_grid(a, numel, n);
-#define ADAMW_LAUNCH(GT, ST)                                                                                       \
+#define ADAMW_LAUNCH(GT, XT, ST)                                                                                       \
   do {                                                                                                             \
     if (a.run != kMtaChunk)                                                                                        \
-      hipLaunchKernelGGL((adamw_mt_kernel<GT, ST, false, true>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); \
-    else if (nt) hipLaunchKernelGGL((adamw_mt_kernel<GT, ST, true>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); \
-    else hipLaunchKernelGGL((adamw_mt_kernel<GT, ST, false>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc);   \
+      hipLaunchKernelGGL((adamw_mt_kernel<GT, XT, ST, false, true>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); \
+    else if (nt) hipLaunchKernelGGL((adamw_mt_kernel<GT, XT, ST, true>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); \
+    else hipLaunchKernelGGL((adamw_mt_kernel<GT, XT, ST, false>), grid, dim3(256), 0, st, a, n, lr_dev, wd_dev, sc);   \
   } while (0)
-  if (g_dtype == 0) {
-    if (s_dtype == 0) ADAMW_LAUNCH(bf16_t, bf16_t); else ADAMW_LAUNCH(bf16_t, float);
+  if (s_dtype == 0) {
+    if (g_dtype == 0) ADAMW_LAUNCH(bf16_t, bf16_t, bf16_t); else ADAMW_LAUNCH(float, bf16_t, bf16_t);
+  } else if (x_dtype == 0) {
+    if (g_dtype == 0) ADAMW_LAUNCH(bf16_t, bf16_t, float); else ADAMW_LAUNCH(float, bf16_t, float);
   } else {
-    if (s_dtype == 0) ADAMW_LAUNCH(float, bf16_t); else ADAMW_LAUNCH(float, float);
+    if (g_dtype == 0) ADAMW_LAUNCH(bf16_t, float, float); else ADAMW_LAUNCH(float, float, float);
   }
 #undef ADAMW_LAUNCH
   return hipGetLastError();

@@ -78,7 +78,8 @@ def adamw_update_foreach(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: L
                          beta1: Scalar, beta2: Scalar, weight_decay: Scalar, step: Optional[int] = None,
                          epsilon: float = 1e-8, cautious_wd: bool = False,
                          state_steps: Optional[List[Tensor]] = None) -> None:
-    """Same call as dion/scalar_opts.py:121-134.  ``state_steps`` (per-parameter 0-d fp32 device counters,
+    """Same call as dion/scalar_opts.py:121-134.  ``M`` and ``V`` in the dtype of ``X``, or float32 beside bfloat16
+    parameters.  ``state_steps`` (per-parameter 0-d fp32 device counters,
     advanced on the device) or the legacy python-int ``step`` (the value to use for this update)."""
     if not X:
         return
@@ -93,6 +94,24 @@ def adamw_update_foreach(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: L
             state_steps += [counter] * min(48, len(X) - i0)
     ops.adamw_step(X, [g.contiguous() for g in G], M, V, state_steps, _device_scalar(lr, dev), _host_float(beta1),
                    _host_float(beta2), weight_decay, float(epsilon), cautious_wd)
+
+
+def adamw8_update_foreach(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: List[Tensor], V: List[Tensor],
+                          V_scales: List[Tensor], lr: Scalar, beta1: Scalar, beta2: Scalar, weight_decay: Scalar,
+                          state_steps: List[Tensor], epsilon: float = 1e-8, cautious_wd: bool = False,
+                          seed: int = 0) -> None:
+    """``adamw_update_foreach`` with moments in 8 bits: ``M`` int8 and ``V`` uint8 codes, ``M_scales`` and ``V_scales`` one
+    float32 scale for every 128 elements (``state8_blocks(numel)``), all zero before the first step.  ``seed``: of the random
+    rounding of the codes; equal seeds give equal results bit for bit.  ``state8_values`` gives the moments back."""
+    if not X:
+        return
+    ops.adamw8_step(X, [g.contiguous() for g in G], M, M_scales, V, V_scales, state_steps,
+                    _device_scalar(lr, X[0].device), _host_float(beta1), _host_float(beta2), weight_decay, float(epsilon),
+                    cautious_wd, seed)
+
+
+state8_blocks = ops.state8_blocks
+state8_values = ops.state8_values
 
 
 def lion_update_foreach(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Scalar, beta1: Scalar, beta2: Scalar,

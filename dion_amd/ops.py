@@ -885,15 +885,17 @@ def dion2_post_masked(X: List[Tensor], M: List[Tensor], U: Tensor, norms: Tensor
 # ---------------------------------------------------------------------------------------------
 # multi-tensor AdamW / Lion for the non-matrix parameter groups
 # ---------------------------------------------------------------------------------------------
-def _mta_tables(X: List[Tensor], G: List[Tensor], states: List[List[Tensor]]):
+def _mta_tables(X: List[Tensor], G: List[Tensor], states: List[List[Tensor]], state_dtype=None):
+    """Tables of pointers and sizes.  The states are in ``state_dtype``, or in that of X."""
     n = len(X)
     assert n > 0 and len(G) == n and all(len(s) == n for s in states)
     gdt = G[0].dtype
-    sdt = X[0].dtype
+    xdt = X[0].dtype
+    sdt = state_dtype or xdt
     for x, g in zip(X, G):
         _require_gpu(x, "X")
         _require_gpu(g, "G")
-        if x.dtype != sdt:
+        if x.dtype != xdt:
             raise TypeError("X: one parameter dtype per call")
         if g.dtype != gdt:
             raise TypeError("G: one gradient dtype per call")
@@ -909,21 +911,90 @@ def _mta_tables(X: List[Tensor], G: List[Tensor], states: List[List[Tensor]]):
     return tabs, numels, _dtype_code(G[0], "G"), _dtype_code(X[0], "X")
 
 
+def _check_steps(steps: List[Tensor]) -> None:
+    for s in steps:
+        if not (s.is_cuda and s.dtype == torch.float32 and s.numel() == 1):
+            raise TypeError("steps must be 0-d float32 GPU tensors")
+
+
 def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor], steps: List[Tensor],
                lr: Tensor, beta1: float, beta2: float, weight_decay, epsilon: float,
                cautious_wd: bool = False) -> None:
     """One fused AdamW step over tensors of any sizes (dion/scalar_opts.py:7-65, :121-268).  ``steps``
-    are 0-d float32 device counters (one per tensor; tensors may share one), advanced on the device."""
-    (xp, gp, mp, vp), numels, gcode, scode = _mta_tables(X, G, [M, V])
-    for s in steps:
-        if not (s.is_cuda and s.dtype == torch.float32 and s.numel() == 1):
-            raise TypeError("steps must be 0-d float32 GPU tensors")
+    are 0-d float32 device counters (one per tensor; tensors may share one), advanced on the device.  ``M`` and ``V``
+    have the dtype of ``X``, or are float32 beside bfloat16 parameters."""
+    wide = len(M) > 0 and M[0].dtype == torch.float32 and X[0].dtype == torch.bfloat16
+    (xp, gp, mp, vp), numels, gcode, xcode = _mta_tables(X, G, [M, V], torch.float32 if wide else None)
+    _check_steps(steps)
     sp = ptr_table([s.data_ptr() for s in steps])
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     lib = _lib.load()
-    check(lib.dion_adamw_step(xp, gp, gcode, mp, vp, scode, sp, numels, len(X), lr_p, float(beta1), float(beta2),
-                              float(epsilon), wd_p, wd_h, int(bool(cautious_wd)), _stream_handle(X[0].device)),
-          "adamw_step")
+    rest = (sp, numels, len(X), lr_p, float(beta1), float(beta2), float(epsilon), wd_p, wd_h, int(bool(cautious_wd)),
+            _stream_handle(X[0].device))
+    if wide:
+        check(lib.dion_adamw_fp32_state_step(xp, xcode, gp, gcode, mp, vp, *rest), "adamw_step")
+    else:
+        check(lib.dion_adamw_step(xp, gp, gcode, mp, vp, xcode, *rest), "adamw_step")
+
+
+STATE8_BLOCK = 128  # elements that share a scale
+
+
+def state8_blocks(numel: int) -> int:
+    """Scales of a tensor of ``numel`` elements kept in 8 bits."""
+    return -(-numel // STATE8_BLOCK)
+
+
+def adamw8_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: List[Tensor], V: List[Tensor],
+                V_scales: List[Tensor], steps: List[Tensor], lr: Tensor, beta1: float, beta2: float, weight_decay,
+                epsilon: float, cautious_wd: bool = False, seed: int = 0) -> None:
+    """``adamw_step`` with moments in 8 bits: ``M`` int8 and ``V`` uint8 codes shaped like ``X``, ``*_scales`` float32, one
+    for every 128 elements (``state8_blocks``).  Codes are rounded up or down at random, without bias, by numbers that depend on
+    ``seed``, the step counter and the element alone."""
+    if not X:
+        return
+    n = len(X)
+    if any(len(t) != n for t in (G, M, M_scales, V, V_scales, steps)):
+        raise ValueError("adamw8_step: all lists must have one tensor for every parameter")
+    (xp, gp), numels, gcode, xcode = _mta_tables(X, G, [])
+    for name, dtype, codes, scales in (("M", torch.int8, M, M_scales), ("V", torch.uint8, V, V_scales)):
+        for x, c, s in zip(X, codes, scales):
+            _require_gpu(c, name)
+            _require_gpu(s, name + "_scales")
+            if c.dtype != dtype or not c.is_contiguous() or c.numel() != x.numel():
+                raise ValueError(f"{name}: codes must be contiguous {dtype} tensors shaped like X")
+            if s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != state8_blocks(x.numel()):
+                raise ValueError(f"{name}_scales: one contiguous float32 scale for every {STATE8_BLOCK} elements of X")
+    _check_steps(steps)
+    lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
+    tabs = [ptr_table([t.data_ptr() for t in ts]) for ts in (M, M_scales, V, V_scales, steps)]
+    check(_lib.load().dion_adamw8_step(xp, xcode, gp, gcode, *tabs, numels, n, lr_p, float(beta1), float(beta2),
+                                       float(epsilon), wd_p, wd_h, int(bool(cautious_wd)), _as_int32(seed),
+                                       _stream_handle(X[0].device)), "adamw8_step")
+
+
+def _as_int32(seed: int) -> int:
+    """The low 32 bits of a seed as the C int that carries them."""
+    low = int(seed) & 0xFFFFFFFF
+    return low - (1 << 32) if low >> 31 else low
+
+
+def state8_values(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.float32) -> Tensor:
+    """What 8-bit moments stand for, shaped like ``codes``: int8 codes (first moments) times their block's scale, the
+    square of that for uint8 codes (second moments)."""
+    _require_gpu(codes, "codes")
+    _require_gpu(scales, "scales")
+    if codes.dtype not in (torch.int8, torch.uint8):
+        raise TypeError(f"codes: dtype {codes.dtype} not supported (int8 or uint8)")
+    if not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError("state8_values: tensors must be contiguous")
+    if scales.dtype != torch.float32 or scales.numel() != state8_blocks(codes.numel()):
+        raise ValueError(f"scales: one float32 scale for every {STATE8_BLOCK} codes")
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    check(_lib.load().dion_state8_values(codes.data_ptr(), int(codes.dtype == torch.uint8), scales.data_ptr(),
+                                         codes.numel(), out.data_ptr(), _dtype_code(out, "dtype"),
+                                         _stream_handle(codes.device)), "state8_values")
+    return out
 
 
 def lion_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Tensor, beta1: float, beta2: float,

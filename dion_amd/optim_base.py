@@ -120,8 +120,12 @@ class OrthoOptimizer(Optimizer):
 
     # ------------------------------------------------------------------ state
     def _create_state(self, group: dict) -> None:
+        bits = self._state_bits(group)
         for p in group["params"]:
-            self._get_or_initialize_state(p, group["algorithm"])
+            if bits is not None:
+                self._adamw_state(p, bits)
+            else:
+                self._get_or_initialize_state(p, group["algorithm"])
 
     def add_param_group(self, param_group: dict) -> None:
         """torch calls this from ``Optimizer.__init__`` for every group and users call it later; only a
@@ -141,6 +145,34 @@ class OrthoOptimizer(Optimizer):
         if algo == "adamw" and "step_dev" not in state:
             state["step_dev"] = torch.zeros((), dtype=torch.float32, device=param.device)
         return state
+
+    # ``state_bits`` of an AdamW group: its moments in 8 bits (codes and a float32 scale for every 128 elements) or in float32
+    # whatever the parameters' dtype; without it they have the parameters' dtype.
+    @staticmethod
+    def _state_bits(group: dict) -> Optional[int]:
+        bits = group.get("state_bits")
+        if bits is None:
+            return None
+        if isinstance(bits, bool) or bits not in (8, 32):
+            raise ValueError(f"state_bits: expected 8, 32 or None, got {bits!r}")
+        if group["algorithm"] != "adamw":
+            raise ValueError(f"state_bits is an option of adamw groups, not of {group['algorithm']!r} ones")
+        return bits
+
+    @staticmethod
+    def _adamw_state_dtypes(bits: int) -> Dict[str, torch.dtype]:
+        if bits == 32:
+            return {"momentum": torch.float32, "variance": torch.float32}
+        return {"momentum": torch.int8, "momentum_scale": torch.float32, "variance": torch.uint8,
+                "variance_scale": torch.float32}
+
+    def _adamw_state(self, param: Tensor, bits: int) -> dict:
+        state = self.state[param]
+        if not state:
+            for key, dtype in self._adamw_state_dtypes(bits).items():
+                state[key] = (torch.zeros(ops.state8_blocks(param.numel()), dtype=dtype, device=param.device)
+                              if key.endswith("_scale") else torch.zeros_like(param, dtype=dtype))
+        return self._get_or_initialize_state(param, "adamw")
 
     # ------------------------------------------------- live hyper-parameters
     def bind_live_scalars(self) -> None:
@@ -174,15 +206,32 @@ class OrthoOptimizer(Optimizer):
         self.bind_live_scalars()
         # AdamW's device step counter: float32 on the parameter's device whatever the checkpoint
         # held, and rebuilt from the group's host counter when the checkpoint predates it
-        for group in self.param_groups:
+        for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
             if group["algorithm"] != "adamw":
                 continue
+            bits = self._state_bits(group)
+            if bits is not None:
+                for p, pid in zip(group["params"], saved_group["params"]):
+                    self._restore_adamw_state(p, bits, state_dict["state"].get(pid))
             for p in group["params"]:
                 if p not in self.state:
                     continue
                 saved = self.state[p].get("step_dev")
                 value = float(group["step"]) if saved is None else float(saved)
                 self.state[p]["step_dev"] = torch.full((), value, dtype=torch.float32, device=p.device)
+
+    def _restore_adamw_state(self, param: Tensor, bits: int, saved: Optional[dict]) -> None:
+        """Moments as the checkpoint holds them: torch has cast them to the parameter's dtype, which loses the scales' last
+        bits and is not what the kernels read."""
+        if saved is None:
+            return
+        for key, dtype in self._adamw_state_dtypes(bits).items():
+            shape = (ops.state8_blocks(param.numel()),) if key.endswith("_scale") else tuple(param.shape)
+            value = saved.get(key)
+            if not isinstance(value, Tensor) or value.dtype != dtype or tuple(value.shape) != shape:
+                raise ValueError(f"state_bits={bits}: the checkpoint's {key!r} of a parameter of shape "
+                                 f"{tuple(param.shape)} is not a {dtype} tensor of shape {shape}")
+            self.state[param][key] = value.to(device=param.device, copy=True).contiguous()
 
     # ------------------------------------------------------------ validation
     # How a group's 2D weights are cut into independent matrices: ``num_heads`` equal row bands

@@ -34,11 +34,30 @@ def lion_step(opt, group: dict) -> None:
 def adamw_step(opt, group: dict) -> None:
     """Bias-corrected AdamW with decoupled (optionally cautious) weight decay
     (dion/scalar_opts.py:7-65); every parameter's step counter lives on the device in ``step_dev``
-    and is advanced there."""
+    and is advanced there.  ``state_bits`` 8 or 32: moments in 8 bits, or in float32 beside bfloat16 parameters
+    (``state_seed``: of the random rounding of 8-bit moments)."""
+    bits = opt._state_bits(group)
     for params in _with_grad(group).values():
+        if bits is not None:
+            _adamw_bits_step(opt, group, params, bits)
+            continue
         states = [opt._get_or_initialize_state(p, "adamw") for p in params]
         X = [p.data for p in params]
         G = [p.grad.contiguous() for p in params]
         ops.adamw_step(X, G, [s["momentum"] for s in states], [s["variance"] for s in states],
                        [s["step_dev"] for s in states], group["lr"], group["beta1"], group["beta2"],
                        group["weight_decay"], group["epsilon"], group.get("cautious_wd", False))
+
+
+def _adamw_bits_step(opt, group: dict, params, bits: int) -> None:
+    states = [opt._adamw_state(p, bits) for p in params]
+    X = [p.data for p in params]
+    G = [p.grad.contiguous() for p in params]
+    M, V, steps = ([s[key] for s in states] for key in ("momentum", "variance", "step_dev"))
+    rest = (steps, group["lr"], group["beta1"], group["beta2"], group["weight_decay"], group["epsilon"],
+            group.get("cautious_wd", False))
+    if bits == 32:
+        ops.adamw_step(X, G, M, V, *rest)
+    else:
+        ops.adamw8_step(X, G, M, [s["momentum_scale"] for s in states], V, [s["variance_scale"] for s in states], *rest,
+                        group.get("state_seed", 0))

@@ -446,6 +446,30 @@ int dion_adamw_step(const uint64_t* X_ptrs, const uint64_t* G_ptrs, int g_dtype,
                     const float* lr_dev, float beta1, float beta2, float eps, const float* wd_dev,
                     float wd_host, int cautious, void* stream);
 
+/* The same with M and V in fp32 whatever the parameters' type (x_dtype: DION_BF16 or DION_F32). */
+int dion_adamw_fp32_state_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype,
+                               const uint64_t* M_ptrs, const uint64_t* V_ptrs, const uint64_t* step_ptrs,
+                               const int64_t* numels, int n, const float* lr_dev, float beta1, float beta2,
+                               float eps, const float* wd_dev, float wd_host, int cautious, void* stream);
+
+/* The same with M and V in 8 bits, in blocks of 128 consecutive elements of a tensor (the last one may be shorter):
+ *   m = c s,      c int8  (M_ptrs), s fp32 per block (M_scale_ptrs: ceil(numel / 128) each), s = max |m| / 127
+ *   v = (k q)^2,  k uint8 (V_ptrs), q fp32 per block (V_scale_ptrs),                         q = max sqrt(v) / 255
+ * The update is computed in fp32 from the decoded moments; the new ones are rounded up or down at random, without bias in
+ * m and in v, by u = ((h + j 0x9E3779B9) mod 2^32 >> 8) 2^-24 for element 8 i + j of a tensor, h = mix(key ^ i), key =
+ * mix(mix(seed) + step) (mix: adamw8.hip):  c = floor(m / s + u);  k = floor(t), t = sqrt(v) / q, or one more where
+ * u (2 k + 1) < t^2 - k^2.  v > 0 keeps k >= 1.  Zeroed codes and scales are the state before the first step.  First moments of a
+ * block whose largest is below 1e-30, and second ones below 1e-60, become zero; a value that is not finite makes the scale of
+ * its block NaN.  Codes, parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
+int dion_adamw8_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype, const uint64_t* M_ptrs,
+                     const uint64_t* M_scale_ptrs, const uint64_t* V_ptrs, const uint64_t* V_scale_ptrs,
+                     const uint64_t* step_ptrs, const int64_t* numels, int n, const float* lr_dev, float beta1,
+                     float beta2, float eps, const float* wd_dev, float wd_host, int cautious, int seed, void* stream);
+
+/* out[i] = codes[i] scales[i / 128] of int8 codes, or (squared) the square of that of uint8 codes; out bf16 or fp32. */
+int dion_state8_values(const void* codes, int squared, const float* scales, int64_t numel, void* out, int out_dtype,
+                       void* stream);
+
 /* Lion:  U = sign(lerp(M, G, 1-beta1)); M = lerp(M, G, 1-beta2);
  *   X = X (1 - lr wd)   [cautious: X -= X [U X >= 0] lr wd];   X -= lr U
  * Replaces lion_update / lion_update_foreach (dion/scalar_opts.py:68-118, :271-325). */
