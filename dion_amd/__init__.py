@@ -11,6 +11,7 @@ from .newton_schulz import (  # noqa: F401
     zeropower_via_newtonschulz5,
 )
 
+from .linear import linear  # noqa: E402,F401
 from .hip_graph import CudaGraphOptimizer, HipGraphOptimizer  # noqa: E402,F401
 from .optimizers import Dion2, Dion3, Muon, NorDion2, NorMuon  # noqa: E402,F401
 
@@ -23,6 +24,7 @@ __all__ = [
     "HipGraphOptimizer",
     "CudaGraphOptimizer",
     "gram_newton_schulz",
+    "linear",
     "newton_schulz_triton",
     "ns_line_1",
     "ns_line_2",

@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libdion_hip.so")
 DION_BF16 = 0
 DION_F32 = 1
 DION_NS_GRAM = 1
+DION_LINEAR_COPY_X, DION_LINEAR_COPY_W, DION_LINEAR_COPY_DY = 1, 2, 4
 DION_NS_STATIC_SCRATCH_BYTES = 64 << 20
 ABI_VERSION = 15  # dion_abi_version() of the library these signatures describe
 
@@ -102,6 +103,11 @@ SIGNATURES = {
     "dion_dion2_post_masked": (c_int, [_u64p, _u64p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_float, c_float,
                                        c_void_p]),
+    "dion_linear_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "dion_linear_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p,
+                                    c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dion_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "dion_adamw_step": (c_int, [_u64p, _u64p, c_int, _u64p, _u64p, c_int, _u64p, _i64p, c_int, c_void_p, c_float,
                                 c_float, c_float, c_void_p, c_float, c_int, c_void_p]),
     "dion_adamw_fp32_state_step": (c_int, [_u64p, c_int, _u64p, c_int, _u64p, _u64p, _u64p, _i64p, c_int, c_void_p,

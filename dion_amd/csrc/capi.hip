@@ -9,6 +9,7 @@
 
 #include "../../include/dion_hip.h"
 #include "elementwise.h"
+#include "linear.h"
 
 using namespace dion;
 
@@ -1890,6 +1891,197 @@ extern "C" int dion_lion_step(const uint64_t* X_ptrs, const uint64_t* G_ptrs, in
                            lr_dev, beta1,
                            beta2, wd_dev, wd_host, cautious, (hipStream_t)stream),
             "dion_lion_step");
+  }
+  return DION_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// The product of a weight and its gradients
+// ---------------------------------------------------------------------------------------------
+static int round8(int v) { return (v + 7) & ~7; }
+
+// Whether the kernels read a [rows][cols] operand where it lies.
+static bool lin_whole(const void* p, int64_t ld, int cols) {
+  return aligned16((uint64_t)(uintptr_t)p) && ld % 8 == 0 && cols % 8 == 0 && ld <= kLinMaxLd;
+}
+
+// Places in the workspace of a call, 256-byte aligned; `copies`: DION_LINEAR_COPY_* bits.
+struct LinSpace {
+  size_t x, w, dz, sums, scratch, total;
+};
+static LinSpace lin_space(int tokens, int fan_in, int fan_out, int backward, int activation, int copies) {
+  LinSpace s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  const int kp = round8(fan_in), np = round8(fan_out);
+  s.x = take(copies & DION_LINEAR_COPY_X ? (size_t)tokens * kp * 2 : 0);
+  s.w = take(copies & DION_LINEAR_COPY_W ? (size_t)fan_out * kp * 2 : 0);
+  s.dz = s.sums = at;
+  size_t scratch;
+  if (backward) {
+    s.dz = take((copies & DION_LINEAR_COPY_DY) || activation ? (size_t)tokens * np * 2 : 0);
+    s.sums = take(tokens > 0 ? (size_t)lin_sum_parts(tokens) * fan_out * sizeof(float) : 0);
+    const size_t a = lin_product_scratch(tokens, fan_in, fan_out, 0, 1), b = lin_product_scratch(fan_out, fan_in, tokens, 1, 1);
+    scratch = a > b ? a : b;  // (the two products run one after the other)
+  } else {
+    scratch = lin_product_scratch(tokens, fan_out, fan_in, 0, 0);
+  }
+  s.scratch = take(scratch);
+  s.total = at;
+  return s;
+}
+
+static int check_linear(const char* who, int tokens, int fan_in, int fan_out, int activation) {
+  if (tokens < 0 || fan_in < 1 || fan_out < 1)
+    return fail(DION_E_INVALID, "%s: %d tokens, %d x %d weight", who, tokens, fan_out, fan_in);
+  if (tokens > (1 << 30) || fan_in > kLinMaxLd - 8 || fan_out > kLinMaxLd - 8)
+    return fail(DION_E_INVALID, "%s: more than 2^30 tokens or features past 2^22 - 8", who);
+  if (activation < 0 || activation >= kActCount) return fail(DION_E_INVALID, "%s: activation %d", who, activation);
+  return DION_OK;
+}
+
+static int check_lin_rows(const char* who, const char* arg, const void* p, int64_t ld, int rows, int cols) {
+  if (rows > 0 && !p) return fail(DION_E_INVALID, "%s: %s is null", who, arg);
+  if ((uintptr_t)p & 1) return fail(DION_E_INVALID, "%s: %s is not 2-byte aligned", who, arg);
+  if (rows > 1 && ld < cols)
+    return fail(DION_E_INVALID, "%s: rows of %s overlap (%lld elements apart, %d long)", who, arg, (long long)ld, cols);
+  return DION_OK;
+}
+
+extern "C" size_t dion_linear_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int activation, int copies) {
+  if (check_linear("dion_linear_workspace_bytes", tokens, fan_in, fan_out, activation)) return 0;
+  return lin_space(tokens, fan_in, fan_out, backward, activation, copies).total;
+}
+
+extern "C" int dion_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                                   int activation, const void* residual, int64_t ldr, void* y, void* slope, int tokens,
+                                   int fan_in, int fan_out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dion_linear_forward";
+  if (int rc = check_linear(who, tokens, fan_in, fan_out, activation)) return rc;
+  if (bias && bias_dtype != DION_BF16 && bias_dtype != DION_F32) return fail(DION_E_INVALID, "%s: bias_dtype", who);
+  if (tokens == 0) return DION_OK;
+  if (int rc = check_lin_rows(who, "x", x, ldx, tokens, fan_in)) return rc;
+  if (int rc = check_lin_rows(who, "w", w, ldw, fan_out, fan_in)) return rc;
+  if (residual)
+    if (int rc = check_lin_rows(who, "residual", residual, ldr, tokens, fan_out)) return rc;
+  if (!y) return fail(DION_E_INVALID, "%s: y is null", who);
+  if (slope && activation == kActNone) return fail(DION_E_INVALID, "%s: slopes without an activation", who);
+  const int copies = (lin_whole(x, ldx, fan_in) ? 0 : DION_LINEAR_COPY_X) | (lin_whole(w, ldw, fan_in) ? 0 : DION_LINEAR_COPY_W);
+  const LinSpace s = lin_space(tokens, fan_in, fan_out, 0, activation, copies);
+  if (s.total > 0 && (!workspace || workspace_bytes < s.total || !aligned16((uint64_t)(uintptr_t)workspace)))
+    return fail(DION_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, s.total, workspace_bytes);
+  char* ws = (char*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  LinProduct p;
+  memset(&p, 0, sizeof(p));
+  p.P = (const bf16_t*)x;
+  p.ldp = ldx;
+  p.Q = (const bf16_t*)w;
+  p.ldq = ldw;
+  if (copies & DION_LINEAR_COPY_X) {
+    HIP_TRY(launch_lin_prepare(p.P, ldx, nullptr, 0, tokens, fan_in, (bf16_t*)(ws + s.x), nullptr, st), who);
+    p.P = (const bf16_t*)(ws + s.x);
+    p.ldp = round8(fan_in);
+  }
+  if (copies & DION_LINEAR_COPY_W) {
+    HIP_TRY(launch_lin_prepare(p.Q, ldw, nullptr, 0, fan_out, fan_in, (bf16_t*)(ws + s.w), nullptr, st), who);
+    p.Q = (const bf16_t*)(ws + s.w);
+    p.ldq = round8(fan_in);
+  }
+  p.M = tokens;
+  p.N = fan_out;
+  p.K = fan_in;
+  p.C = (bf16_t*)y;
+  p.act = activation;
+  p.bias = bias;
+  p.bias_dtype = dt(bias_dtype);
+  p.R = (const bf16_t*)residual;
+  p.ldr = ldr;
+  p.slope = (uint16_t*)slope;
+  p.scratch = (float*)(ws + s.scratch);
+  HIP_TRY(launch_lin_product(p, st), who);
+  return DION_OK;
+}
+
+extern "C" int dion_linear_backward(const void* dy, int64_t lddy, const void* slope, int activation, const void* x, int64_t ldx,
+                                    const void* w, int64_t ldw, void* dx, void* dw, void* db, int db_dtype, int tokens,
+                                    int fan_in, int fan_out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dion_linear_backward";
+  if (int rc = check_linear(who, tokens, fan_in, fan_out, activation)) return rc;
+  if (db && db_dtype != DION_BF16 && db_dtype != DION_F32) return fail(DION_E_INVALID, "%s: db_dtype", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (tokens == 0) {
+    // sums over nothing
+    const int64_t all = (int64_t)fan_out * fan_in;
+    for (int64_t at = 0; dw && at < all; at += 1 << 30)
+      HIP_TRY(launch_lin_sum(nullptr, 0, (int)(all - at < (1 << 30) ? all - at : 1 << 30), (bf16_t*)dw + at, 0, st), who);
+    if (db) HIP_TRY(launch_lin_sum(nullptr, 0, fan_out, db, dt(db_dtype), st), who);
+    return DION_OK;
+  }
+  if (int rc = check_lin_rows(who, "dy", dy, lddy, tokens, fan_out)) return rc;
+  if (dw)
+    if (int rc = check_lin_rows(who, "x", x, ldx, tokens, fan_in)) return rc;
+  if (dx)
+    if (int rc = check_lin_rows(who, "w", w, ldw, fan_out, fan_in)) return rc;
+  if ((activation != kActNone) != (slope != nullptr))
+    return fail(DION_E_INVALID, "%s: slopes go with an activation, and none without", who);
+  const int copies = (dw && !lin_whole(x, ldx, fan_in) ? DION_LINEAR_COPY_X : 0) |
+                     (dx && !lin_whole(w, ldw, fan_in) ? DION_LINEAR_COPY_W : 0) |
+                     (lin_whole(dy, lddy, fan_out) ? 0 : DION_LINEAR_COPY_DY);
+  const LinSpace s = lin_space(tokens, fan_in, fan_out, 1, activation, copies);
+  if (s.total > 0 && (!workspace || workspace_bytes < s.total || !aligned16((uint64_t)(uintptr_t)workspace)))
+    return fail(DION_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, s.total, workspace_bytes);
+  char* ws = (char*)workspace;
+  const bf16_t *pdz = (const bf16_t*)dy, *px = (const bf16_t*)x, *pw = (const bf16_t*)w;
+  int64_t lddz = lddy;
+  // dz = dy act'(z) and its column sums in one pass
+  const bool product = dx || dw, need_dz = product && (slope || (copies & DION_LINEAR_COPY_DY));
+  if (need_dz || db) {
+    HIP_TRY(launch_lin_prepare(pdz, lddy, (const uint16_t*)slope, activation, tokens, fan_out,
+                               need_dz ? (bf16_t*)(ws + s.dz) : nullptr, db ? (float*)(ws + s.sums) : nullptr, st), who);
+    if (db) HIP_TRY(launch_lin_sum((const float*)(ws + s.sums), lin_sum_parts(tokens), fan_out, db, dt(db_dtype), st), who);
+  }
+  if (need_dz) {
+    pdz = (const bf16_t*)(ws + s.dz);
+    lddz = round8(fan_out);
+  }
+  if (copies & DION_LINEAR_COPY_X) {
+    HIP_TRY(launch_lin_prepare(px, ldx, nullptr, 0, tokens, fan_in, (bf16_t*)(ws + s.x), nullptr, st), who);
+    px = (const bf16_t*)(ws + s.x);
+    ldx = round8(fan_in);
+  }
+  if (copies & DION_LINEAR_COPY_W) {
+    HIP_TRY(launch_lin_prepare(pw, ldw, nullptr, 0, fan_out, fan_in, (bf16_t*)(ws + s.w), nullptr, st), who);
+    pw = (const bf16_t*)(ws + s.w);
+    ldw = round8(fan_in);
+  }
+  LinProduct p;
+  memset(&p, 0, sizeof(p));
+  p.scratch = (float*)(ws + s.scratch);
+  p.P = pdz;
+  p.ldp = lddz;
+  p.q_kmajor = 1;
+  p.N = fan_in;
+  if (dx) {
+    p.Q = pw;
+    p.ldq = ldw;
+    p.M = tokens;
+    p.K = fan_out;
+    p.C = (bf16_t*)dx;
+    HIP_TRY(launch_lin_product(p, st), who);
+  }
+  if (dw) {
+    p.p_kmajor = 1;
+    p.Q = px;
+    p.ldq = ldx;
+    p.M = fan_out;
+    p.K = tokens;
+    p.C = (bf16_t*)dw;
+    HIP_TRY(launch_lin_product(p, st), who);
   }
   return DION_OK;
 }

@@ -44,6 +44,22 @@ def _dtype_code(t: Tensor, name: str) -> int:
     raise TypeError(f"{name}: dtype {t.dtype} not supported (bfloat16 or float32)")
 
 
+class _SameDevice:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _device_of(t: Tensor):
+    """Context in which the current device is that of ``t``."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 _workspaces = {}
 
 
@@ -1005,3 +1021,107 @@ def lion_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Tensor, bet
     lib = _lib.load()
     check(lib.dion_lion_step(xp, gp, gcode, mp, scode, numels, len(X), lr_p, float(beta1), float(beta2), wd_p, wd_h,
                              int(bool(cautious_wd)), _stream_handle(X[0].device)), "lion_step")
+
+
+# ---------------------------------------------------------------------------------------------
+# the product of a weight and its gradients
+# ---------------------------------------------------------------------------------------------
+ACTIVATIONS = {None: 0, "relu": 1, "relu_squared": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
+
+
+def _rows(t: Tensor) -> Tuple[Tensor, int]:
+    """A 2D tensor whose rows are dense and do not overlap (itself, or a copy), and the elements between them."""
+    rows, cols = t.shape
+    if t.stride(1) != 1 and cols > 1 or rows > 1 and t.stride(0) < cols:
+        t = t.contiguous()
+    return t, (t.stride(0) if rows > 1 else cols)
+
+
+def _whole_chunks(t: Tensor, ld: int) -> bool:
+    return t.data_ptr() % 16 == 0 and ld % 8 == 0 and t.shape[1] % 8 == 0 and ld <= 1 << 22
+
+
+def _check_linear(name: str, t: Tensor, shape, device, dtypes=(torch.bfloat16,)) -> None:
+    _require_gpu(t, name)
+    if t.device != device:
+        raise ValueError(f"linear: {name} is on {t.device}, x on {device}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"linear: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"linear: expected {name} of shape {shape}, got {tuple(t.shape)}")
+
+
+def check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
+                 residual: Optional[Tensor]) -> None:
+    """Raises for what ``linear_forward`` does not take (``x`` of any number of dimensions)."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"linear: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear: x of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
+    if weight.numel() == 0:
+        raise ValueError(f"linear: empty weight of shape {tuple(weight.shape)}")
+    _check_linear("x", x, tuple(x.shape), x.device)
+    _check_linear("weight", weight, tuple(weight.shape), x.device)
+    if bias is not None:
+        _check_linear("bias", bias, (weight.shape[0],), x.device, (torch.bfloat16, torch.float32))
+    if residual is not None:
+        _check_linear("residual", residual, (*x.shape[:-1], weight.shape[0]), x.device)
+
+
+def _linear_space(tokens: int, weight: Tensor, backward: bool, act: int, copies: int) -> Tuple[Optional[Tensor], int]:
+    # (the caching allocator's: a captured graph has its own, and no two calls in flight share one)
+    nbytes = _lib.load().dion_linear_workspace_bytes(tokens, weight.shape[1], weight.shape[0], int(backward), act, copies)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=weight.device) if nbytes else None), nbytes
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
+                   residual: Optional[Tensor], keep_slope: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """``act(x W^T + b) + residual`` of 2D ``x`` and ``residual``, and with ``keep_slope`` act' at every element, in the 16
+    bits that ``linear_backward`` reads."""
+    act = ACTIVATIONS[activation]
+    tokens, fan_out = x.shape[0], weight.shape[0]
+    with _device_of(x):
+        y = torch.empty(tokens, fan_out, dtype=torch.bfloat16, device=x.device)
+        slope = torch.empty(tokens, fan_out, dtype=torch.int16, device=x.device) if keep_slope and act else None
+        (x, ldx), (w, ldw) = _rows(x), _rows(weight)
+        r, ldr = (None, 0) if residual is None else _rows(residual)
+        b = None if bias is None else bias.contiguous()
+        copies = (0 if _whole_chunks(x, ldx) else _lib.DION_LINEAR_COPY_X) | (0 if _whole_chunks(w, ldw) else _lib.DION_LINEAR_COPY_W)
+        ws, nbytes = _linear_space(tokens, weight, False, act, copies)
+        check(_lib.load().dion_linear_forward(x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b),
+                                              DION_BF16 if b is None else _dtype_code(b, "bias"), act, _ptr(r), ldr,
+                                              y.data_ptr(), _ptr(slope), tokens, weight.shape[1], fan_out, _ptr(ws), nbytes,
+                                              _stream_handle(x.device)), "linear")
+    return y, slope
+
+
+def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
+                    weight: Tensor, need_dx: bool, need_dw: bool,
+                    bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients ``(dx, dW, db)`` of ``linear_forward``, None where not asked for (``bias_dtype`` None: no ``db``).  ``x`` is
+    read for ``dW``, the weight for ``dx``."""
+    act = ACTIVATIONS[activation]
+    fan_out, fan_in = weight.shape
+    tokens = dy.shape[0]
+    with _device_of(dy):
+        dy, lddy = _rows(dy)
+        copies = 0 if _whole_chunks(dy, lddy) else _lib.DION_LINEAR_COPY_DY
+        xr, ldx = _rows(x) if need_dw else (None, 0)
+        w, ldw = _rows(weight) if need_dx else (None, 0)
+        if need_dw and not _whole_chunks(xr, ldx):
+            copies |= _lib.DION_LINEAR_COPY_X
+        if need_dx and not _whole_chunks(w, ldw):
+            copies |= _lib.DION_LINEAR_COPY_W
+        ws, nbytes = _linear_space(tokens, weight, True, act, copies)
+        new = lambda *shape, dtype=torch.bfloat16: torch.empty(shape, dtype=dtype, device=dy.device)  # noqa: E731
+        dx = new(tokens, fan_in) if need_dx else None
+        dw = new(fan_out, fan_in) if need_dw else None
+        db = new(fan_out, dtype=bias_dtype) if bias_dtype is not None else None
+        check(_lib.load().dion_linear_backward(dy.data_ptr(), lddy, _ptr(slope), act, _ptr(xr), ldx, _ptr(w), ldw, _ptr(dx),
+                                               _ptr(dw), _ptr(db), DION_BF16 if db is None else _dtype_code(db, "bias"), tokens,
+                                               fan_in, fan_out, _ptr(ws), nbytes, _stream_handle(dy.device)), "linear backward")
+    return dx, dw, db

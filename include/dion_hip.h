@@ -428,6 +428,34 @@ int dion_dion2_post_masked(const uint64_t* X_ptrs, const uint64_t* M_ptrs, int s
                            void* stream);
 
 /* --------------------------------------------------------------------------------------------
+ * The product a weight matrix stands for, and its gradients.  Row-major bf16 matrices, `ld*` elements between their rows:
+ * x [tokens][fan_in], w [fan_out][fan_in], residual and dy [tokens][fan_out]; results are dense.  bias, db [fan_out], bf16 or
+ * fp32 (DION_BF16 / DION_F32).  Sums are fp32; a result is rounded once.  Any sizes and alignments of a multiple of an element;
+ * operands whose rows are not whole 16-byte chunks (address, distance and length) are copied into the workspace first.
+ * ------------------------------------------------------------------------------------------ */
+enum { DION_ACT_NONE, DION_ACT_RELU, DION_ACT_RELU_SQUARED, DION_ACT_GELU, DION_ACT_GELU_TANH, DION_ACT_SILU };
+
+/* Bytes of workspace a call uses.  copies: DION_LINEAR_COPY_* of the operands whose rows are not whole chunks (all of them: an
+ * upper bound).  Nothing has to be kept between calls; calls that overlap need one each. */
+#define DION_LINEAR_COPY_X 1
+#define DION_LINEAR_COPY_W 2
+#define DION_LINEAR_COPY_DY 4
+size_t dion_linear_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int activation, int copies);
+
+/* y = act(x w^T + bias) + residual.  bias, residual may be null.  slope (null, or [tokens][fan_out] of 16 bits; not without an
+ * activation): act' at every element, for dion_linear_backward -- fp16, of the squared relu seven bits of exponent and
+ * nine of mantissa.  Neither y nor slope may overlap an operand, but y may be the residual where that is dense. */
+int dion_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
+                        int activation, const void* residual, int64_t ldr, void* y, void* slope, int tokens, int fan_in,
+                        int fan_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dz = dy act' (rounded to bf16 for the products, not for db):  dx = dz w,  dw = dz^T x,  db = sum of dz over the tokens.
+ * dx, dw, db may be null; x is read for dw, w for dx, slope with an activation.  (The residual's gradient is dy.) */
+int dion_linear_backward(const void* dy, int64_t lddy, const void* slope, int activation, const void* x, int64_t ldx,
+                         const void* w, int64_t ldw, void* dx, void* dw, void* db, int db_dtype, int tokens, int fan_in,
+                         int fan_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------------------------------------------------
  * Multi-tensor AdamW / Lion for the non-matrix parameter groups (algorithm "adamw" / "lion").
  * X_ptrs, G_ptrs, M_ptrs, V_ptrs: host ptr tables of n device pointers; tensor i has numels[i]
  * elements (host array); X, M, V share s_dtype, G bf16 or fp32 per g_dtype (one dtype each per call).
