@@ -1939,7 +1939,7 @@ static int check_linear(const char* who, int tokens, int fan_in, int fan_out, in
   if (tokens < 0 || fan_in < 1 || fan_out < 1)
     return fail(DION_E_INVALID, "%s: %d tokens, %d x %d weight", who, tokens, fan_out, fan_in);
   if (tokens > (1 << 30) || fan_in > kLinMaxLd - 8 || fan_out > kLinMaxLd - 8)
-    return fail(DION_E_INVALID, "%s: more than 2^30 tokens or features past 2^22 - 8", who);
+    return fail(DION_E_INVALID, "%s: more than 2^30 tokens or features past 2^21 - 8", who);
   if (activation < 0 || activation >= kActCount) return fail(DION_E_INVALID, "%s: activation %d", who, activation);
   return DION_OK;
 }

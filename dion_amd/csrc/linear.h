@@ -26,7 +26,7 @@ struct LinProduct {
   // partial sums of a split reduction: lin_product_scratch(...) bytes
   float* scratch;
 };
-constexpr int64_t kLinMaxLd = int64_t(1) << 22;
+constexpr int64_t kLinMaxLd = int64_t(1) << 21;
 
 size_t lin_product_scratch(int M, int N, int K, int p_kmajor, int q_kmajor);
 hipError_t launch_lin_product(const LinProduct& p, hipStream_t st);

@@ -9,8 +9,6 @@
 // kept in fp16 (eleven bits); those of the squared relu, 2 max(z, 0), have no sign and no bound, and are kept as seven bits of
 // exponent and nine of mantissa, from 2^-63 to where z^2 leaves fp32.  bf16's eight bits would add an error of the size of
 // the rounding of dz itself; so it stays an eighth (a quarter) of that, for the same bytes.
-#include <hip/hip_fp16.h>
-
 #include <atomic>
 
 #include "gemm_tile.h"
@@ -23,45 +21,59 @@ static __device__ __forceinline__ float rcp_fast(float v) { return __builtin_amd
 
 // act(z), and act'(z) in `slope`.  Exponentials and quotients by the hardware's approximations (1 ulp): the result is rounded
 // to bf16, the slope to eleven bits.
-static __device__ __forceinline__ float activate(int act, float z, float& slope) {
-  switch (act) {
-    case kActRelu:
-      slope = z > 0.f ? 1.f : 0.f;
-      return z < 0.f ? 0.f : z;  // (NaN stays)
-    case kActReluSquared: {
-      const float r = z < 0.f ? 0.f : z;
-      slope = 2.f * r;
-      return r * r;
-    }
-    case kActSilu: {
-      const float s = rcp_fast(1.f + __expf(-z));
-      slope = s * (1.f + z * (1.f - s));
-      return z * s;
-    }
-    case kActGelu: {
-      const float cdf = 0.5f * (1.f + erff(z * 0.70710678f));
-      slope = cdf + z * 0.39894228f * __expf(-0.5f * z * z);
-      return z * cdf;
-    }
-    case kActGeluTanh: {
-      const float u = 0.79788456f * z * (1.f + 0.044715f * z * z);
-      const float t = 1.f - 2.f * rcp_fast(1.f + __expf(2.f * u));
-      slope = 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456f * (1.f + 0.134145f * z * z);
-      return 0.5f * z * (1.f + t);
-    }
-    default:
-      slope = 1.f;
-      return z;
+template <int ACT>
+static __device__ __forceinline__ float activate(float z, float& slope) {
+  if constexpr (ACT == kActRelu) {
+    slope = z > 0.f ? 1.f : 0.f;
+    return z < 0.f ? 0.f : z;  // (NaN stays)
+  } else if constexpr (ACT == kActReluSquared) {
+    const float r = z < 0.f ? 0.f : z;
+    slope = 2.f * r;
+    return r * r;
+  } else if constexpr (ACT == kActSilu) {
+    const float s = rcp_fast(1.f + __expf(-z));
+    slope = s * (1.f + z * (1.f - s));
+    return z * s;
+  } else if constexpr (ACT == kActGelu) {
+    // The normal distribution's upper tail at a = |z| is exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.3 a), P fitted to it with a
+    // relative error of 1.5e-7 (5e-7 in fp32) up to a = 14, where fp32 ends: one exponential for the tail and the density.
+    const float a = fabsf(z), t = rcp_fast(1.f + 0.3f * a), e = __expf(-0.5f * z * z);
+    float q = 0.03567495f;
+    q = fmaf(q, t, -0.15720376f);
+    q = fmaf(q, t, 0.20635456f);
+    q = fmaf(q, t, -0.053684533f);
+    q = fmaf(q, t, 0.12856206f);
+    q = fmaf(q, t, 0.09991337f);
+    q = fmaf(q, t, 0.12075397f);
+    q = fmaf(q, t, 0.1196293f);
+    const float tail = q * t * e;
+    const float cdf = z > 0.f ? 1.f - tail : tail;
+    slope = cdf + z * 0.39894228f * e;
+    return z * cdf;
+  } else if constexpr (ACT == kActGeluTanh) {
+    const float u = 0.79788456f * z * (1.f + 0.044715f * z * z);
+    const float s = rcp_fast(1.f + __expf(-2.f * u));  // (1 + tanh u) / 2
+    slope = s + 2.f * z * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z * z);
+    return z * s;
+  } else {
+    slope = 1.f;
+    return z;
   }
 }
 
-static __device__ __forceinline__ uint16_t slope_pack(int act, float s) {
-  if (act != kActReluSquared) return __builtin_bit_cast(uint16_t, (_Float16)s);
-  // Round to nine bits of mantissa; code 0 is zero, 0xffff NaN and everything past 2^65.
-  const uint32_t b = __float_as_uint(s) + 0x2000u;
-  if (b < (64u << 23) + (1u << 14)) return 0;
-  const uint32_t c = (b >> 14) - (64u << 9);
-  return c > 0xffffu ? 0xffffu : (uint16_t)c;
+// Two slopes as the forward pass keeps them.
+template <int ACT>
+static __device__ __forceinline__ uint32_t slope_pack2(float a, float b) {
+  if constexpr (ACT != kActReluSquared) {
+    return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+  } else {
+    // Rounded to nine bits of mantissa; code 0 is zero (and 2^-63 and below), 0xffff NaN and everything past 2^65.
+    auto code = [](float s) {
+      const uint32_t c = (__float_as_uint(s) + 0x2000u) >> 14;
+      return min(c > (64u << 9) ? c - (64u << 9) : 0u, 0xffffu);
+    };
+    return code(a) | code(b) << 16;
+  }
 }
 static __device__ __forceinline__ float slope_unpack(int act, uint16_t c) {
   if (act != kActReluSquared) return (float)__builtin_bit_cast(_Float16, c);
@@ -77,7 +89,7 @@ struct LinEpilogue {
   uint16_t* slope;
   int64_t ldr;
   int M, N, act, bias_dtype;
-  int vec;  // N, ldr and the addresses allow 8-byte accesses to four neighbours
+  int vec;  // 8, 4, 2, 1: neighbours of a row that N, ldr and the addresses allow to be moved at once
 };
 
 // Bias of columns col .. col + 3.
@@ -95,67 +107,83 @@ static __device__ __forceinline__ uint2 residual4(const LinEpilogue& p, int row,
   uint2 w = make_uint2(0, 0);
   if (!p.R || row >= p.M || col >= p.N) return w;
   const bf16_t* r = p.R + (int64_t)row * p.ldr + col;
-  if (p.vec) return *(const uint2*)r;
+  if (p.vec >= 4) return *(const uint2*)r;
+  if (p.vec == 2) {
+    w.x = *(const uint32_t*)r;
+    if (col + 2 < p.N) w.y = *(const uint32_t*)(r + 2);
+    return w;
+  }
   w.x = r[0];
   if (col + 1 < p.N) w.x |= (uint32_t)r[1] << 16;
   if (col + 2 < p.N) w.y = r[2];
   if (col + 3 < p.N) w.y |= (uint32_t)r[3] << 16;
   return w;
 }
-// Finishes and stores elements (row, col .. col + 3).  ACT: an activation may be there.
-template <bool ACT>
-static __device__ __forceinline__ void finish4(const LinEpilogue& p, int row, int col, f32x4 z, f32x4 b, uint2 r) {
-  if (row >= p.M || col >= p.N) return;
+// Stores four 16-bit elements of a row, as far as it goes.
+static __device__ __forceinline__ void store4(const LinEpilogue& p, uint16_t* o, int col, uint2 w) {
+  if (p.vec >= 4) {
+    *(uint2*)o = w;
+  } else if (p.vec == 2) {
+    *(uint32_t*)o = w.x;
+    if (col + 2 < p.N) *(uint32_t*)(o + 2) = w.y;
+  } else {
+    o[0] = (uint16_t)w.x;
+    if (col + 1 < p.N) o[1] = (uint16_t)(w.x >> 16);
+    if (col + 2 < p.N) o[2] = (uint16_t)w.y;
+    if (col + 3 < p.N) o[3] = (uint16_t)(w.y >> 16);
+  }
+}
+// Four sums of a row as they are stored, y and the slopes.
+template <int ACT, bool SLOPE>
+static __device__ __forceinline__ void finish4(const LinEpilogue& p, f32x4 z, f32x4 b, uint2 r, uint2& y, uint2& slopes) {
   float v[4], s[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = z[e] + b[e];
-    if constexpr (ACT) v[e] = activate(p.act, v[e], s[e]);
-  }
-  const int64_t at = (int64_t)row * p.N + col;
-  if constexpr (ACT) {
-    if (p.slope) {
-      uint16_t c[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = slope_pack(p.act, s[e]);
-      if (p.vec) {
-        *(uint2*)(p.slope + at) = make_uint2(c[0] | (uint32_t)c[1] << 16, c[2] | (uint32_t)c[3] << 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < p.N) p.slope[at + e] = c[e];
-      }
-    }
-  }
+  for (int e = 0; e < 4; ++e) v[e] = activate<ACT>(z[e] + b[e], s[e]);
+  if constexpr (SLOPE) slopes = make_uint2(slope_pack2<ACT>(s[0], s[1]), slope_pack2<ACT>(s[2], s[3]));
   if (p.R) {
     v[0] += __uint_as_float(r.x << 16);
     v[1] += __uint_as_float(r.x & 0xffff0000u);
     v[2] += __uint_as_float(r.y << 16);
     v[3] += __uint_as_float(r.y & 0xffff0000u);
   }
-  if (p.vec) {
-    *(uint2*)(p.C + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < p.N) p.C[at + e] = f32_to_bf16(v[e]);
+  y = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+// Finishes and stores elements (row, col .. col + 3), where the activation is not worth a kernel of its own.
+static __device__ __forceinline__ void finish4_any(const LinEpilogue& p, int row, int col, f32x4 z) {
+  if (row >= p.M || col >= p.N) return;
+  const f32x4 b = bias4(p, col);
+  const uint2 r = residual4(p, row, col);
+  uint2 y, s;
+  switch (p.act) {
+    case kActRelu: finish4<kActRelu, true>(p, z, b, r, y, s); break;
+    case kActReluSquared: finish4<kActReluSquared, true>(p, z, b, r, y, s); break;
+    case kActGelu: finish4<kActGelu, true>(p, z, b, r, y, s); break;
+    case kActGeluTanh: finish4<kActGeluTanh, true>(p, z, b, r, y, s); break;
+    case kActSilu: finish4<kActSilu, true>(p, z, b, r, y, s); break;
+    default: finish4<kActNone, true>(p, z, b, r, y, s); break;
   }
+  const int64_t at = (int64_t)row * p.N + col;
+  if (p.slope) store4(p, p.slope + at, col, s);
+  store4(p, p.C + at, col, y);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int NS_>
 struct LinCfg {
-  static constexpr int BM = BM_, BN = BN_, BK = 64, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, BK = 64, WM = WM_, WN = WN_, NS = NS_;
   static constexpr int NT = WM * WN * 64;
   static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 16, TN = WTN / 16;
   static constexpr int HALVES = TM / 4, ST = BK / 32;
-  static constexpr int OP_BYTES = BM * BK * 2;  // one operand of one slab
-  static constexpr int LDS_BYTES = 4 * OP_BYTES;
-  static constexpr int OP_LOADS = OP_BYTES / (NT * 16);
-  static_assert(BM == BN && TN == 4 && (TM == 4 || TM == 8) && OP_LOADS == 4, "square tiles, wavefronts of 64 or 128 rows by 64 columns");
+  static constexpr int PB = BM * BK * 2, QB = BN * BK * 2;  // bytes of an operand's slab
+  static constexpr int RING_BYTES = NS * (PB + QB);
+  static constexpr int STG_BYTES = 16 * 128;  // a wavefront's staging: 16 rows of 64 16-bit elements
+  static constexpr int LDS_BYTES = RING_BYTES + WM * WN * STG_BYTES;
+  static constexpr int PL = PB / (NT * 16), QL = QB / (NT * 16), LPS = PL + QL;  // loads of a thread per slab
+  static_assert(TN == 4 && (TM == 4 || TM == 8) && LPS <= 8 && LDS_BYTES <= 160 * 1024, "wavefronts of 64 or 128 rows by 64 columns");
 };
-typedef LinCfg<256, 256, 2, 4> Lin256;  // 8 wavefronts: one workgroup per CU
-typedef LinCfg<128, 128, 2, 2> Lin128;  // 4 wavefronts: two workgroups per CU
+typedef LinCfg<256, 256, 2, 4, 2> Lin256;   // 8 wavefronts of 128 x 64
+typedef LinCfg<256, 128, 4, 2, 3> LinWide;  // 8 wavefronts of 64 x 64
+typedef LinCfg<128, 128, 2, 2, 4> Lin128;   // 4 wavefronts of 64 x 64
 
 // Issue order of the fragment reads behind the MFMAs, and how many LDS instructions may be outstanding when an MFMA issues (the
 // LDS returns in order).  A 32-deep step is HALVES halves of sixteen MFMAs (A fragment q / 4 against B fragment q % 4); while a half
@@ -189,126 +217,153 @@ struct LinTileParams {
   int ldp, ldq, K;
   float* part;  // [splits][M][N] sums, where the reduction is split
   int tilesM, tilesN, splits, slabs;  // slabs: of 64, per split
+  int total, grid;                    // tiles of the list, workgroups
   uint32_t inv_tiles, inv_group, inv_tail;
 };
 
-// One output tile (of one part of the reduction) per workgroup.  Operand slabs reach a two-slot LDS ring by direct-to-LDS
-// buffer loads, whose descriptors end where the matrix does: rows past an edge arrive as zeros, and need no padded copy.  Chunks
-// behind the reduction's end in the last slab of an operand with the reduction along rows get an offset past the end.  XOR
-// swizzles keep the LDS writes and the fragment reads free of bank conflicts.  The MFMA operands are swapped (B fragment
-// first), so that a lane's four sums are neighbours of one row of C: 8-byte accesses to C, the addend and the slopes.
+// One workgroup per CU walks a list of output tiles (of parts of the reduction).  Operand slabs reach a ring of NS slots in LDS
+// by direct-to-LDS buffer loads, whose descriptors end where the matrix does: rows past an edge arrive as zeros, and need no
+// padded copy.  Chunks behind the reduction's end in the last slab of an operand with the reduction along rows get an offset past
+// the end.  The ring runs on across tiles: the last slabs of one are computed while the first ones of the next arrive.
+// XOR swizzles keep the LDS writes and the fragment reads free of bank conflicts.  The MFMA operands are swapped (B
+// fragment first), so that a lane's four sums are neighbours of one row of C: 8-byte accesses to C, the addend and the slopes.
 // SPLIT: the sums of a part go to p.part as fp32, and lin_join_kernel finishes them.
-template <class Cfg, bool PK, bool QK, bool ACT, bool SPLIT>
+template <class Cfg, bool PK, bool QK, int ACT, bool SLOPE, bool SPLIT>
 __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParams p) {
   constexpr int BM = Cfg::BM, BN = Cfg::BN, BK = Cfg::BK, TM = Cfg::TM, TN = Cfg::TN, ST = Cfg::ST, HALVES = Cfg::HALVES;
-  constexpr int HP = HALVES * ST, OPB = Cfg::OP_BYTES, NT = Cfg::NT;
+  constexpr int HP = HALVES * ST, PB = Cfg::PB, QB = Cfg::QB, NT = Cfg::NT, NS = Cfg::NS, PL = Cfg::PL, QL = Cfg::QL, LPS = Cfg::LPS;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
 
-  // ---- which tile: every XCD gets one contiguous run of the list, eight rows of tiles at a time, columns first within them
-  int ti, tj, part;
-  {
-    const int total = gridDim.x, xcd = blockIdx.x & 7, q = total >> 3, r = total & 7;
-    const int lt = xcd * q + (xcd < r ? xcd : r) + (blockIdx.x >> 3);
-    int t, tg;
-    part = div_known(lt, p.tilesM * p.tilesN, p.inv_tiles, t);
-    const int first = div_known(t, 8 * p.tilesN, p.inv_group, tg) * 8;
+  // ---- tile `pid` of the list: every XCD has one contiguous run of it, eight rows of tiles at a time, columns first within them
+  struct Tile {
+    int part, ti, tj, KT;  // KT: slabs of its reduction
+  };
+  auto tile = [&](int pid) __attribute__((always_inline)) {
+    Tile t;
+    const int xcd = pid & 7, q = p.total >> 3, r = p.total & 7;
+    const int lt = xcd * q + (xcd < r ? xcd : r) + (pid >> 3);
+    int in_part, tg;
+    t.part = div_known(lt, p.tilesM * p.tilesN, p.inv_tiles, in_part);
+    const int first = div_known(in_part, 8 * p.tilesN, p.inv_group, tg) * 8;
     if (p.tilesM - first >= 8) {
-      ti = first + (tg & 7);
-      tj = tg >> 3;
+      t.ti = first + (tg & 7);
+      t.tj = tg >> 3;
     } else {
       int row;
-      tj = div_known(tg, p.tilesM - first, p.inv_tail, row);
-      ti = first + row;
+      t.tj = div_known(tg, p.tilesM - first, p.inv_tail, row);
+      t.ti = first + row;
     }
-    part = __builtin_amdgcn_readfirstlane(part);
-    ti = __builtin_amdgcn_readfirstlane(ti);
-    tj = __builtin_amdgcn_readfirstlane(tj);
-  }
-  const int k_first = part * p.slabs * BK;
-  const int k_left = p.K - k_first;  // > 0
-  const int KT = min((k_left + BK - 1) / BK, p.slabs);
+    t.part = __builtin_amdgcn_readfirstlane(t.part);
+    t.ti = __builtin_amdgcn_readfirstlane(t.ti);
+    t.tj = __builtin_amdgcn_readfirstlane(t.tj);
+    t.KT = min((p.K + BK - 1) / BK - t.part * p.slabs, p.slabs);
+    return t;
+  };
 
-  // ---- global -> LDS: operand X is a tile of BM (BN) rows of 64, or (X K-major) of 64 rows of BM (BN); 16-byte chunk
-  // j * NT + tid of it, in LDS order, comes from voff[j].  Rows along the reduction are 128 bytes: chunk c of row r lies at
+  // ---- global -> LDS: an operand's slab is a tile of BM (BN) rows of 64, or (K-major) of 64 rows of BM (BN); 16-byte chunk
+  // j * NT + tid of it, in LDS order, is load j's.  Rows along the reduction are 128 bytes: chunk c of row r lies at
   // c ^ (r / 2) % 8.  K-major rows: 64-byte group g of row r at g ^ r % 4, its 32-byte halves swapped where r / 8 is odd.
-  // (K-major: chunks of the four loads lie 16 rows apart, added when they are issued, which leaves six registers more.)
-  uint32_t voffP[PK ? 1 : 4], voffQ[QK ? 1 : 4];
-  auto offsets = [&](uint32_t* v, bool kmajor, int width, int ld) {
-    if (kmajor) {
-      const int cpr = width / 8, row = tid / cpr, c = tid % cpr;
-      const int chunk = (((c >> 2) ^ (row & 3)) << 2) | ((c & 3) ^ (((row >> 3) & 1) << 1));
-      v[0] = (uint32_t)(row * ld + chunk * 8) * 2u;
+  // A descriptor ends where the operand's rows do: past the last row of the tile with the reduction along the rows (wherever along
+  // it the slab is: that is the scalar offset), past the last index of the reduction K-major.  Chunks that start behind the end of a
+  // row -- the reduction's or, K-major, the matrix's -- get an offset past every descriptor's end.
+  constexpr int P_ROWS = PK ? NT / (BM / 8) : NT / 8, Q_ROWS = QK ? NT / (BN / 8) : NT / 8;  // between two loads of a slab
+  static_assert(P_ROWS % 16 == 0 && Q_ROWS % 16 == 0, "the swizzles repeat every 16 rows");
+  constexpr uint32_t kEnd = 0xb0000000u;  // past every descriptor's end, with room for the rows between the loads
+  static_assert(kEnd + 256ull * kLinMaxLd * 2 < (1ull << 32) && 256ull * kLinMaxLd * 2 < kEnd, "offsets within a tile");
+  // The thread's number where what follows from it is not to be kept in registers over the loops.
+  auto again = [&]() __attribute__((always_inline)) {
+    int v = tid;
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  auto offset = [&](int tid, bool kmajor, int width, int ld, int in) __attribute__((always_inline)) {  // in: elements of a row from the tile's start
+    const int cpr = kmajor ? width / 8 : 8, row = tid / cpr, c = tid % cpr;
+    const int chunk = kmajor ? (((c >> 2) ^ (row & 3)) << 2) | ((c & 3) ^ (((row >> 3) & 1) << 1)) : c ^ ((row >> 1) & 7);
+    return chunk * 8 < in ? (uint32_t)(row * ld + chunk * 8) * 2u : kEnd;
+  };
+  // 64-row wavefront tiles have a register for every load's offset; 128-row ones one per operand, the rest is added.
+  constexpr int VP = TM == 4 ? PL : 1, VQ = TM == 4 ? QL : 1;
+  uint32_t voffP[VP], voffQ[VQ];
+  auto set_offsets = [&](int inP, int inQ) __attribute__((always_inline)) {
+    const int t = again();
+    const uint32_t vp = offset(t, PK, BM, p.ldp, inP), vq = offset(t, QK, BN, p.ldq, inQ);
+#pragma unroll
+    for (int j = 0; j < VP; ++j) voffP[j] = vp + (uint32_t)j * (uint32_t)(P_ROWS * p.ldp * 2);
+#pragma unroll
+    for (int j = 0; j < VQ; ++j) voffQ[j] = vq + (uint32_t)j * (uint32_t)(Q_ROWS * p.ldq * 2);
+  };
+  // what is loaded next: slab nxt of a tile of KT_in, into slot slot_in
+  const char *baseP = (const char*)p.P, *baseQ = (const char*)p.Q;
+  const int64_t stepP = PK ? (int64_t)BK * p.ldp * 2 : 0, stepQ = QK ? (int64_t)BK * p.ldq * 2 : 0;
+  int pid_in = blockIdx.x, k_in = 0, nxt = 0, KT_in = 0, slot_in = 0, soff = 0, endP = 0, endQ = 0, inP = 0, inQ = 0;
+  int recsP = 0, recsQ = 0;
+  // What changes with the last slab of a tile and behind it.  (Slabs behind an odd number of them, and behind the last tile, are
+  // loaded as zeros: the loop is two slabs long, and its waits count on every load.)
+  auto turn = [&]() __attribute__((always_inline)) {
+    if (nxt >= ((KT_in + 1) & ~1) && pid_in < p.total) {
+      const Tile t = tile(pid_in);
+      pid_in += p.grid;
+      nxt = 0;
+      soff = 0;
+      KT_in = t.KT;
+      k_in = t.part * p.slabs * BK;
+      auto begin = [&](const bf16_t* base, bool kmajor, int extent, int at, int ld, const char*& from, int& end, int& recs, int& in) __attribute__((always_inline)) {
+        from = (const char*)(base + (kmajor ? (int64_t)k_in * ld + at : (int64_t)at * ld + k_in));
+        // (K-major: rows from the tile's last slab on; all of a slab's rows are there before it)
+        const int64_t n = (int64_t)(kmajor ? p.K - k_in - (t.KT - 1) * BK : extent - at) * ld * 2;
+        end = (int)(uint32_t)(n < (int64_t)kEnd ? n : (int64_t)kEnd);
+        recs = kmajor ? (int)kEnd : end;
+        in = kmajor ? ((extent + 7) & ~7) - at : BK;
+      };
+      begin(p.P, PK, p.e.M, t.ti * BM, p.ldp, baseP, endP, recsP, inP);
+      begin(p.Q, QK, p.e.N, t.tj * BN, p.ldq, baseQ, endQ, recsQ, inQ);
+      set_offsets(inP, inQ);
+    }
+    const bool last = nxt == KT_in - 1, behind = nxt >= KT_in;
+    recsP = behind ? 0 : PK && last ? endP : recsP;
+    recsQ = behind ? 0 : QK && last ? endQ : recsQ;
+    soff = behind ? 0 : soff;  // (a scalar offset past a descriptor's end may turn its check around)
+    if ((!PK || !QK) && last && (p.K & (BK - 1))) {  // the reduction may end inside this slab
+      const int in = p.K - k_in - nxt * BK;
+      set_offsets(PK ? inP : in, QK ? inQ : in);
+    }
+  };
+  // LDS: the slots of P, then those of Q
+  auto load = [&](int slot, auto jc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value, jo = j < PL ? j : j - PL;
+    constexpr bool isP = j < PL, kmajor = isP ? PK : QK;
+    uint32_t v;
+    if constexpr (TM == 4) {
+      v = isP ? voffP[isP ? jo : 0] : voffQ[isP ? 0 : jo];
     } else {
-      const int row = tid >> 3, chunk = (tid & 7) ^ ((row >> 1) & 7);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (uint32_t)((row + j * (NT / 8)) * ld + chunk * 8) * 2u;
+      // (the sums stay here instead of in registers of the whole loop)
+      if constexpr (isP) asm volatile("" : "+v"(voffP[0]));
+      else asm volatile("" : "+v"(voffQ[0]));
+      v = isP ? voffP[0] : voffQ[0];
+      if constexpr (jo != 0) v += (uint32_t)jo * (uint32_t)((isP ? P_ROWS * p.ldp : Q_ROWS * p.ldq) * 2);
     }
-  };
-  static_assert(NT / (BM / 8) == 16, "a load brings 16 rows of a K-major tile");
-  offsets(voffP, PK, BM, p.ldp);
-  offsets(voffQ, QK, BN, p.ldq);
-  // start of the tile's first slab, and bytes from there to the end of the matrix
-  auto begin = [&](const bf16_t* base, bool kmajor, int extent, int at, int ld, const char*& from, int64_t& left) {
-    const int64_t skip = kmajor ? (int64_t)k_first * ld + at : (int64_t)at * ld + k_first;
-    // (rows are whole chunks)
-    const int64_t all = kmajor ? (int64_t)(p.K - 1) * ld + ((extent + 7) & ~7) : (int64_t)(extent - 1) * ld + ((p.K + 7) & ~7);
-    from = (const char*)(base + skip);
-    left = (all - skip) * 2;
-  };
-  const char *nextP, *nextQ;
-  int64_t leftP, leftQ;
-  begin(p.P, PK, p.e.M, ti * BM, p.ldp, nextP, leftP);
-  begin(p.Q, QK, p.e.N, tj * BN, p.ldq, nextQ, leftQ);
-  const int64_t stepP = PK ? (int64_t)BK * p.ldp * 2 : BK * 2, stepQ = QK ? (int64_t)BK * p.ldq * 2 : BK * 2;
-  int nxt = 0;  // the slab that is loaded next
-  auto records = [&](int64_t left) -> int {
-    // (slabs past the last one are loaded as zeros: the loop is two slabs long, and its waits count on every load)
-    const int64_t n = nxt < KT && left > 0 ? (left < 0xfffffff0ll ? left : 0xfffffff0ll) : 0;
-    return (int)(uint32_t)n;
-  };
-  int recsP, recsQ;
-  auto prepare = [&]() {
-    recsP = records(leftP);
-    recsQ = records(leftQ);
-    if ((!PK || !QK) && nxt == KT - 1 && (k_left & (BK - 1)) && k_left <= KT * BK) {
-      // the reduction ends inside this slab
-      const int in = k_left - nxt * BK;
-      const int chunk = ((tid & 7) ^ ((tid >> 4) & 7)) * 8;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!PK && chunk >= in) voffP[PK ? 0 : j] = 0xfffffff0u;
-        if (!QK && chunk >= in) voffQ[QK ? 0 : j] = 0xfffffff0u;
-      }
-    }
-  };
-  auto load = [&](int slot, int j) {
-    const int jo = j & 3;
-    uint32_t& own = j < 4 ? voffP[PK ? 0 : jo] : voffQ[QK ? 0 : jo];
-    asm volatile("" : "+v"(own));  // (the sums below stay here instead of in registers of the whole loop)
-    uint32_t v = own;
-    if ((j < 4 ? PK : QK) && jo) v += (uint32_t)jo * (uint32_t)(32 * (j < 4 ? p.ldp : p.ldq));
     const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(j < 4 ? nextP : nextQ), 0, j < 4 ? recsP : recsQ, 0x00020000);
-    char* l = lds + (j < 4 ? 0 : 2 * OPB) + slot * OPB + (j & 3) * (NT * 16) + wave * (64 * 16);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(l), 16, (int)v, 0, 0, 0);
+        __builtin_amdgcn_make_buffer_rsrc((void*)(isP ? baseP : baseQ), 0, isP ? recsP : recsQ, 0x00020000);
+    char* l = lds + (isP ? slot * PB : NS * PB + slot * QB) + jo * (NT * 16) + wave * (64 * 16);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(l), 16, (int)v, kmajor ? 0 : soff, 0, 0);
   };
-  auto loaded = [&]() {
-    ++nxt;
-    nextP += stepP;
-    nextQ += stepQ;
-    leftP -= stepP;
-    leftQ -= stepQ;
-    prepare();
+  auto loaded = [&]() __attribute__((always_inline)) {
+    slot_in = slot_in == NS - 1 ? 0 : slot_in + 1;
+    if constexpr (!PK || !QK) soff += BK * 2;
+    if constexpr (PK) baseP += stepP;
+    if constexpr (QK) baseQ += stepQ;
+    if (++nxt >= KT_in - 1) turn();
   };
-  prepare();
 
   // ---- LDS -> fragments: lane l holds row (column) l % 16 and reduction indices 8 (l / 16) .. + 7 of a 32-deep step
   const uint32_t lds_base = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds;
   const int l16 = lane & 15, quad = lane >> 4;
-  uint32_t aoff[PK ? TM : ST], boff[QK ? TN : ST];
+  // (fragments f and f + 1 of a K-major operand differ in bit 5 of the address: where registers are short, one serves both)
+  constexpr int AF = PK ? (TM == 8 ? 2 : 1) : 1, NA = PK ? TM / AF : ST, NB = QK ? TN : ST;
+  uint32_t aoff[NA], boff[NB];
   auto kmajor_off = [&](int base, int width, int at, int f) {
     return lds_base + (uint32_t)(base + (8 * quad + (l16 >> 2)) * (width * 2) + ((((at + f * 16) >> 5) ^ (l16 >> 2)) << 6) +
                                  ((f ^ quad) & 1) * 32 + (l16 & 3) * 8);
@@ -317,148 +372,235 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
     return lds_base + (uint32_t)(base + (at + l16) * (BK * 2) + ((st * 4 + quad) ^ (l16 >> 1)) * 16);
   };
 #pragma unroll
-  for (int f = 0; f < (PK ? TM : ST); ++f) aoff[f] = PK ? kmajor_off(0, BM, wm * Cfg::WTM, f) : row_off(0, wm * Cfg::WTM, f);
+  for (int f = 0; f < NA; ++f) aoff[f] = PK ? kmajor_off(0, BM, wm * Cfg::WTM, f * AF) : row_off(0, wm * Cfg::WTM, f);
 #pragma unroll
-  for (int f = 0; f < (QK ? TN : ST); ++f)
-    boff[f] = QK ? kmajor_off(2 * OPB, BN, wn * Cfg::WTN, f) : row_off(2 * OPB, wn * Cfg::WTN, f);
+  for (int f = 0; f < NB; ++f)
+    boff[f] = QK ? kmajor_off(NS * PB, BN, wn * Cfg::WTN, f) : row_off(NS * PB, wn * Cfg::WTN, f);
 
   f32x4 acc[TM][TN];
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  typedef LinSched<HALVES, ST, PK ? 2 : 1, QK ? 2 : 1> FS;
-  typedef std::integral_constant<int, 0> ic0;
-  bf16x8 fa[2][4], fb[2][TN];  // A by parity of the half, B by parity of the step
-  auto read_a = [&](auto slotc, auto stc, auto setc, auto ic) {
-    constexpr int slot = decltype(slotc)::value, st = decltype(stc)::value, i = decltype(ic)::value;
-    bf16x8& dst = fa[decltype(setc)::value][i & 3];
-    if constexpr (PK) lds_read_tr<slot * OPB + st * (32 * BM * 2), 4 * BM * 2>(dst, aoff[i]);
-    else lds_read16<slot * OPB + i * (16 * BK * 2)>(dst, aoff[st]);
-  };
-  auto read_frag = [&](auto slotc, auto hnc, auto rc) {  // read r of those half hn of a slab needs
-    constexpr int slot = decltype(slotc)::value, hn = decltype(hnc)::value, r = decltype(rc)::value;
-    constexpr int st = hn / HALVES, part_ = hn % HALVES;
-    typedef std::integral_constant<int, st> stc;
-    typedef std::integral_constant<int, (hn & 1)> setc;
-    if constexpr (part_ != 0) read_a(slotc, stc(), setc(), std::integral_constant<int, 4 + r>());
-    else if constexpr (r == 0 || r > 4) read_a(slotc, stc(), setc(), std::integral_constant<int, (r == 0 ? 0 : r - 4)>());
-    else if constexpr (QK) lds_read_tr<slot * OPB + st * (32 * BN * 2), 4 * BN * 2>(fb[st & 1][r - 1], boff[r - 1]);
-    else lds_read16<slot * OPB + (r - 1) * (16 * BK * 2)>(fb[st & 1][r - 1], boff[st]);
-  };
-
-  // ---- slab 0, its first fragments, slab 1
-#pragma unroll
-  for (int j = 0; j < 8; ++j) load(0, j);
-  loaded();
-  pipeline_barrier<0>();
-  static_for<0, 8>([&](auto rc) { read_frag(ic0(), ic0(), rc); });
-#pragma unroll
-  for (int j = 0; j < 8; ++j) load(1, j);
-  loaded();
-  __builtin_amdgcn_sched_barrier(0);
-  for (int kt = 0; kt < KT; kt += 2) {
-    static_for<0, 2 * HP>([&](auto shc) {
-      constexpr int s = decltype(shc)::value / HP, hp = decltype(shc)::value % HP;
-      constexpr int st = hp / HALVES, half = hp % HALVES;
-      constexpr bool last = hp == HP - 1;
-      if constexpr (last) pipeline_barrier<0>();  // the next slab has landed, this one is read: its slot is refilled
-      static_for<0, 16>([&](auto qc) {
-        constexpr int q = decltype(qc)::value, i = q / 4, j = q % 4;
-        frag_wait<FS::allowed(hp, q)>(fa[hp & 1][i], fb[st & 1][j]);
-        acc[half * 4 + i][j] =
-            __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[st & 1][j], fa[hp & 1][i], acc[half * 4 + i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (FS::read_behind(hp, q) >= 0) {
-          typedef std::integral_constant<int, FS::read_behind(hp, q)> rc;
-          if constexpr (last) read_frag(std::integral_constant<int, s ^ 1>(), ic0(), rc());
-          else read_frag(std::integral_constant<int, s>(), std::integral_constant<int, hp + 1>(), rc());
-        }
-        if constexpr (last && (q & 1)) load(s, q / 2);
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      if constexpr (last) loaded();
-    });
-  }
-  wait_vmcnt<0>();
-  // The reads behind the last half's MFMAs, which nobody uses, land before their registers are let go.
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-  for (int f = 0; f < 2; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      asm volatile("" ::"v"(fa[f][i]));
-      asm volatile("" ::"v"(fb[f][i]));
-    }
-
-  // ---- element e of a lane: row l16, column 4 * quad + e of its 16 x 16 tile
-  const int row0 = ti * BM + wm * Cfg::WTM + l16, col0 = tj * BN + wn * Cfg::WTN + 4 * quad;
-  if constexpr (SPLIT) {
-    float* out = p.part + (int64_t)part * p.e.M * p.e.N;
+  auto clear_acc = [&]() {
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int row = row0 + i * 16, col = col0 + j * 16;
-        if (row >= p.e.M || col >= p.e.N) continue;
-        float* o = out + (int64_t)row * p.e.N + col;
-        if (p.e.N % 4 == 0) {
-          *(f32x4*)o = acc[i][j];
-        } else {
+      for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  clear_acc();
+
+  typedef std::integral_constant<int, 0> ic0;
+  typedef std::integral_constant<int, 1> ic1;
+  // AHEAD (64 x 64 wavefront tiles): the fragments of a whole slab are requested one slab ahead, by parity of the slab, with
+  // one wait for them and one barrier per slab.  128-row wavefront tiles have registers for half a step ahead: A by parity
+  // of the half (four fragments), B by parity of the step.
+  constexpr bool AHEAD = TM == 4;
+  bf16x8 fa[2][AHEAD ? ST * 4 : 4], fb[2][AHEAD ? ST * TN : TN];
+  auto read_a = [&](auto slotc, auto stc, auto ic, bf16x8& dst) {
+    constexpr int slot = decltype(slotc)::value, st = decltype(stc)::value, i = decltype(ic)::value;
+    if constexpr (PK && AF == 2) {
+      asm volatile("" : "+v"(aoff[i / 2]));  // (the other address is not kept)
+      lds_read_tr<slot * PB + st * (32 * BM * 2), 4 * BM * 2>(dst, aoff[i / 2] ^ (i & 1 ? 32u : 0u));
+    } else if constexpr (PK) lds_read_tr<slot * PB + st * (32 * BM * 2), 4 * BM * 2>(dst, aoff[i]);
+    else lds_read16<slot * PB + i * (16 * BK * 2)>(dst, aoff[st]);
+  };
+  auto read_b = [&](auto slotc, auto stc, auto jc, bf16x8& dst) {
+    constexpr int slot = decltype(slotc)::value, st = decltype(stc)::value, j = decltype(jc)::value;
+    if constexpr (QK) lds_read_tr<slot * QB + st * (32 * BN * 2), 4 * BN * 2>(dst, boff[j]);
+    else lds_read16<slot * QB + j * (16 * BK * 2)>(dst, boff[st]);
+  };
+  // To the next slot, where slots are in the offsets (more than two: P's would pass the reads' 16-bit offset).
+  int slot_out = 0;
+  auto next_slot = [&]() {
+    if constexpr (NS > 2) {
+      const bool wrap = slot_out == NS - 1;
+      const uint32_t dp = wrap ? (uint32_t)(-(NS - 1) * PB) : (uint32_t)PB, dq = wrap ? (uint32_t)(-(NS - 1) * QB) : (uint32_t)QB;
+      slot_out = wrap ? 0 : slot_out + 1;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < p.e.N) o[e] = acc[i][j][e];
-        }
-      }
-  } else {
-    if constexpr (ACT) {
-      // Through the wavefront's eighth (quarter) of the ring, 64 rows at a time: sums [row][column], 16-byte chunk c of row r at
-      // c ^ r % 16.  The activation then stands once in a loop of four rows a pass, not once for every accumulator,
-      // and C, the addend and the slopes are moved in whole 128-byte lines.
-      __syncthreads();  // every wavefront's loads have landed, and every fragment is read
-      char* const mine = lds + wave * (64 * 64 * 4);
-      static_assert(Cfg::LDS_BYTES >= Cfg::WM * Cfg::WN * 64 * 64 * 4, "staging");
-      const int col = tj * BN + wn * Cfg::WTN + 4 * l16;
-      const f32x4 b = bias4(p.e, col);
-      static_for<0, TM / 4>([&](auto hc) {
-        constexpr int h = decltype(hc)::value;
+      for (int f = 0; f < NA; ++f) aoff[f] += dp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) *(f32x4*)(mine + (i * 16 + l16) * 256 + ((4 * j + quad) ^ l16) * 16) = acc[h * 4 + i][j];
-        asm volatile("" ::: "memory");
-        const int row_h = ti * BM + wm * Cfg::WTM + h * 64 + quad;
-        uint2 r = residual4(p.e, row_h, col);
-#pragma unroll 1
-        for (int t = 0; t < 16; ++t) {
-          const int lr = t * 4 + quad;
-          const f32x4 z = *(const f32x4*)(mine + lr * 256 + ((l16 ^ (lr & 15)) * 16));
-          const uint2 rn = t < 15 ? residual4(p.e, row_h + t * 4 + 4, col) : make_uint2(0, 0);
-          finish4<true>(p.e, row_h + t * 4, col, z, b, r);
-          r = rn;
-        }
-        asm volatile("" ::: "memory");
+      for (int f = 0; f < NB; ++f) boff[f] += dq;
+    }
+  };
+
+  typedef LinSched<HALVES, ST, PK ? 2 : 1, QK ? 2 : 1> FS;
+  auto read_frag = [&](auto slotc, auto hnc, auto rc) {  // read r of those half hn of a slab needs (not AHEAD)
+    constexpr int hn = decltype(hnc)::value, r = decltype(rc)::value, st = hn / HALVES, half = hn % HALVES;
+    typedef std::integral_constant<int, st> stc;
+    if constexpr (half != 0) read_a(slotc, stc(), std::integral_constant<int, 4 + r>(), fa[hn & 1][r]);
+    else if constexpr (r == 0 || r > 4) read_a(slotc, stc(), std::integral_constant<int, (r == 0 ? 0 : r - 4)>(), fa[hn & 1][r == 0 ? 0 : r - 4]);
+    else read_b(slotc, stc(), std::integral_constant<int, r - 1>(), fb[st & 1][r - 1]);
+  };
+  auto read_ahead = [&](auto parc, auto rc) {  // read r of a slab's sixteen, from where the offsets point
+    constexpr int par = decltype(parc)::value, r = decltype(rc)::value, st = r / 8, f = r % 8;
+    typedef std::integral_constant<int, st> stc;
+    if constexpr (f < 4) read_a(ic0(), stc(), std::integral_constant<int, f>(), fa[par][st * 4 + f]);
+    else read_b(ic0(), stc(), std::integral_constant<int, f - 4>(), fb[par][st * TN + f - 4]);
+  };
+  // every fragment of that parity that may be in flight has arrived
+  auto landed = [&](auto parc) {
+    auto& a = fa[decltype(parc)::value];
+    auto& b = fb[decltype(parc)::value];
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]), "+v"(b[3]));
+    if constexpr (AHEAD)
+      asm volatile("" : "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(a[7]), "+v"(b[4]), "+v"(b[5]), "+v"(b[6]), "+v"(b[7]));
+  };
+
+  // One slab, whose first fragments (AHEAD: all of them) are on their way, in slot `slotc` (0, 1) where there are two.
+  auto slab = [&](auto slotc) __attribute__((always_inline)) {
+    constexpr int here = NS == 2 ? decltype(slotc)::value : 0, next = NS == 2 ? here ^ 1 : 0, par = decltype(slotc)::value;
+    if constexpr (AHEAD) {
+      pipeline_barrier<(NS - 2) * LPS>();  // the next slab has landed, this one is read: its slot is refilled
+      landed(slotc);
+      next_slot();
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, 32>([&](auto qc) {
+        constexpr int q = decltype(qc)::value, st = q / 16, i = (q % 16) / 4, j = q % 4;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[par][st * TN + j], fa[par][st * 4 + i], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // a refill behind every fourth MFMA, a read behind each of the others
+        constexpr bool refill = q % 4 == 3 && q / 4 < LPS;
+        constexpr int r = q - (q / 4 < LPS ? q / 4 : LPS);
+        if constexpr (refill) load(slot_in, std::integral_constant<int, q / 4>());
+        else if constexpr (r < 16) read_ahead(std::integral_constant<int, par ^ 1>(), std::integral_constant<int, r>());
+        __builtin_amdgcn_sched_barrier(0);
       });
+      loaded();
+    } else {
+      static_for<0, HP>([&](auto hpc) {
+        constexpr int hp = decltype(hpc)::value, st = hp / HALVES, half = hp % HALVES;
+        constexpr bool last = hp == HP - 1;
+        if constexpr (last) pipeline_barrier<(NS - 2) * LPS>();
+        static_for<0, 16>([&](auto qc) {
+          constexpr int q = decltype(qc)::value, i = q / 4, j = q % 4;
+          frag_wait<FS::allowed(hp, q)>(fa[hp & 1][i], fb[st & 1][j]);
+          acc[half * 4 + i][j] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[st & 1][j], fa[hp & 1][i], acc[half * 4 + i][j], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (FS::read_behind(hp, q) >= 0) {
+            typedef std::integral_constant<int, FS::read_behind(hp, q)> rc;
+            if constexpr (last) read_frag(std::integral_constant<int, next>(), ic0(), rc());
+            else read_frag(std::integral_constant<int, here>(), std::integral_constant<int, hp + 1>(), rc());
+          }
+          if constexpr (last && (q & 1) && q / 2 < LPS) load(here, std::integral_constant<int, q / 2>());
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (last) loaded();
+      });
+    }
+  };
+
+  // ---- the ring is filled; slab 0's fragments
+  turn();
+  static_for<0, NS>([&](auto sc) {
+    static_for<0, LPS>([&](auto jc) { load(decltype(sc)::value, jc); });
+    loaded();
+  });
+  pipeline_barrier<(NS - 1) * LPS>();
+  if constexpr (AHEAD) static_for<0, 16>([&](auto rc) { read_ahead(ic0(), rc); });
+  else static_for<0, 8>([&](auto rc) { read_frag(ic0(), ic0(), rc); });
+  __builtin_amdgcn_sched_barrier(0);
+
+  for (int pid = blockIdx.x;;) {
+    const Tile t = tile(pid);
+    for (int kt = 0; kt < t.KT; kt += 2) {  // (a slab of zeros behind an odd number)
+      slab(ic0());
+      slab(ic1());
+    }
+    // The first fragments of the next tile are on their way: they land before the epilogue, whose register traffic must not
+    // meet a read in flight.
+    landed(ic0());
+
+    // ---- element e of a lane: row l16, column 4 * quad + e of its 16 x 16 tile
+    const int lane = again() & 63, l16 = lane & 15, quad = lane >> 4;
+    const int row0 = t.ti * BM + wm * Cfg::WTM + l16, col0 = t.tj * BN + wn * Cfg::WTN + 4 * quad;
+    if constexpr (SPLIT) {
+      float* out = p.part + (int64_t)t.part * p.e.M * p.e.N;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const int row = row0 + i * 16, col = col0 + j * 16;
+          if (row >= p.e.M || col >= p.e.N) continue;
+          float* o = out + (int64_t)row * p.e.N + col;
+          if (p.e.N % 4 == 0) {
+            *(f32x4*)o = acc[i][j];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (col + e < p.e.N) o[e] = acc[i][j][e];
+          }
+        }
     } else {
       f32x4 b[TN];
+      if constexpr (!PK && !QK)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = bias4(p.e, col0 + j * 16);
+        for (int j = 0; j < TN; ++j) b[j] = bias4(p.e, col0 + j * 16);
+      // Sixteen rows at a time through the wavefront's staging, so that C (and the slopes) leave in whole 128-byte lines: an
+      // 8-byte piece q of row r lies at q ^ 2 ((r / 2) % 8), which spreads writes and reads over all banks.
+      char* const stg = lds + Cfg::RING_BYTES + wave * Cfg::STG_BYTES;
+      const int sr = lane >> 3, sq = lane & 7;  // row and 16-byte piece of a lane in the lines
+      const int wrow = t.ti * BM + wm * Cfg::WTM, wcol = t.tj * BN + wn * Cfg::WTN;
+      const bool lines = p.e.vec == 8 && wcol + 64 <= p.e.N;  // (the same for the whole wavefront)
+      auto put = [&](int j, uint2 w) { *(uint2*)(stg + l16 * 128 + (((4 * j + quad) ^ (((l16 >> 1) & 7) << 1)) << 3)) = w; };
+      auto send = [&](uint16_t* o, int row) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = sr + 8 * h;
+          const uint4 w = *(const uint4*)(stg + r * 128 + (((2 * sq) ^ (((r >> 1) & 7) << 1)) << 3));
+          if (row + r < p.e.M) *(uint4*)(o + (int64_t)(row + r) * p.e.N + wcol + sq * 8) = w;
+        }
+        asm volatile("" ::: "memory");
+      };
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        uint2 r[TN];
+        const int row = row0 + i * 16;
+        uint2 y[TN], sl[TN];
+        if constexpr (PK || QK) {  // a gradient: nothing to add
 #pragma unroll
-        for (int j = 0; j < TN; ++j) r[j] = residual4(p.e, row0 + i * 16, col0 + j * 16);
+          for (int j = 0; j < TN; ++j)
+            y[j] = make_uint2(pack_bf16x2(acc[i][j][0], acc[i][j][1]), pack_bf16x2(acc[i][j][2], acc[i][j][3]));
+        } else {
+          uint2 r[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) finish4<false>(p.e, row0 + i * 16, col0 + j * 16, acc[i][j], b[j], r[j]);
+          for (int j = 0; j < TN; ++j) r[j] = residual4(p.e, row, col0 + j * 16);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) finish4<ACT, SLOPE>(p.e, acc[i][j], b[j], r[j], y[j], sl[j]);
+        }
+        if (lines) {
+          if constexpr (SLOPE) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j) put(j, sl[j]);
+            send(p.e.slope, wrow + i * 16);
+          }
+#pragma unroll
+          for (int j = 0; j < TN; ++j) put(j, y[j]);
+          send(p.e.C, wrow + i * 16);
+        } else {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            const int col = col0 + j * 16;
+            if (row >= p.e.M || col >= p.e.N) continue;
+            const int64_t at = (int64_t)row * p.e.N + col;
+            if constexpr (SLOPE) store4(p.e, p.e.slope + at, col, sl[j]);
+            store4(p.e, p.e.C + at, col, y[j]);
+          }
+        }
         asm volatile("" ::: "memory");
       }
     }
+    pid += p.grid;
+    if (pid >= p.total) break;
+    clear_acc();
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  wait_vmcnt<0>();  // loads of zeros behind the last tile land before the LDS is given back
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(fa[0]) / sizeof(fa[0][0])); ++i) {
+    asm volatile("" ::"v"(fa[0][i]));
+    asm volatile("" ::"v"(fb[0][i]));
   }
 }
 
 // Adds the parts of a split reduction, in their order, and finishes: four elements per thread.
-template <bool ACT>
 __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, const float* __restrict__ part, int splits) {
   const int per_row = (p.N + 3) / 4;
   const int64_t all = (int64_t)p.M * per_row, one = (int64_t)p.M * p.N;
@@ -475,16 +617,16 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, cons
         for (int e = 0; e < 4; ++e)
           if (col + e < p.N) s[e] += q[k * one + e];
     }
-    finish4<ACT>(p, row, col, s, bias4(p, col), residual4(p, row, col));
+    finish4_any(p, row, col, s);
   }
 }
 
 // ---------------------------------------------------------------------------------------------- few tokens
 // Up to 64 rows of x: the weight is read once and nothing else counts.  A workgroup takes 16 rows of W, its wavefronts an
 // equal run of the reduction each; fragments go from memory to registers with no LDS between (a lane's chunk is its MFMA operand
-// as it lies), eight loads of W in flight per wavefront.  MFMA row: a row of W; column: a token (past the last one, the
+// as it lies), the next U steps' while the MFMAs of these run.  MFMA row: a row of W; column: a token (past the last one, the
 // last one again).  The wavefronts' sums meet in LDS and are added in their order.
-template <int TB, int WAVES, bool ACT>
+template <int TB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
                                                              const bf16_t* __restrict__ w, int64_t ldw, int K) {
   __shared__ f32x4 sums[WAVES][TB][64];
@@ -501,30 +643,33 @@ __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p
   for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int steps = (K + 31) / 32;
   const int s0 = (int)((int64_t)steps * wave / WAVES), s1 = (int)((int64_t)steps * (wave + 1) / WAVES);
-  constexpr int U = 8;
-  int s = s0;
-  for (; s + U <= s1 && (s + U) * 32 <= K; s += U) {
-    bf16x8 fw[U];
+  constexpr int U = TB == 4 ? 2 : 4;
+  struct Set {
+    bf16x8 w[U], x[TB][U];
+  };
+  auto fetch = [&](Set& f, int s) {  // steps s .. s + U - 1, zeros behind the run's end and the reduction's
 #pragma unroll
-    for (int u = 0; u < U; ++u) fw[u] = *(const bf16x8*)(wp + (s + u) * 32);
+    for (int u = 0; u < U; ++u) {
+      const bool in = s + u < s1 && (s + u) * 32 + quad * 8 < K;
+      const bf16x8 zero = {};
+      f.w[u] = in ? *(const bf16x8*)(wp + (s + u) * 32) : zero;
 #pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      bf16x8 fx[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) fx[u] = *(const bf16x8*)(xp[b] + (s + u) * 32);
-#pragma unroll
-      for (int u = 0; u < U; ++u) acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[u], fx[u], acc[b], 0, 0, 0);
+      for (int b = 0; b < TB; ++b) f.x[b][u] = in ? *(const bf16x8*)(xp[b] + (s + u) * 32) : zero;
     }
-  }
-  for (; s < s1; ++s) {
-    const bool in = s * 32 + quad * 8 < K;
-    const bf16x8 zero = {};
-    const bf16x8 fw = in ? *(const bf16x8*)(wp + s * 32) : zero;
+  };
+  auto multiply = [&](const Set& f) {
 #pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      const bf16x8 fx = in ? *(const bf16x8*)(xp[b] + s * 32) : zero;
-      acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, fx, acc[b], 0, 0, 0);
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int b = 0; b < TB; ++b) acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.w[u], f.x[b][u], acc[b], 0, 0, 0);
+  };
+  Set even, odd;
+  fetch(even, s0);
+  for (int s = s0; s < s1; s += 2 * U) {
+    fetch(odd, s + U);
+    multiply(even);
+    fetch(even, s + 2 * U);
+    multiply(odd);
   }
 #pragma unroll
   for (int b = 0; b < TB; ++b) sums[wave][b][lane] = acc[b];
@@ -535,7 +680,7 @@ __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p
 #pragma unroll
     for (int k = 1; k < WAVES; ++k) t += sums[k][b][l];
     const int row = b * 16 + (l & 15), col = n0 + 4 * (l >> 4);
-    finish4<ACT>(p, row, col, t, bias4(p, col), residual4(p, row, col));
+    finish4_any(p, row, col, t);
   }
 }
 
@@ -595,18 +740,21 @@ __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restri
   }
 }
 
-// out[c] = sum of partial[0 .. parts)[c]: 64 columns of a workgroup, four threads a column.
+// out[c] = sum of partial[0 .. parts)[c]: 16 columns of a workgroup, sixteen threads a column.
 __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* out,
                                                       int out_dtype) {
-  __shared__ float sums[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+  __shared__ float sums[16][17];
+  const int tx = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
   float s = 0.f;
   if (c < cols)
-    for (int k = g; k < parts; k += 4) s += partial[(int64_t)k * cols + c];
-  sums[g][threadIdx.x & 63] = s;
+#pragma unroll 4
+    for (int k = g; k < parts; k += 16) s += partial[(int64_t)k * cols + c];
+  sums[g][tx] = s;
   __syncthreads();
   if (g == 0 && c < cols) {
-    s = (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    s = sums[0][tx];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sums[k][tx];
     if (out_dtype) ((float*)out)[c] = s;
     else ((bf16_t*)out)[c] = f32_to_bf16(s);
   }
@@ -614,29 +762,29 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
 
 // ---------------------------------------------------------------------------------------------- host
 // How a product runs: on which tiles, and in how many parts of the reduction.
+enum LinTile { kLinFew, kLin128, kLinWide, kLin256 };
 struct LinPlan {
-  int edge;    // 256, 128, or 0: lin_few_kernel
+  LinTile tile;
   int splits, slabs;
 };
 static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
-  if (M <= 64 && !p_kmajor && !q_kmajor) return {0, 1, 0};
+  if (M <= 64 && !p_kmajor && !q_kmajor) return {kLinFew, 1, 0};
   const int KT = (K + 63) / 64;
-  LinPlan best{128, 1, KT};
+  LinPlan best{kLin128, 1, KT};
   double least = 1e30;
-  for (int edge = 128; edge <= 256; edge += 128) {
-    const int64_t tiles = (int64_t)((M + edge - 1) / edge) * ((N + edge - 1) / edge);
+  for (int t = kLin128; t <= kLin256; ++t) {
+    const int bm = t == kLin128 ? 128 : 256, bn = t == kLin256 ? 256 : 128;
+    const double slab = t == kLin256 ? 1.2 : t == kLinWide ? 0.65 : 0.36, fixed = t == kLin256 ? 6.0 : t == kLinWide ? 4.0 : 3.0;
+    const int64_t tiles = (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     for (int s = 1; s <= 16 && s <= KT; ++s) {
-      const int slabs = ((KT + s - 1) / s + 1) & ~1;
+      const int slabs = (KT + s - 1) / s;
       const int parts = (KT + slabs - 1) / slabs;
       if (parts != s) continue;
-      const int64_t wgs = tiles * parts;
-      double us;
-      if (edge == 256) us = (double)((wgs + 255) / 256) * (slabs * 1.3 + 4.0);
-      else us = wgs <= 256 ? slabs * 0.4 + 3.0 : (double)((wgs + 511) / 512) * (slabs * 0.65 + 4.0);
+      double us = (double)((tiles * parts + 255) / 256) * (slabs * slab + fixed);
       if (parts > 1) us += 3.0 + (double)M * N * parts * 8.0 / 4e6;
       if (us < least) {
         least = us;
-        best = {edge, parts, slabs};
+        best = {(LinTile)t, parts, slabs};
       }
     }
   }
@@ -648,15 +796,32 @@ size_t lin_product_scratch(int M, int N, int K, int p_kmajor, int q_kmajor) {
   return plan.splits > 1 ? (size_t)plan.splits * M * N * sizeof(float) : 0;
 }
 
-template <class Cfg, bool PK, bool QK, bool ACT, bool SPLIT>
-static hipError_t launch_tile(const LinTileParams& tp, hipStream_t st) {
+template <class Cfg, bool PK, bool QK, int ACT, bool SLOPE, bool SPLIT>
+static hipError_t launch_tile(LinTileParams tp, hipStream_t st) {
   static std::atomic<uint64_t> attr_done{0};
-  auto kern = lin_tile_kernel<Cfg, PK, QK, ACT, SPLIT>;
+  auto kern = lin_tile_kernel<Cfg, PK, QK, ACT, SLOPE, SPLIT>;
   if (hipError_t e = set_max_dynamic_lds_once((const void*)kern, Cfg::LDS_BYTES, attr_done)) return e;
   const int64_t total = (int64_t)tp.tilesM * tp.tilesN * tp.splits;
   if (total > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kern, dim3((unsigned)total), dim3(Cfg::NT), Cfg::LDS_BYTES, st, tp);
+  static std::atomic<int> cu_count[64];
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev)) return e;
+  int cus = cu_count[dev & 63].load(std::memory_order_relaxed);
+  if (cus == 0) {
+    if (hipError_t e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev)) return e;
+    if (cus <= 0) return hipErrorInvalidValue;
+    cu_count[dev & 63].store(cus, std::memory_order_relaxed);
+  }
+  tp.total = (int)total;
+  tp.grid = total < cus ? (int)total : cus;
+  hipLaunchKernelGGL(kern, dim3((unsigned)tp.grid), dim3(Cfg::NT), Cfg::LDS_BYTES, st, tp);
   return hipGetLastError();
+}
+
+template <class Cfg, int ACT>
+static hipError_t launch_act(const LinTileParams& tp, hipStream_t st) {
+  return tp.e.slope ? launch_tile<Cfg, false, false, ACT, true, false>(tp, st)
+                    : launch_tile<Cfg, false, false, ACT, false, false>(tp, st);
 }
 
 template <class Cfg>
@@ -667,22 +832,27 @@ static hipError_t launch_tiles(const LinProduct& p, LinTileParams tp, hipStream_
   tp.inv_tiles = (uint32_t)(0xffffffffu / ((int64_t)tp.tilesM * tp.tilesN));
   tp.inv_group = (uint32_t)(0xffffffffu / (8 * (int64_t)tp.tilesN));
   tp.inv_tail = tp.tilesM % 8 ? 0xffffffffu / (tp.tilesM % 8) : 0;
-  const bool act = tp.e.act != kActNone, split = tp.splits > 1;
-  if (!p.p_kmajor && !p.q_kmajor) {
-    if (split) return launch_tile<Cfg, false, false, false, true>(tp, st);
-    return act ? launch_tile<Cfg, false, false, true, false>(tp, st) : launch_tile<Cfg, false, false, false, false>(tp, st);
+  const bool split = tp.splits > 1;
+  if (p.p_kmajor)
+    return split ? launch_tile<Cfg, true, true, kActNone, false, true>(tp, st) : launch_tile<Cfg, true, true, kActNone, false, false>(tp, st);
+  if (p.q_kmajor)
+    return split ? launch_tile<Cfg, false, true, kActNone, false, true>(tp, st) : launch_tile<Cfg, false, true, kActNone, false, false>(tp, st);
+  if (split) return launch_tile<Cfg, false, false, kActNone, false, true>(tp, st);
+  switch (tp.e.act) {
+    case kActNone: return launch_tile<Cfg, false, false, kActNone, false, false>(tp, st);
+    case kActRelu: return launch_act<Cfg, kActRelu>(tp, st);
+    case kActReluSquared: return launch_act<Cfg, kActReluSquared>(tp, st);
+    case kActGelu: return launch_act<Cfg, kActGelu>(tp, st);
+    case kActGeluTanh: return launch_act<Cfg, kActGeluTanh>(tp, st);
+    case kActSilu: return launch_act<Cfg, kActSilu>(tp, st);
+    default: return hipErrorInvalidValue;
   }
-  if (!p.p_kmajor) {
-    return split ? launch_tile<Cfg, false, true, false, true>(tp, st) : launch_tile<Cfg, false, true, false, false>(tp, st);
-  }
-  return split ? launch_tile<Cfg, true, true, false, true>(tp, st) : launch_tile<Cfg, true, true, false, false>(tp, st);
 }
 
 template <int TB, int WAVES>
 static hipError_t launch_few(const LinProduct& p, const LinEpilogue& e, hipStream_t st) {
-  const dim3 grid((unsigned)((p.N + 15) / 16)), block(WAVES * 64);
-  if (e.act != kActNone) hipLaunchKernelGGL((lin_few_kernel<TB, WAVES, true>), grid, block, 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
-  else hipLaunchKernelGGL((lin_few_kernel<TB, WAVES, false>), grid, block, 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
+  hipLaunchKernelGGL((lin_few_kernel<TB, WAVES>), dim3((unsigned)((p.N + 15) / 16)), dim3(WAVES * 64), 0, st, e, p.P, p.ldp, p.Q,
+                     p.ldq, p.K);
   return hipGetLastError();
 }
 
@@ -692,7 +862,7 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
     return ((uint64_t)ptr & 15) == 0 && ld % 8 == 0 && ld >= ((extent + 7) & ~7) && ld <= kLinMaxLd;
   };
   if (!whole(p.P, p.ldp, p.p_kmajor ? p.M : p.K) || !whole(p.Q, p.ldq, p.q_kmajor ? p.N : p.K)) return hipErrorInvalidValue;
-  if ((p.p_kmajor && !p.q_kmajor) || (p.act != kActNone && p.q_kmajor)) return hipErrorInvalidValue;
+  if ((p.p_kmajor && !p.q_kmajor) || (p.q_kmajor && (p.act != kActNone || p.bias || p.R || p.slope))) return hipErrorInvalidValue;
   LinEpilogue e;
   e.C = p.C;
   e.bias = p.bias;
@@ -703,9 +873,10 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
   e.N = p.N;
   e.act = p.act;
   e.bias_dtype = p.bias_dtype;
-  e.vec = p.N % 4 == 0 && (((uint64_t)p.C | (uint64_t)p.slope | (uint64_t)p.R) & 7) == 0 && (!p.R || p.ldr % 4 == 0);
+  const uint64_t bytes = ((uint64_t)p.C | (uint64_t)p.slope | (uint64_t)p.R) | (uint64_t)p.N * 2 | (p.R ? (uint64_t)p.ldr * 2 : 0);
+  e.vec = bytes % 16 == 0 ? 8 : bytes % 8 == 0 ? 4 : bytes % 4 == 0 ? 2 : 1;
   const LinPlan plan = lin_plan(p.M, p.N, p.K, p.p_kmajor, p.q_kmajor);
-  if (plan.edge == 0) {
+  if (plan.tile == kLinFew) {
     // sixteen wavefronts share a reduction where the rows of W alone do not fill the chip
     const bool wide = (p.N + 15) / 16 < 1024;
     if (p.M <= 16) return wide ? launch_few<1, 16>(p, e, st) : launch_few<1, 4>(p, e, st);
@@ -723,12 +894,13 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
   tp.splits = plan.splits;
   tp.slabs = plan.slabs;
   if (plan.splits > 1 && !p.scratch) return hipErrorInvalidValue;
-  if (hipError_t err = plan.edge == 256 ? launch_tiles<Lin256>(p, tp, st) : launch_tiles<Lin128>(p, tp, st)) return err;
+  if (hipError_t err = plan.tile == kLin256 ? launch_tiles<Lin256>(p, tp, st)
+                       : plan.tile == kLinWide ? launch_tiles<LinWide>(p, tp, st) : launch_tiles<Lin128>(p, tp, st))
+    return err;
   if (plan.splits > 1) {
     const int64_t wg = ((int64_t)p.M * ((p.N + 3) / 4) + 255) / 256;
     const dim3 grid((unsigned)(wg < 65536 ? wg : 65536));
-    if (e.act != kActNone) hipLaunchKernelGGL((lin_join_kernel<true>), grid, dim3(256), 0, st, e, p.scratch, plan.splits);
-    else hipLaunchKernelGGL((lin_join_kernel<false>), grid, dim3(256), 0, st, e, p.scratch, plan.splits);
+    hipLaunchKernelGGL(lin_join_kernel, grid, dim3(256), 0, st, e, p.scratch, plan.splits);
   }
   return hipGetLastError();
 }
@@ -760,7 +932,7 @@ hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slo
 }
 
 hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st) {
-  hipLaunchKernelGGL(lin_sum_kernel, dim3((cols + 63) / 64), dim3(256), 0, st, partial, parts, cols, out, out_dtype);
+  hipLaunchKernelGGL(lin_sum_kernel, dim3((cols + 15) / 16), dim3(256), 0, st, partial, parts, cols, out, out_dtype);
   return hipGetLastError();
 }
 

@@ -1038,7 +1038,7 @@ def _rows(t: Tensor) -> Tuple[Tensor, int]:
 
 
 def _whole_chunks(t: Tensor, ld: int) -> bool:
-    return t.data_ptr() % 16 == 0 and ld % 8 == 0 and t.shape[1] % 8 == 0 and ld <= 1 << 22
+    return t.data_ptr() % 16 == 0 and ld % 8 == 0 and t.shape[1] % 8 == 0 and ld <= 1 << 21
 
 
 def _check_linear(name: str, t: Tensor, shape, device, dtypes=(torch.bfloat16,)) -> None:

@@ -20,7 +20,7 @@ def test_tile_kernels_keep_their_reads_apart(tmp_path):
     subprocess.run(cmd, check=True, capture_output=True, timeout=900)
     text = out.read_text().split("\n")
     starts = [i for i, line in enumerate(text) if re.match(r"_ZN4dion\d+lin_tile_kernel\S*:", line)]
-    assert len(starts) == 14
+    assert len(starts) == 48
     transposing = 0
     for i in starts:
         body = text[i + 1:next(j for j in range(i, len(text)) if "s_endpgm" in text[j]) + 1]
@@ -30,4 +30,4 @@ def test_tile_kernels_keep_their_reads_apart(tmp_path):
         mfma = [j for j, line in enumerate(body) if "v_mfma" in line]
         loop = body[mfma[0]:mfma[-1] + 1]
         assert not [line for line in loop if "scratch_" in line or "s_load" in line], text[i]
-    assert transposing == 8
+    assert transposing == 12

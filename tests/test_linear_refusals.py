@@ -24,7 +24,7 @@ def backward(lib, dy=P, lddy=32, slope=None, act=0, x=P, ldx=64, w=P, ldw=64, dx
 @NEEDS_LIB
 def test_c_entry_points_refuse():
     lib = _lib.load()
-    for call, cases in ((forward, ({"t": -1}, {"k": 0}, {"n": 0}, {"n": 1 << 22}, {"k": 1 << 22}, {"t": (1 << 30) + 1}, {"act": 6}, {"act": -1},
+    for call, cases in ((forward, ({"t": -1}, {"k": 0}, {"n": 0}, {"n": 1 << 21}, {"k": 1 << 21}, {"t": (1 << 30) + 1}, {"act": 6}, {"act": -1},
                                    {"x": None}, {"w": None}, {"y": None}, {"x": P + 1}, {"ldx": 63}, {"ldw": 63},
                                    {"bias": P, "bdt": 2}, {"r": P, "ldr": 31}, {"slope": P})),
                         (backward, ({"t": -1}, {"dy": None}, {"lddy": 31}, {"x": None}, {"w": None}, {"ldx": 8}, {"act": 1}, {"slope": P},
