@@ -1970,6 +1970,7 @@ extern "C" int dion_linear_forward(const void* x, int64_t ldx, const void* w, in
     if (int rc = check_lin_rows(who, "residual", residual, ldr, tokens, fan_out)) return rc;
   if (!y) return fail(DION_E_INVALID, "%s: y is null", who);
   if (slope && activation == kActNone) return fail(DION_E_INVALID, "%s: slopes without an activation", who);
+  if (!aligned16((uint64_t)(uintptr_t)slope)) return fail(DION_E_INVALID, "%s: slopes are not 16-byte aligned", who);
   const int copies = (lin_whole(x, ldx, fan_in) ? 0 : DION_LINEAR_COPY_X) | (lin_whole(w, ldw, fan_in) ? 0 : DION_LINEAR_COPY_W);
   const LinSpace s = lin_space(tokens, fan_in, fan_out, 0, activation, copies);
   if (s.total > 0 && (!workspace || workspace_bytes < s.total || !aligned16((uint64_t)(uintptr_t)workspace)))
@@ -2029,6 +2030,7 @@ extern "C" int dion_linear_backward(const void* dy, int64_t lddy, const void* sl
     if (int rc = check_lin_rows(who, "w", w, ldw, fan_out, fan_in)) return rc;
   if ((activation != kActNone) != (slope != nullptr))
     return fail(DION_E_INVALID, "%s: slopes go with an activation, and none without", who);
+  if (!aligned16((uint64_t)(uintptr_t)slope)) return fail(DION_E_INVALID, "%s: slopes are not 16-byte aligned", who);
   const int copies = (dw && !lin_whole(x, ldx, fan_in) ? DION_LINEAR_COPY_X : 0) |
                      (dx && !lin_whole(w, ldw, fan_in) ? DION_LINEAR_COPY_W : 0) |
                      (lin_whole(dy, lddy, fan_out) ? 0 : DION_LINEAR_COPY_DY);

@@ -22,7 +22,7 @@ struct LinProduct {
   int bias_dtype;    // 0 bf16, 1 fp32
   const bf16_t* R;   // [M][N] addend or null, ldr elements between rows
   int64_t ldr;
-  uint16_t* slope;  // [M][N] act'(z), or null: see linear.hip
+  uint16_t* slope;  // [M][N rounded up to 8] act'(z), 16-byte aligned, or null: see linear.hip
   // partial sums of a split reduction: lin_product_scratch(...) bytes
   float* scratch;
 };
@@ -31,8 +31,8 @@ constexpr int64_t kLinMaxLd = int64_t(1) << 21;
 size_t lin_product_scratch(int M, int N, int K, int p_kmajor, int q_kmajor);
 hipError_t launch_lin_product(const LinProduct& p, hipStream_t st);
 
-// dst[rows][cols_padded] = src (times slope), bf16, zero behind column cols; partial[lin_sum_parts(rows)][cols]: sums over runs of
-// rows, in fp32, before rounding.  dst or partial may be null.  cols_padded: a multiple of 8, less than cols + 8.
+// dst[rows][cols rounded up to 8] = src (times slope, laid out like dst), bf16, zero behind column cols;
+// partial[lin_sum_parts(rows)][cols]: sums over runs of rows, in fp32, before rounding.  dst or partial may be null.
 int lin_sum_parts(int rows);
 hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slope, int act, int rows, int cols, bf16_t* dst,
                               float* partial, hipStream_t st);

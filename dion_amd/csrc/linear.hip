@@ -133,6 +133,9 @@ static __device__ __forceinline__ void store4(const LinEpilogue& p, uint16_t* o,
     if (col + 3 < p.N) o[3] = (uint16_t)(w.y >> 16);
   }
 }
+// Slopes lie in whole 16-byte chunks, whatever N is.
+static __host__ __device__ __forceinline__ int slope_pitch(int n) { return (n + 7) & ~7; }
+
 // Four sums of a row as they are stored, y and the slopes.
 template <int ACT, bool SLOPE>
 static __device__ __forceinline__ void finish4(const LinEpilogue& p, f32x4 z, f32x4 b, uint2 r, uint2& y, uint2& slopes) {
@@ -162,9 +165,8 @@ static __device__ __forceinline__ void finish4_any(const LinEpilogue& p, int row
     case kActSilu: finish4<kActSilu, true>(p, z, b, r, y, s); break;
     default: finish4<kActNone, true>(p, z, b, r, y, s); break;
   }
-  const int64_t at = (int64_t)row * p.N + col;
-  if (p.slope) store4(p, p.slope + at, col, s);
-  store4(p, p.C + at, col, y);
+  if (p.slope) *(uint2*)(p.slope + (int64_t)row * slope_pitch(p.N) + col) = s;
+  store4(p, p.C + (int64_t)row * p.N + col, col, y);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
@@ -540,13 +542,13 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
       const int wrow = t.ti * BM + wm * Cfg::WTM, wcol = t.tj * BN + wn * Cfg::WTN;
       const bool lines = p.e.vec == 8 && wcol + 64 <= p.e.N;  // (the same for the whole wavefront)
       auto put = [&](int j, uint2 w) { *(uint2*)(stg + l16 * 128 + (((4 * j + quad) ^ (((l16 >> 1) & 7) << 1)) << 3)) = w; };
-      auto send = [&](uint16_t* o, int row) {
+      auto send = [&](uint16_t* o, int pitch, int row) {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = sr + 8 * h;
           const uint4 w = *(const uint4*)(stg + r * 128 + (((2 * sq) ^ (((r >> 1) & 7) << 1)) << 3));
-          if (row + r < p.e.M) *(uint4*)(o + (int64_t)(row + r) * p.e.N + wcol + sq * 8) = w;
+          if (row + r < p.e.M) *(uint4*)(o + (int64_t)(row + r) * pitch + wcol + sq * 8) = w;
         }
         asm volatile("" ::: "memory");
       };
@@ -569,19 +571,18 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
           if constexpr (SLOPE) {
 #pragma unroll
             for (int j = 0; j < TN; ++j) put(j, sl[j]);
-            send(p.e.slope, wrow + i * 16);
+            send(p.e.slope, slope_pitch(p.e.N), wrow + i * 16);
           }
 #pragma unroll
           for (int j = 0; j < TN; ++j) put(j, y[j]);
-          send(p.e.C, wrow + i * 16);
+          send(p.e.C, p.e.N, wrow + i * 16);
         } else {
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
             const int col = col0 + j * 16;
             if (row >= p.e.M || col >= p.e.N) continue;
-            const int64_t at = (int64_t)row * p.e.N + col;
-            if constexpr (SLOPE) store4(p.e, p.e.slope + at, col, sl[j]);
-            store4(p.e, p.e.C + at, col, y[j]);
+            if constexpr (SLOPE) *(uint2*)(p.e.slope + (int64_t)row * slope_pitch(p.e.N) + col) = sl[j];
+            store4(p.e, p.e.C + (int64_t)row * p.e.N + col, col, y[j]);
           }
         }
         asm volatile("" ::: "memory");
@@ -622,13 +623,14 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, cons
 }
 
 // ---------------------------------------------------------------------------------------------- few tokens
-// Up to 64 rows of x: the weight is read once and nothing else counts.  A workgroup takes 16 rows of W, its wavefronts an
+// Up to 32 rows of x and a weight of a few megabytes: latency is what counts.  A workgroup takes 16 rows of W, its wavefronts an
 // equal run of the reduction each; fragments go from memory to registers with no LDS between (a lane's chunk is its MFMA operand
 // as it lies), the next U steps' while the MFMAs of these run.  MFMA row: a row of W; column: a token (past the last one, the
 // last one again).  The wavefronts' sums meet in LDS and are added in their order.
-template <int TB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
+template <int TB>
+__global__ __launch_bounds__(1024) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
                                                              const bf16_t* __restrict__ w, int64_t ldw, int K) {
+  constexpr int WAVES = 16, U = 4;
   __shared__ f32x4 sums[WAVES][TB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, quad = lane >> 4;
@@ -643,7 +645,6 @@ __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p
   for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int steps = (K + 31) / 32;
   const int s0 = (int)((int64_t)steps * wave / WAVES), s1 = (int)((int64_t)steps * (wave + 1) / WAVES);
-  constexpr int U = TB == 4 ? 2 : 4;
   struct Set {
     bf16x8 w[U], x[TB][U];
   };
@@ -687,37 +688,44 @@ __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p
 // ---------------------------------------------------------------------------------------------- operands and column sums
 constexpr int kPrepCols = 256;  // columns of a workgroup: 32 threads of eight, by eight rows
 
-int lin_sum_parts(int rows) {
-  const int per = rows <= 8192 ? 64 : (rows + 1023) / 1024 * 8;  // rows of a part, a multiple of eight
-  return (rows + per - 1) / per;
-}
+// Rows of a part, a multiple of eight: about 128 parts, which fill the chip where there are few columns.
+static int sum_rows(int rows) { return (rows + 1023) / 1024 * 8; }
+int lin_sum_parts(int rows) { return (rows + sum_rows(rows) - 1) / sum_rows(rows); }
 
-// SLOPE: src is dy, and dz = dy * act'(z) goes on.  VEC: rows of src, slope and dst are whole 16-byte chunks.
-template <bool SLOPE, bool DST, bool SUM, bool VEC>
+// SLOPE: src is dy, and dz = dy * act'(z) goes on.  W: elements of src that are read at once; 8: every row is whole chunks.
+template <bool SLOPE, bool DST, bool SUM, int W>
 __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restrict__ src, int64_t ld,
                                                           const uint16_t* __restrict__ slope, int act, int rows, int cols,
                                                           bf16_t* __restrict__ dst, float* __restrict__ partial, int per) {
   __shared__ float sums[8][kPrepCols];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int c0 = blockIdx.x * kPrepCols + tx * 8, padded = (cols + 7) & ~7;
+  const int c0 = blockIdx.x * kPrepCols + tx * 8, padded = slope_pitch(cols);
   const int r_first = blockIdx.y * per, r_end = r_first + per < rows ? r_first + per : rows;
   float acc[8] = {};
   if (c0 < cols) {
+#pragma unroll 2
     for (int r = r_first + ty; r < r_end; r += 8) {
+      const bf16_t* q = src + (int64_t)r * ld + c0;
       float v[8];
-      if constexpr (VEC) {
-        st_load8<bf16_t>(src + (int64_t)r * ld + c0, 0, v);
-        if constexpr (SLOPE) {
-          const u32x4_t s = *(const u32x4_t*)(slope + (int64_t)r * cols + c0);
+      if constexpr (W == 8) {
+        st_load8<bf16_t>(q, 0, v);
+      } else if constexpr (W == 2) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= slope_unpack(act, (uint16_t)(s[e >> 1] >> (16 * (e & 1))));
+        for (int e = 0; e < 8; e += 2) {  // (an even number of columns)
+          const uint32_t w = c0 + e < cols ? *(const uint32_t*)(q + e) : 0;
+          v[e] = __uint_as_float(w << 16);
+          v[e + 1] = __uint_as_float(w & 0xffff0000u);
         }
       } else {
 #pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c0 + e < cols ? bf16_to_f32(q[e]) : 0.f;
+      }
+      if constexpr (SLOPE) {
+        const u32x4_t s = *(const u32x4_t*)(slope + (int64_t)r * padded + c0);
+#pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = c0 + e < cols ? bf16_to_f32(src[(int64_t)r * ld + c0 + e]) : 0.f;
-          if constexpr (SLOPE)
-            if (c0 + e < cols) v[e] *= slope_unpack(act, slope[(int64_t)r * cols + c0 + e]);
+          const float f = slope_unpack(act, (uint16_t)(s[e >> 1] >> (16 * (e & 1))));
+          v[e] = c0 + e < cols ? v[e] * f : 0.f;
         }
       }
       if constexpr (DST) st_store8<bf16_t>(dst + (int64_t)r * padded + c0, 0, v);
@@ -768,25 +776,28 @@ struct LinPlan {
   int splits, slabs;
 };
 static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
-  if (M <= 64 && !p_kmajor && !q_kmajor) return {kLinFew, 1, 0};
   const int KT = (K + 63) / 64;
   LinPlan best{kLin128, 1, KT};
   double least = 1e30;
   for (int t = kLin128; t <= kLin256; ++t) {
     const int bm = t == kLin128 ? 128 : 256, bn = t == kLin256 ? 256 : 128;
-    const double slab = t == kLin256 ? 1.2 : t == kLinWide ? 0.65 : 0.36, fixed = t == kLin256 ? 6.0 : t == kLinWide ? 4.0 : 3.0;
+    const double slab = t == kLin256 ? 1.65 : t == kLinWide ? 0.9 : 0.45, fixed = t == kLin256 ? 8.0 : t == kLinWide ? 5.0 : 4.5;
     const int64_t tiles = (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     for (int s = 1; s <= 16 && s <= KT; ++s) {
       const int slabs = (KT + s - 1) / s;
       const int parts = (KT + slabs - 1) / slabs;
       if (parts != s) continue;
       double us = (double)((tiles * parts + 255) / 256) * (slabs * slab + fixed);
-      if (parts > 1) us += 3.0 + (double)M * N * parts * 8.0 / 4e6;
+      if (parts > 1) us += 2.5 + (double)M * N * parts * 8.0 / 4e6;
       if (us < least) {
         least = us;
         best = {(LinTile)t, parts, slabs};
       }
     }
+  }
+  if (M <= 32 && !p_kmajor && !q_kmajor) {
+    const double wgs = (N + 15) / 16, few = 2.6 + (M <= 16 ? 0.85 : 1.3) * (K / 512.0) * (wgs > 256 ? wgs / 256 : 1);
+    if (few < least) return {kLinFew, 1, 0};
   }
   return best;
 }
@@ -849,13 +860,6 @@ static hipError_t launch_tiles(const LinProduct& p, LinTileParams tp, hipStream_
   }
 }
 
-template <int TB, int WAVES>
-static hipError_t launch_few(const LinProduct& p, const LinEpilogue& e, hipStream_t st) {
-  hipLaunchKernelGGL((lin_few_kernel<TB, WAVES>), dim3((unsigned)((p.N + 15) / 16)), dim3(WAVES * 64), 0, st, e, p.P, p.ldp, p.Q,
-                     p.ldq, p.K);
-  return hipGetLastError();
-}
-
 hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
   if (p.M <= 0 || p.N <= 0 || p.K <= 0) return hipErrorInvalidValue;
   auto whole = [](const void* ptr, int64_t ld, int extent) {
@@ -873,15 +877,14 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
   e.N = p.N;
   e.act = p.act;
   e.bias_dtype = p.bias_dtype;
-  const uint64_t bytes = ((uint64_t)p.C | (uint64_t)p.slope | (uint64_t)p.R) | (uint64_t)p.N * 2 | (p.R ? (uint64_t)p.ldr * 2 : 0);
+  const uint64_t bytes = ((uint64_t)p.C | (uint64_t)p.R) | (uint64_t)p.N * 2 | (p.R ? (uint64_t)p.ldr * 2 : 0);
   e.vec = bytes % 16 == 0 ? 8 : bytes % 8 == 0 ? 4 : bytes % 4 == 0 ? 2 : 1;
   const LinPlan plan = lin_plan(p.M, p.N, p.K, p.p_kmajor, p.q_kmajor);
   if (plan.tile == kLinFew) {
-    // sixteen wavefronts share a reduction where the rows of W alone do not fill the chip
-    const bool wide = (p.N + 15) / 16 < 1024;
-    if (p.M <= 16) return wide ? launch_few<1, 16>(p, e, st) : launch_few<1, 4>(p, e, st);
-    if (p.M <= 32) return wide ? launch_few<2, 16>(p, e, st) : launch_few<2, 4>(p, e, st);
-    return wide ? launch_few<4, 8>(p, e, st) : launch_few<4, 4>(p, e, st);
+    const dim3 grid((unsigned)((p.N + 15) / 16));
+    if (p.M <= 16) hipLaunchKernelGGL((lin_few_kernel<1>), grid, dim3(1024), 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
+    else hipLaunchKernelGGL((lin_few_kernel<2>), grid, dim3(1024), 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
+    return hipGetLastError();
   }
   LinTileParams tp;
   tp.e = e;
@@ -908,19 +911,21 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
 template <bool SLOPE, bool DST, bool SUM>
 static hipError_t launch_prepare(const bf16_t* src, int64_t ld, const uint16_t* slope, int act, int rows, int cols, bf16_t* dst,
                                  float* partial, hipStream_t st) {
-  const int parts = lin_sum_parts(rows);
-  int per = (rows + parts - 1) / parts;
-  per = (per + 7) & ~7;
-  const dim3 grid((cols + kPrepCols - 1) / kPrepCols, parts);
-  const bool vec = cols % 8 == 0 && ld % 8 == 0 && (((uint64_t)src | (uint64_t)slope | (uint64_t)dst) & 15) == 0;
-  if (vec) hipLaunchKernelGGL((lin_prepare_kernel<SLOPE, DST, SUM, true>), grid, dim3(256), 0, st, src, ld, slope, act, rows, cols, dst, partial, per);
-  else hipLaunchKernelGGL((lin_prepare_kernel<SLOPE, DST, SUM, false>), grid, dim3(256), 0, st, src, ld, slope, act, rows, cols, dst, partial, per);
+  const dim3 grid((cols + kPrepCols - 1) / kPrepCols, lin_sum_parts(rows));
+  const uint64_t bytes = (uint64_t)src | (uint64_t)cols * 2 | (uint64_t)ld * 2;
+  auto go = [&](auto wc) {
+    hipLaunchKernelGGL((lin_prepare_kernel<SLOPE, DST, SUM, decltype(wc)::value>), grid, dim3(256), 0, st, src, ld, slope, act, rows,
+                       cols, dst, partial, sum_rows(rows));
+  };
+  if (bytes % 16 == 0) go(std::integral_constant<int, 8>());
+  else if (bytes % 4 == 0) go(std::integral_constant<int, 2>());
+  else go(std::integral_constant<int, 1>());
   return hipGetLastError();
 }
 
 hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slope, int act, int rows, int cols, bf16_t* dst,
                               float* partial, hipStream_t st) {
-  if (rows <= 0 || cols <= 0 || (!dst && !partial) || (dst && ((uint64_t)dst & 15))) return hipErrorInvalidValue;
+  if (rows <= 0 || cols <= 0 || (!dst && !partial) || ((uint64_t)dst & 15) || ((uint64_t)slope & 15)) return hipErrorInvalidValue;
   if (slope) {
     if (dst && partial) return launch_prepare<true, true, true>(src, ld, slope, act, rows, cols, dst, partial, st);
     if (dst) return launch_prepare<true, true, false>(src, ld, slope, act, rows, cols, dst, partial, st);

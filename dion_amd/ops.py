@@ -1086,7 +1086,8 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation
     tokens, fan_out = x.shape[0], weight.shape[0]
     with _device_of(x):
         y = torch.empty(tokens, fan_out, dtype=torch.bfloat16, device=x.device)
-        slope = torch.empty(tokens, fan_out, dtype=torch.int16, device=x.device) if keep_slope and act else None
+        # (in whole 16-byte chunks)
+        slope = torch.empty(tokens, -(-fan_out // 8) * 8, dtype=torch.int16, device=x.device) if keep_slope and act else None
         (x, ldx), (w, ldw) = _rows(x), _rows(weight)
         r, ldr = (None, 0) if residual is None else _rows(residual)
         b = None if bias is None else bias.contiguous()

@@ -442,8 +442,8 @@ enum { DION_ACT_NONE, DION_ACT_RELU, DION_ACT_RELU_SQUARED, DION_ACT_GELU, DION_
 #define DION_LINEAR_COPY_DY 4
 size_t dion_linear_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int activation, int copies);
 
-/* y = act(x w^T + bias) + residual.  bias, residual may be null.  slope (null, or [tokens][fan_out] of 16 bits; not without an
- * activation): act' at every element, for dion_linear_backward -- fp16, of the squared relu seven bits of exponent and
+/* y = act(x w^T + bias) + residual.  bias, residual may be null.  slope (null, or [tokens][fan_out rounded up to 8] of 16 bits,
+ * 16-byte aligned; not without an activation): act' at every element, for dion_linear_backward -- fp16, of the squared relu seven bits of exponent and
  * nine of mantissa.  Neither y nor slope may overlap an operand, but y may be the residual where that is dense. */
 int dion_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
                         int activation, const void* residual, int64_t ldr, void* y, void* slope, int tokens, int fan_in,
