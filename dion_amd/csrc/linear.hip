@@ -627,10 +627,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, cons
 // equal run of the reduction each; fragments go from memory to registers with no LDS between (a lane's chunk is its MFMA operand
 // as it lies), the next U steps' while the MFMAs of these run.  MFMA row: a row of W; column: a token (past the last one, the
 // last one again).  The wavefronts' sums meet in LDS and are added in their order.
-template <int TB>
-__global__ __launch_bounds__(1024) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
+template <int TB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
                                                              const bf16_t* __restrict__ w, int64_t ldw, int K) {
-  constexpr int WAVES = 16, U = 4;
+  constexpr int U = 4;
   __shared__ f32x4 sums[WAVES][TB][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, quad = lane >> 4;
@@ -769,7 +769,11 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// How a product runs: on which tiles, and in how many parts of the reduction.
+// How a product runs: on which tiles, and in how many parts of the reduction: what is estimated to take least.  A round of the
+// 256 CUs takes so much a slab and so much for itself (first loads, epilogue).  Measured, us, reductions of 1024 / 8192: one
+// round of 128-wide tiles 12.9 / 63, of 256 x 128 21 / 122, of 256-wide 34 / 224; of 64 128-wide tiles the slab costs 0.37 instead of
+// 0.45 (the clock, on this power-limited part, and L2).  Splitting pays where a round is not full: 32 tokens of 2048 x 8192, 16
+// tiles, in 1 / 4 / 16 parts 46 / 16.8 / 10.8 us with the kernel that joins them.
 enum LinTile { kLinFew, kLin128, kLinWide, kLin256 };
 struct LinPlan {
   LinTile tile;
@@ -779,6 +783,7 @@ static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
   const int KT = (K + 63) / 64;
   LinPlan best{kLin128, 1, KT};
   double least = 1e30;
+  const double streaming = 4.0 + 2.0 * ((double)M * K + (double)N * K + (double)M * N) / 5e6;
   for (int t = kLin128; t <= kLin256; ++t) {
     const int bm = t == kLin128 ? 128 : 256, bn = t == kLin256 ? 256 : 128;
     const double slab = t == kLin256 ? 1.65 : t == kLinWide ? 0.9 : 0.45, fixed = t == kLin256 ? 8.0 : t == kLinWide ? 5.0 : 4.5;
@@ -788,6 +793,7 @@ static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
       const int parts = (KT + slabs - 1) / slabs;
       if (parts != s) continue;
       double us = (double)((tiles * parts + 255) / 256) * (slabs * slab + fixed);
+      if (us < streaming) us = streaming;
       if (parts > 1) us += 2.5 + (double)M * N * parts * 8.0 / 4e6;
       if (us < least) {
         least = us;
@@ -796,8 +802,8 @@ static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
     }
   }
   if (M <= 32 && !p_kmajor && !q_kmajor) {
-    const double wgs = (N + 15) / 16, few = 2.6 + (M <= 16 ? 0.85 : 1.3) * (K / 512.0) * (wgs > 256 ? wgs / 256 : 1);
-    if (few < least) return {kLinFew, 1, 0};
+    const double wgs = (N + 15) / 16, each = M <= 16 ? 0.77 + 0.033 * (M - 1) : 1.5;
+    if (2.5 + each * (K / 512.0) * (wgs > 256 ? wgs / 256 : 1) < least) return {kLinFew, 1, 0};
   }
   return best;
 }
@@ -882,8 +888,16 @@ hipError_t launch_lin_product(const LinProduct& p, hipStream_t st) {
   const LinPlan plan = lin_plan(p.M, p.N, p.K, p.p_kmajor, p.q_kmajor);
   if (plan.tile == kLinFew) {
     const dim3 grid((unsigned)((p.N + 15) / 16));
-    if (p.M <= 16) hipLaunchKernelGGL((lin_few_kernel<1>), grid, dim3(1024), 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
-    else hipLaunchKernelGGL((lin_few_kernel<2>), grid, dim3(1024), 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
+    auto go = [&](auto tbc, auto wavesc) {
+      constexpr int TB = decltype(tbc)::value, WAVES = decltype(wavesc)::value;
+      hipLaunchKernelGGL((lin_few_kernel<TB, WAVES>), grid, dim3(WAVES * 64), 0, st, e, p.P, p.ldp, p.Q, p.ldq, p.K);
+    };
+    // Sixteen wavefronts share a reduction, or four where the rows of W make two workgroups of those per CU: one token of
+    // 14336 x 4096 26.0 / 24.0 us, of 50304 x 768 33.5 / 15.8, of 4096 x 14336 24.0 / 26.5, of 2048 x 8192 11.4 / 13.6.
+    typedef std::integral_constant<int, 16> many;
+    if (p.M > 16) go(std::integral_constant<int, 2>(), many());
+    else if (p.N >= 8192) go(std::integral_constant<int, 1>(), std::integral_constant<int, 4>());
+    else go(std::integral_constant<int, 1>(), many());
     return hipGetLastError();
   }
   LinTileParams tp;

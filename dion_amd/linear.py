@@ -10,17 +10,19 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
+def _rows(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation, residual):
         need = ctx.needs_input_grad
-        rows = x.reshape(-1, x.shape[-1])
-        r = None if residual is None else residual.reshape(-1, weight.shape[0])
-        y, slope = ops.linear_forward(rows, weight, bias, activation, r, keep_slope=need[0] or need[1] or need[2])
+        y, slope = ops.linear_forward(_rows(x), weight, bias, activation, _rows(residual), need[0] or need[1] or need[2])
         ctx.save_for_backward(x if need[1] else None, weight, slope)
         ctx.activation, ctx.lead = activation, x.shape[:-1]
         ctx.bias_dtype = bias.dtype if bias is not None and need[2] else None
-        return y.view(*x.shape[:-1], weight.shape[0])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -29,10 +31,9 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[1] or ctx.bias_dtype is not None:
-            rows = None if x is None else x.reshape(-1, x.shape[-1])
-            dx, dw, db = ops.linear_backward(dy.reshape(-1, weight.shape[0]), slope, ctx.activation, rows, weight, need[0],
-                                             need[1], ctx.bias_dtype)
-            if dx is not None:
+            dx, dw, db = ops.linear_backward(_rows(dy), slope, ctx.activation, _rows(x), weight, need[0], need[1],
+                                             ctx.bias_dtype)
+            if dx is not None and len(ctx.lead) != 1:
                 dx = dx.view(*ctx.lead, weight.shape[1])
         return dx, dw, db, None, dy if need[4] else None
 
@@ -48,8 +49,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     products, not for the bias.  Any sizes and strides; rows that are not whole 16-byte chunks (feature counts that are not
     multiples of 8) are copied first."""
     ops.check_linear(x, weight, bias, activation, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, activation, residual)
-    r = None if residual is None else residual.reshape(-1, weight.shape[0])
-    y, _slope = ops.linear_forward(x.reshape(-1, x.shape[-1]), weight, bias, activation, r, keep_slope=False)
-    return y.view(*x.shape[:-1], weight.shape[0])
+    y, _slope = ops.linear_forward(_rows(x), weight, bias, activation, _rows(residual), False)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])

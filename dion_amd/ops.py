@@ -5,6 +5,7 @@ hands raw device pointers and the current stream to the library, and returns tor
 torch is used for device memory and streams only; all arithmetic happens in the HIP kernels.
 There is no CPU implementation behind these functions: CPU tensors raise.
 """
+import functools
 import math
 from typing import List, Optional, Sequence, Tuple
 
@@ -20,6 +21,9 @@ def _stream_handle(device: torch.device) -> int:
     index = device.index
     # (the handle alone: a Stream object per launch was 2 us of host time)
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+
+
+_PLAIN = (Tensor, torch.nn.Parameter)  # neither has an inner tensor
 
 
 def _require_gpu(t: Tensor, name: str) -> None:
@@ -901,36 +905,53 @@ def dion2_post_masked(X: List[Tensor], M: List[Tensor], U: Tensor, norms: Tensor
 # ---------------------------------------------------------------------------------------------
 # multi-tensor AdamW / Lion for the non-matrix parameter groups
 # ---------------------------------------------------------------------------------------------
+def _pointers(ts: List[Tensor], name: str, dtype: torch.dtype, numels: List[int], index: int, what: str) -> List[int]:
+    """Addresses of a list's tensors: dense, of one dtype, on one device, of the given sizes.  (A step passes hundreds of tensors
+    through here: the properties are read in one go, and looked at one by one only to say what is wrong.)"""
+    if len(ts) != len(numels):
+        raise ValueError(f"{name}: expected {len(numels)} tensors, got {len(ts)}")
+    seen = [(t.numel(), t.dtype, t.get_device(), t.is_contiguous()) for t in ts]
+    if seen != [(n, dtype, index, True) for n in numels] or not set(map(type, ts)) <= _PLAIN_SET:
+        for t, n in zip(ts, numels):
+            _require_gpu(t, name)
+            if t.get_device() != index:
+                raise ValueError(f"{name}: tensors of one call must be on one device, got {t.device} beside device {index}")
+            if t.dtype != dtype or not t.is_contiguous() or t.numel() != n:
+                raise ValueError(f"{name}: {what}")
+    return [t.data_ptr() for t in ts]
+
+
+_PLAIN_SET = set(_PLAIN)
+
+
 def _mta_tables(X: List[Tensor], G: List[Tensor], states: List[List[Tensor]], state_dtype=None):
     """Tables of pointers and sizes.  The states are in ``state_dtype``, or in that of X."""
     n = len(X)
     assert n > 0 and len(G) == n and all(len(s) == n for s in states)
-    gdt = G[0].dtype
-    xdt = X[0].dtype
+    x0, gdt = X[0], G[0].dtype
+    if not set(map(type, X)) <= _PLAIN_SET or not x0.is_cuda:
+        for x in X:
+            _require_gpu(x, "X")
+    xdt, index = x0.dtype, x0.get_device()
     sdt = state_dtype or xdt
-    for x, g in zip(X, G):
-        _require_gpu(x, "X")
-        _require_gpu(g, "G")
-        if x.dtype != xdt:
-            raise TypeError("X: one parameter dtype per call")
-        if g.dtype != gdt:
-            raise TypeError("G: one gradient dtype per call")
-        if not x.is_contiguous() or not g.is_contiguous() or g.numel() != x.numel():
-            raise ValueError("X / G must be contiguous and of equal size")
+    if any(x.dtype != xdt for x in X):
+        raise TypeError("X: one parameter dtype per call")
+    if any(g.dtype != gdt for g in G):
+        raise TypeError("G: one gradient dtype per call")
+    sizes = [x.numel() for x in X]
+    dense = "X / G must be contiguous and of equal size"
+    tabs = [ptr_table(_pointers(X, "X", xdt, sizes, index, dense)), ptr_table(_pointers(G, "G", gdt, sizes, index, dense))]
     for name, st in zip("MV", states):
-        for x, s in zip(X, st):
-            if s.dtype != sdt or not s.is_contiguous() or s.numel() != x.numel() or not s.is_cuda:
-                raise ValueError(f"{name}: optimizer state must be contiguous GPU tensors shaped like X, in the "
-                                 f"dtype of X ({sdt})")
-    numels = (_lib.ctypes.c_int64 * n)(*[x.numel() for x in X])
-    tabs = [ptr_table([t.data_ptr() for t in ts]) for ts in (X, G, *states)]
-    return tabs, numels, _dtype_code(G[0], "G"), _dtype_code(X[0], "X")
+        tabs.append(ptr_table(_pointers(st, name, sdt, sizes, index, "optimizer state must be contiguous GPU tensors shaped "
+                                        f"like X, in the dtype of X ({sdt})")))
+    return tabs, (_lib.ctypes.c_int64 * n)(*sizes), _dtype_code(G[0], "G"), _dtype_code(x0, "X")
 
 
-def _check_steps(steps: List[Tensor]) -> None:
+def _check_steps(steps: List[Tensor]) -> List[int]:
     for s in steps:
-        if not (s.is_cuda and s.dtype == torch.float32 and s.numel() == 1):
+        if s.dtype != torch.float32 or s.numel() != 1 or not s.is_cuda:
             raise TypeError("steps must be 0-d float32 GPU tensors")
+    return [s.data_ptr() for s in steps]
 
 
 def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor], steps: List[Tensor],
@@ -941,8 +962,7 @@ def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor
     have the dtype of ``X``, or are float32 beside bfloat16 parameters."""
     wide = len(M) > 0 and M[0].dtype == torch.float32 and X[0].dtype == torch.bfloat16
     (xp, gp, mp, vp), numels, gcode, xcode = _mta_tables(X, G, [M, V], torch.float32 if wide else None)
-    _check_steps(steps)
-    sp = ptr_table([s.data_ptr() for s in steps])
+    sp = ptr_table(_check_steps(steps))
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     lib = _lib.load()
     rest = (sp, numels, len(X), lr_p, float(beta1), float(beta2), float(epsilon), wd_p, wd_h, int(bool(cautious_wd)),
@@ -973,20 +993,19 @@ def adamw8_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: Lis
     if any(len(t) != n for t in (G, M, M_scales, V, V_scales, steps)):
         raise ValueError("adamw8_step: all lists must have one tensor for every parameter")
     (xp, gp), numels, gcode, xcode = _mta_tables(X, G, [])
+    sizes, index = list(numels), X[0].get_device()
+    blocks = [state8_blocks(k) for k in sizes]
+    tabs = []
     for name, dtype, codes, scales in (("M", torch.int8, M, M_scales), ("V", torch.uint8, V, V_scales)):
-        for x, c, s in zip(X, codes, scales):
-            _require_gpu(c, name)
-            _require_gpu(s, name + "_scales")
-            if c.dtype != dtype or not c.is_contiguous() or c.numel() != x.numel():
-                raise ValueError(f"{name}: codes must be contiguous {dtype} tensors shaped like X")
-            if s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != state8_blocks(x.numel()):
-                raise ValueError(f"{name}_scales: one contiguous float32 scale for every {STATE8_BLOCK} elements of X")
-    _check_steps(steps)
+        tabs.append(ptr_table(_pointers(codes, name, dtype, sizes, index, f"codes must be contiguous {dtype} tensors shaped like X")))
+        tabs.append(ptr_table(_pointers(scales, name + "_scales", torch.float32, blocks, index,
+                                        f"one contiguous float32 scale for every {STATE8_BLOCK} elements of X")))
+    tabs.append(ptr_table(_check_steps(steps)))
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
-    tabs = [ptr_table([t.data_ptr() for t in ts]) for ts in (M, M_scales, V, V_scales, steps)]
-    check(_lib.load().dion_adamw8_step(xp, xcode, gp, gcode, *tabs, numels, n, lr_p, float(beta1), float(beta2),
-                                       float(epsilon), wd_p, wd_h, int(bool(cautious_wd)), _as_int32(seed),
-                                       _stream_handle(X[0].device)), "adamw8_step")
+    with _device_of(X[0]):
+        check(_lib.load().dion_adamw8_step(xp, xcode, gp, gcode, *tabs, numels, n, lr_p, float(beta1), float(beta2),
+                                           float(epsilon), wd_p, wd_h, int(bool(cautious_wd)), _as_int32(seed),
+                                           _stream_handle(X[0].device)), "adamw8_step")
 
 
 def _as_int32(seed: int) -> int:
@@ -1000,6 +1019,8 @@ def state8_values(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.floa
     square of that for uint8 codes (second moments)."""
     _require_gpu(codes, "codes")
     _require_gpu(scales, "scales")
+    if codes.device != scales.device:
+        raise ValueError(f"scales are on {scales.device}, codes on {codes.device}")
     if codes.dtype not in (torch.int8, torch.uint8):
         raise TypeError(f"codes: dtype {codes.dtype} not supported (int8 or uint8)")
     if not codes.is_contiguous() or not scales.is_contiguous():
@@ -1007,9 +1028,10 @@ def state8_values(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.floa
     if scales.dtype != torch.float32 or scales.numel() != state8_blocks(codes.numel()):
         raise ValueError(f"scales: one float32 scale for every {STATE8_BLOCK} codes")
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    check(_lib.load().dion_state8_values(codes.data_ptr(), int(codes.dtype == torch.uint8), scales.data_ptr(),
-                                         codes.numel(), out.data_ptr(), _dtype_code(out, "dtype"),
-                                         _stream_handle(codes.device)), "state8_values")
+    with _device_of(codes):
+        check(_lib.load().dion_state8_values(codes.data_ptr(), int(codes.dtype == torch.uint8), scales.data_ptr(),
+                                             codes.numel(), out.data_ptr(), _dtype_code(out, "dtype"),
+                                             _stream_handle(codes.device)), "state8_values")
     return out
 
 
@@ -1041,14 +1063,15 @@ def _whole_chunks(t: Tensor, ld: int) -> bool:
     return t.data_ptr() % 16 == 0 and ld % 8 == 0 and t.shape[1] % 8 == 0 and ld <= 1 << 21
 
 
-def _check_linear(name: str, t: Tensor, shape, device, dtypes=(torch.bfloat16,)) -> None:
-    _require_gpu(t, name)
-    if t.device != device:
-        raise ValueError(f"linear: {name} is on {t.device}, x on {device}")
-    if t.dtype not in dtypes:
-        raise TypeError(f"linear: {name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"linear: expected {name} of shape {shape}, got {tuple(t.shape)}")
+def _check_linear(name: str, t: Tensor, shape, index: int, fp32: bool = False) -> None:
+    if type(t) not in _PLAIN or not t.is_cuda:
+        _require_gpu(t, name)
+    if t.dtype != torch.bfloat16 and not (fp32 and t.dtype == torch.float32):
+        raise TypeError(f"linear: {name} must be torch.bfloat16{' or torch.float32' if fp32 else ''}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"linear: expected {name} of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.get_device() != index:
+        raise ValueError(f"linear: {name} is on {t.device}, x on device {index}")
 
 
 def check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
@@ -1056,21 +1079,28 @@ def check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: 
     """Raises for what ``linear_forward`` does not take (``x`` of any number of dimensions)."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear: x of shape {tuple(x.shape)} does not fit a weight of shape {tuple(weight.shape)}")
-    if weight.numel() == 0:
-        raise ValueError(f"linear: empty weight of shape {tuple(weight.shape)}")
-    _check_linear("x", x, tuple(x.shape), x.device)
-    _check_linear("weight", weight, tuple(weight.shape), x.device)
+    xs, ws = x.shape, weight.shape
+    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1]:
+        raise ValueError(f"linear: x of shape {tuple(xs)} does not fit a weight of shape {tuple(ws)}")
+    if ws[0] == 0 or ws[1] == 0:
+        raise ValueError(f"linear: empty weight of shape {tuple(ws)}")
+    index = x.get_device()
+    _check_linear("x", x, xs, index)
+    _check_linear("weight", weight, ws, index)
     if bias is not None:
-        _check_linear("bias", bias, (weight.shape[0],), x.device, (torch.bfloat16, torch.float32))
+        _check_linear("bias", bias, ws[:1], index, fp32=True)
     if residual is not None:
-        _check_linear("residual", residual, (*x.shape[:-1], weight.shape[0]), x.device)
+        _check_linear("residual", residual, xs[:-1] + ws[:1], index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(tokens: int, fan_in: int, fan_out: int, backward: bool, act: int, copies: int) -> int:
+    return _lib.load().dion_linear_workspace_bytes(tokens, fan_in, fan_out, int(backward), act, copies)
 
 
 def _linear_space(tokens: int, weight: Tensor, backward: bool, act: int, copies: int) -> Tuple[Optional[Tensor], int]:
     # (the caching allocator's: a captured graph has its own, and no two calls in flight share one)
-    nbytes = _lib.load().dion_linear_workspace_bytes(tokens, weight.shape[1], weight.shape[0], int(backward), act, copies)
+    nbytes = _linear_bytes(tokens, weight.shape[1], weight.shape[0], backward, act, copies)
     return (torch.empty(nbytes, dtype=torch.uint8, device=weight.device) if nbytes else None), nbytes
 
 
