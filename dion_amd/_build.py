@@ -21,8 +21,7 @@ HIPCC_FLAGS = [
 
 # The step kernels keep the reference's separate multiply / add roundings (mul_ then add_), so no
 # FMA contraction there; the GEMM epilogues may contract.
-EXTRA_FLAGS = {"elementwise.hip": ["-ffp-contract=off"], "select_scope.hip": ["-ffp-contract=off"], "scalar_opts.hip": ["-ffp-contract=off"],
-               "adamw8.hip": ["-ffp-contract=off"]}
+EXTRA_FLAGS = {"elementwise.hip": ["-ffp-contract=off"], "select_scope.hip": ["-ffp-contract=off"], "scalar_opts.hip": ["-ffp-contract=off"]}
 
 
 def hipcc_path() -> str:

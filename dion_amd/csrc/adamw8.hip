@@ -5,19 +5,20 @@
 //   V  uint8 codes k, one fp32 scale q per block:  v = (k q)^2,  q = max sqrt(v) / 255
 // V's codes are linear in sqrt(v), the quantity the update divides by: the root that the denominator needs is the one
 // that is coded, and a block holds second moments down to 1 / 65025 of its largest.  Arithmetic between reading and writing
-// the codes is fp32, in the order of adamw_one (scalar_opts.hip), every operation rounded on its own.
+// the codes is fp32 with fused multiply-adds; root and quotient are the hardware's (1 ulp each).
 //
 // Rounding to a code is up or down at random, unbiased in m and in v:  c = floor(m / s + u),  k = floor(t) or one more
 // with probability (t^2 - floor(t)^2) / (2 floor(t) + 1), t = sqrt(v) / q.  A step changes v by 1 - beta2 of the difference to g^2,
 // less than half a code (1 / 127 of v near the top of a block, more below) for beta2 = 0.99: rounded to nearest, v would
 // never move.  u in [0, 1) comes from a hash of (seed, step counter, element / 8), spread over the eight elements by a
 // Weyl sequence: the noise of an element is independent from step to step, and a run repeats bit for bit.
-// A second moment above zero keeps a code of at least 1 (unless its whole block is below 1e-30): m may outlive it, and
+// A second moment above zero (the normal numbers of fp32) keeps a code of at least 1: m may outlive it, and
 // nothing may then be divided by epsilon.  First moments of a block whose largest is below 1e-30 are dropped (127 / max would
 // overflow).  A block with a value that is not finite gets a scale of NaN, so that it shows in every later step.
 //
 // Bound by HBM: fp32 parameters, bf16 gradients 14.1 bytes per element (26 with fp32 states): X both ways 8, G 2, codes
-// 4, scales 0.125.
+// 4, scales 0.125.  That leaves about a hundred vector instructions an element (seventy with bf16 parameters), which a plain
+// translation of the formulas takes up: @@FIGURES@@
 #include "elementwise.h"
 
 namespace dion {
@@ -34,7 +35,6 @@ struct Adam8Tensors {
 
 struct Adam8Scalars {
   float beta1, beta2, eps, wd_host;
-  int cautious;
   uint32_t seed;
 };
 
@@ -100,7 +100,7 @@ static __device__ __forceinline__ void raw_values(const Raw8<T>& r, float v[8]) 
   }
 }
 
-template <typename GT, typename XT, bool NT>
+template <typename GT, typename XT, bool NT, bool CAUTIOUS>
 __global__ __launch_bounds__(256) void adamw8_kernel(Adam8Tensors a, int n, const float* __restrict__ lr_dev,
                                                      const float* __restrict__ wd_dev, Adam8Scalars sc) {
   int t = 0;
@@ -147,79 +147,75 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adam8Tensors a, int n, cons
   const float inv_bc2_sqrt = 1.0f / sqrtf(1.0f - powf(sc.beta2, step));
   const float adj_lr = lr / (1.0f - powf(sc.beta1, step));
   const float coeff = lr * wd, keep = 1.0f - coeff;
-  const float w1 = 1.0f - sc.beta1, w2 = 1.0f - sc.beta2;
   const uint32_t key = mix32(mix32(sc.seed) + (uint32_t)step);
 
+  const float w1 = 1.0f - sc.beta1, w2 = 1.0f - sc.beta2;
   for (int r = 0; r < a.rounds; ++r, e0 += kA8Round) {
     if (first + (int64_t)r * kA8Round >= numel) break;  // (the same for the whole workgroup)
     const int left = numel - e0 >= 8 ? 8 : numel > e0 ? (int)(numel - e0) : 0;
     const bool whole = vec && left == 8;
-    float xv[8], gv[8], mv[8], vv[8];
-    const float s = s_old, q = q_old;
+    float xv[8], gv[8];
+    u32x2_t mb, vb;  // codes, first moments' plus 128
+    const float s = s_old, s128 = -128.0f * s_old, q = q_old;
     if (whole) {
       raw_values<XT>(xr, xv);
       raw_values<GT>(gr, gv);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mv[e] = (float)(int8_t)(mr[e >> 2] >> (8 * (e & 3)));
-        vv[e] = (float)(uint8_t)(vr[e >> 2] >> (8 * (e & 3)));
-      }
+      mb = mr ^ 0x80808080u;
+      vb = vr;
     } else {
+      // (zeros where the tensor has ended, which change nothing)
+      mb = u32x2_t{0x80808080u, 0x80808080u};
+      vb = u32x2_t{0, 0};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const bool in = e < left;
         xv[e] = in ? st_load<XT>(x, e0 + e) : 0.f;
         gv[e] = in ? st_load<GT>(g, e0 + e) : 0.f;
-        mv[e] = in ? (float)m[e0 + e] : 0.f;
-        vv[e] = in ? (float)v[e0 + e] : 0.f;
+        if (in) {
+          mb[e >> 2] ^= (uint32_t)(uint8_t)m[e0 + e] << (8 * (e & 3));
+          vb[e >> 2] |= (uint32_t)v[e0 + e] << (8 * (e & 3));
+        }
       }
     }
     if (r + 1 < a.rounds) fetch(e0 + kA8Round);
-    float rt[8];
+    float mv[8], rt[8];
     uint32_t mtop = 0, rtop = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float m0 = mv[e] * s, r0 = vv[e] * q;
-      mv[e] = m0 + w1 * (gv[e] - m0);
-      const float v1 = r0 * r0 * sc.beta2 + w2 * (gv[e] * gv[e]);
-      rt[e] = sqrtf(v1);
-      const float upd = mv[e] / (rt[e] * inv_bc2_sqrt + sc.eps);
-      if (sc.cautious) {
-        if (upd * xv[e] >= 0.0f) xv[e] = xv[e] - xv[e] * coeff;
-      } else {
-        xv[e] = xv[e] * keep;
-      }
-      xv[e] = xv[e] - adj_lr * upd;
-      if (e < left) {
-        mtop = max(mtop, __float_as_uint(mv[e]) & 0x7fffffffu);
-        rtop = max(rtop, __float_as_uint(rt[e]) & 0x7fffffffu);
-      }
+      const float m0 = fmaf((float)((mb[e >> 2] >> (8 * (e & 3))) & 0xffu), s, s128);
+      const float r0 = (float)((vb[e >> 2] >> (8 * (e & 3))) & 0xffu) * q;
+      mv[e] = fmaf(w1, gv[e] - m0, m0);
+      rt[e] = __builtin_amdgcn_sqrtf(fmaf(w2 * gv[e], gv[e], r0 * r0 * sc.beta2));
+      const float upd = mv[e] * __builtin_amdgcn_rcpf(fmaf(rt[e], inv_bc2_sqrt, sc.eps));
+      if constexpr (CAUTIOUS) xv[e] = upd * xv[e] >= 0.0f ? fmaf(-coeff, xv[e], xv[e]) : xv[e];
+      else xv[e] *= keep;
+      xv[e] = fmaf(-adj_lr, upd, xv[e]);
+      mtop = max(mtop, __float_as_uint(mv[e]) & 0x7fffffffu);
+      rtop = max(rtop, __float_as_uint(rt[e]));
     }
     float minv, mscale, rinv, rscale;
     block_scale(block_max(mtop), 127.0f, minv, mscale);
     block_scale(block_max(rtop), 255.0f, rinv, rscale);
     const uint32_t h = mix32(key ^ (uint32_t)(e0 >> 3));
-    uint32_t mc[8], vc[8];
+    u32x2_t mo = {0, 0}, vo = {0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float u = (float)((h + (uint32_t)e * 0x9E3779B9u) >> 8) * 0x1p-24f;
-      // (a scale of zero or NaN has an inverse of zero: codes of zero, also from 0 * infinity, which the clamp drops)
-      const float c = fminf(fmaxf(floorf(mv[e] * minv + u), -127.0f), 127.0f);
-      mc[e] = (uint32_t)(int)(minv > 0.0f ? c : 0.0f) & 0xffu;
-      const float tt = rt[e] * rinv;
-      float k = fminf(floorf(tt), 255.0f);
-      if (u * (2.0f * k + 1.0f) < (tt - k) * (tt + k)) k = fminf(k + 1.0f, 255.0f);
-      if (rt[e] > 0.0f) k = fmaxf(k, 1.0f);
-      vc[e] = (uint32_t)(rinv > 0.0f ? k : 0.0f);
+      // m / s + u, plus 128: an unsigned code (a scale of zero or NaN has an inverse of zero)
+      const float c = floorf(fmaf(mv[e], minv, u + 128.0f));
+      mo[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(c, 1.0f, 255.0f), e & 3, mo[e >> 2]);
+      const float t = rt[e] * rinv, k = floorf(t);
+      const float up = fmaf(u, fmaf(2.0f, k, 1.0f), k * k) < t * t ? k + 1.0f : k;
+      const float least = __builtin_amdgcn_fmed3f(rt[e] * 0x1p127f, 0.0f, 1.0f);  // 1 where v > 0
+      vo[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(up, least, 255.0f), e & 3, vo[e >> 2]);
     }
+    mo ^= 0x80808080u;
     if (left > 0 && (threadIdx.x & 15) == 0) {
       ms[e0 >> 7] = mscale;
       vs[e0 >> 7] = rscale;
     }
     if (whole) {
       st_store8<XT, NT>(x + e0, 0, xv);
-      const u32x2_t mo = {mc[0] | mc[1] << 8 | mc[2] << 16 | mc[3] << 24, mc[4] | mc[5] << 8 | mc[6] << 16 | mc[7] << 24};
-      const u32x2_t vo = {vc[0] | vc[1] << 8 | vc[2] << 16 | vc[3] << 24, vc[4] | vc[5] << 8 | vc[6] << 16 | vc[7] << 24};
       if constexpr (NT) {
         __builtin_nontemporal_store(mo, (u32x2_t*)(m + e0));
         __builtin_nontemporal_store(vo, (u32x2_t*)(v + e0));
@@ -232,8 +228,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adam8Tensors a, int n, cons
       for (int e = 0; e < 8; ++e) {
         if (e >= left) continue;
         st_store<XT>(x, e0 + e, xv[e]);
-        m[e0 + e] = (int8_t)mc[e];
-        v[e0 + e] = (uint8_t)vc[e];
+        m[e0 + e] = (int8_t)(mo[e >> 2] >> (8 * (e & 3)));
+        v[e0 + e] = (uint8_t)(vo[e >> 2] >> (8 * (e & 3)));
       }
     }
   }
@@ -302,11 +298,12 @@ hipError_t launch_adamw8(const uint64_t* X, int x_dtype, const uint64_t* G, int 
   hipLaunchKernelGGL(adamw8_advance_steps_kernel, dim3(1), dim3(64), 0, st, a, n);
   if (wg == 0) return hipGetLastError();
   const bool nt = exceeds_caches(total * (2 + (x_dtype == 0 ? 2 : 4) + (g_dtype == 0 ? 2 : 4)));
-  const Adam8Scalars sc{beta1, beta2, eps, wd_host, cautious, seed};
+  const Adam8Scalars sc{beta1, beta2, eps, wd_host, seed};
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)wg), dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); };
 #define A8_LAUNCH(GT, XT)                                                                                              \
   do {                                                                                                                 \
-    if (nt) hipLaunchKernelGGL((adamw8_kernel<GT, XT, true>), dim3((unsigned)wg), dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); \
-    else hipLaunchKernelGGL((adamw8_kernel<GT, XT, false>), dim3((unsigned)wg), dim3(256), 0, st, a, n, lr_dev, wd_dev, sc);   \
+    if (cautious) nt ? launch(adamw8_kernel<GT, XT, true, true>) : launch(adamw8_kernel<GT, XT, false, true>);         \
+    else nt ? launch(adamw8_kernel<GT, XT, true, false>) : launch(adamw8_kernel<GT, XT, false, false>);                \
   } while (0)
   if (g_dtype == 0) {
     if (x_dtype == 0) A8_LAUNCH(bf16_t, bf16_t); else A8_LAUNCH(bf16_t, float);

@@ -220,6 +220,7 @@ struct LinTileParams {
   float* part;  // [splits][M][N] sums, where the reduction is split
   int tilesM, tilesN, splits, slabs;  // slabs: of 64, per split
   int total, grid;                    // tiles of the list, workgroups
+  int interleave;
   uint32_t inv_tiles, inv_group, inv_tail;
 };
 
@@ -239,14 +240,15 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
 
-  // ---- tile `pid` of the list: every XCD has one contiguous run of it, eight rows of tiles at a time, columns first within them
+  // ---- tile `pid` of the list, eight rows of tiles at a time, columns first within them.  Every XCD has one contiguous run of it,
+  // or (p.interleave) 32 consecutive tiles of every 256, those behind the last whole 256 in runs again.
   struct Tile {
     int part, ti, tj, KT;  // KT: slabs of its reduction
   };
   auto tile = [&](int pid) __attribute__((always_inline)) {
     Tile t;
-    const int xcd = pid & 7, q = p.total >> 3, r = p.total & 7;
-    const int lt = xcd * q + (xcd < r ? xcd : r) + (pid >> 3);
+    const int base = p.interleave ? p.total & ~255 : 0, xcd = pid & 7, q = (p.total - base) >> 3, r = p.total & 7;
+    const int lt = pid < base ? (pid & ~255) + xcd * 32 + ((pid & 255) >> 3) : base + xcd * q + (xcd < r ? xcd : r) + ((pid - base) >> 3);
     int in_part, tg;
     t.part = div_known(lt, p.tilesM * p.tilesN, p.inv_tiles, in_part);
     const int first = div_known(in_part, 8 * p.tilesN, p.inv_group, tg) * 8;
@@ -849,6 +851,11 @@ static hipError_t launch_tiles(const LinProduct& p, LinTileParams tp, hipStream_
   tp.inv_tiles = (uint32_t)(0xffffffffu / ((int64_t)tp.tilesM * tp.tilesN));
   tp.inv_group = (uint32_t)(0xffffffffu / (8 * (int64_t)tp.tilesN));
   tp.inv_tail = tp.tilesM % 8 ? 0xffffffffu / (tp.tilesM % 8) : 0;
+  // P past the 256 MB memory-side cache, Q well within it: the XCDs then work on the same rows of P at the same time.  us, a run
+  // for each XCD / interleaved: 16384 x 4096 x 14336 1531 / 1434, with W K-major 1501 / 1436, 14336 x 4096 x 16384 both K-major
+  // 1729 / 1615, 32768 x 4096 x 8192 1740 / 1615; with Q as large 16384 x 8192 x 16384 3369 / 3534, with P the smaller one
+  // 4096 x 14336 x 16384 1571 / 1629.
+  tp.interleave = Cfg::BM == 256 && Cfg::BN == 256 && (int64_t)p.M * p.K >= (int64_t(128) << 20) && (int64_t)p.N * p.K <= (int64_t(96) << 20);
   const bool split = tp.splits > 1;
   if (p.p_kmajor)
     return split ? launch_tile<Cfg, true, true, kActNone, false, true>(tp, st) : launch_tile<Cfg, true, true, kActNone, false, false>(tp, st);

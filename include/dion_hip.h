@@ -487,7 +487,7 @@ int dion_adamw_fp32_state_step(const uint64_t* X_ptrs, int x_dtype, const uint64
  * m and in v, by u = ((h + j 0x9E3779B9) mod 2^32 >> 8) 2^-24 for element 8 i + j of a tensor, h = mix(key ^ i), key =
  * mix(mix(seed) + step) (mix: adamw8.hip):  c = floor(m / s + u);  k = floor(t), t = sqrt(v) / q, or one more where
  * u (2 k + 1) < t^2 - k^2.  v > 0 keeps k >= 1.  Zeroed codes and scales are the state before the first step.  First moments of a
- * block whose largest is below 1e-30, and second ones below 1e-60, become zero; a value that is not finite makes the scale of
+ * block whose largest is below 1e-30, and second ones below fp32's normal numbers, become zero; a value that is not finite makes the scale of
  * its block NaN.  Codes, parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
 int dion_adamw8_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype, const uint64_t* M_ptrs,
                      const uint64_t* M_scale_ptrs, const uint64_t* V_ptrs, const uint64_t* V_scale_ptrs,

@@ -50,6 +50,8 @@ def oracle(x, g, c, s, k, q, lr, wd, step, cautious, seed):
     off = lr / (1 - B1 ** step) * m_off / (np.sqrt(v / (1 - B2 ** step)) + EPS)
     x_off = 2.0 ** -23 * np.abs(x)  # of the decay: 1 - lr wd is rounded, and its product with x, which the move may cancel
     upd = m / (1 - B1 ** step) / (np.sqrt(v / (1 - B2 ** step)) + EPS)
+    if cautious:  # where m is smaller than what it is off by, its sign is open, and with it whether x decays
+        x_off = x_off + lr * wd * np.abs(x) * (np.abs(m) <= m_off)
     x = np.where(upd * x >= 0, x * (1 - lr * wd), x) if cautious else x * (1 - lr * wd)
     x = x - lr * upd
     off = off + 2e-6 * np.abs(lr * upd) + x_off + 2.0 ** -24 * np.abs(x)
