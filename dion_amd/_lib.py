@@ -159,6 +159,6 @@ def check(rc: int, what: str) -> None:
         raise DionHipError(f"{what} failed ({rc}): {msg}")
 
 
-def ptr_table(ptrs):
-    """Host array of device pointers for the *_ptrs arguments."""
-    return (ctypes.c_uint64 * len(ptrs))(*ptrs)
+def ptr_table(ptrs, n=None):
+    """Host array of device pointers for the *_ptrs arguments (``n``: their number, where ``ptrs`` is an iterator)."""
+    return (ctypes.c_uint64 * (len(ptrs) if n is None else n))(*ptrs)

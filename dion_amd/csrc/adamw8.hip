@@ -278,7 +278,10 @@ hipError_t launch_adamw8(const uint64_t* X, int x_dtype, const uint64_t* G, int 
   Adam8Tensors a;
   int64_t total = 0;
   for (int i = 0; i < n; ++i) total += numel[i];
-  a.rounds = total < (4 << 20) ? 1 : 4;
+  const bool nt = exceeds_caches(total * (2 + (x_dtype == 0 ? 2 : 4) + (g_dtype == 0 ? 2 : 4)));
+  // us with 1 / 2 / 4 / 8 rounds: past the caches 2 x (50304 x 768) fp32 241 / 205 / 212 / 224, 2 x (32000 x 4096) 837 / 782 / 810 /
+  // 845; within them 2 x (32003 x 1001) bf16 146 / 140 / 130 / 133.
+  a.rounds = total < (4 << 20) ? 1 : nt ? 2 : 4;
   int64_t wg = 0;
   for (int i = 0; i < kMtaTensors; ++i) {
     const int j = i < n ? i : 0;
@@ -297,7 +300,6 @@ hipError_t launch_adamw8(const uint64_t* X, int x_dtype, const uint64_t* G, int 
   a.wg0[kMtaTensors] = (unsigned)wg;
   hipLaunchKernelGGL(adamw8_advance_steps_kernel, dim3(1), dim3(64), 0, st, a, n);
   if (wg == 0) return hipGetLastError();
-  const bool nt = exceeds_caches(total * (2 + (x_dtype == 0 ? 2 : 4) + (g_dtype == 0 ? 2 : 4)));
   const Adam8Scalars sc{beta1, beta2, eps, wd_host, seed};
   auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)wg), dim3(256), 0, st, a, n, lr_dev, wd_dev, sc); };
 #define A8_LAUNCH(GT, XT)                                                                                              \

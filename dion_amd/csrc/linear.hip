@@ -537,57 +537,59 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
       if constexpr (!PK && !QK)
 #pragma unroll
         for (int j = 0; j < TN; ++j) b[j] = bias4(p.e, col0 + j * 16);
-      // Sixteen rows at a time through the wavefront's staging, so that C (and the slopes) leave in whole 128-byte lines: an
-      // 8-byte piece q of row r lies at q ^ 2 ((r / 2) % 8), which spreads writes and reads over all banks.
+      // Sixteen rows at a time through the wavefront's staging, so that C and the slopes leave in whole 128-byte lines, as
+      // wide as rows of C allow: an 8-byte piece q of row r lies at q ^ 2 ((r / 2) % 8), which spreads writes and reads over
+      // all banks.
+      constexpr int RB = TM == 8 ? 2 : 4;
       char* const stg = lds + Cfg::RING_BYTES + wave * Cfg::STG_BYTES;
-      const int sr = lane >> 3, sq = lane & 7;  // row and 16-byte piece of a lane in the lines
       const int wrow = t.ti * BM + wm * Cfg::WTM, wcol = t.tj * BN + wn * Cfg::WTN;
-      const bool lines = p.e.vec == 8 && wcol + 64 <= p.e.N;  // (the same for the whole wavefront)
       auto put = [&](int j, uint2 w) { *(uint2*)(stg + l16 * 128 + (((4 * j + quad) ^ (((l16 >> 1) & 7) << 1)) << 3)) = w; };
-      auto send = [&](uint16_t* o, int pitch, int row) {
+      auto send = [&](auto widthc, uint16_t* o, int pitch, int row) __attribute__((always_inline)) {
+        constexpr int W = decltype(widthc)::value, LANES = 64 / W;  // elements of a lane, lanes of a row
+        typedef std::conditional_t<W == 8, uint4, std::conditional_t<W == 4, uint2, std::conditional_t<W == 2, uint32_t, uint16_t>>> piece_t;
+        const int sr = lane / LANES, sc = lane % LANES * W;
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = sr + 8 * h;
-          const uint4 w = *(const uint4*)(stg + r * 128 + (((2 * sq) ^ (((r >> 1) & 7) << 1)) << 3));
-          if (row + r < p.e.M) *(uint4*)(o + (int64_t)(row + r) * pitch + wcol + sq * 8) = w;
+        for (int h = 0; h < 16; h += W) {
+          const int r = sr + h;
+          const piece_t w = *(const piece_t*)(stg + r * 128 + (((sc >> 2) ^ (((r >> 1) & 7) << 1)) << 3) + (sc & 3) * 2);
+          if (row + r < p.e.M && wcol + sc < pitch) *(piece_t*)(o + (int64_t)(row + r) * pitch + wcol + sc) = w;
         }
         asm volatile("" ::: "memory");
       };
 #pragma unroll
-      for (int i = 0; i < TM; ++i) {
-        const int row = row0 + i * 16;
-        uint2 y[TN], sl[TN];
-        if constexpr (PK || QK) {  // a gradient: nothing to add
+      for (int i0 = 0; i0 < TM; i0 += RB) {
+        uint2 r[RB][TN];  // (the addend of RB * 16 rows in one go: one way to memory)
+        if constexpr (!PK && !QK)
 #pragma unroll
-          for (int j = 0; j < TN; ++j)
-            y[j] = make_uint2(pack_bf16x2(acc[i][j][0], acc[i][j][1]), pack_bf16x2(acc[i][j][2], acc[i][j][3]));
-        } else {
-          uint2 r[TN];
+          for (int i = 0; i < RB; ++i)
 #pragma unroll
-          for (int j = 0; j < TN; ++j) r[j] = residual4(p.e, row, col0 + j * 16);
+            for (int j = 0; j < TN; ++j) r[i][j] = residual4(p.e, row0 + (i0 + i) * 16, col0 + j * 16);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int j = 0; j < TN; ++j) finish4<ACT, SLOPE>(p.e, acc[i][j], b[j], r[j], y[j], sl[j]);
-        }
-        if (lines) {
-          if constexpr (SLOPE) {
-#pragma unroll
-            for (int j = 0; j < TN; ++j) put(j, sl[j]);
-            send(p.e.slope, slope_pitch(p.e.N), wrow + i * 16);
-          }
-#pragma unroll
-          for (int j = 0; j < TN; ++j) put(j, y[j]);
-          send(p.e.C, p.e.N, wrow + i * 16);
-        } else {
+        for (int i = 0; i < RB; ++i) {
+          uint2 y[TN];
 #pragma unroll
           for (int j = 0; j < TN; ++j) {
-            const int col = col0 + j * 16;
-            if (row >= p.e.M || col >= p.e.N) continue;
-            if constexpr (SLOPE) *(uint2*)(p.e.slope + (int64_t)row * slope_pitch(p.e.N) + col) = sl[j];
-            store4(p.e, p.e.C + (int64_t)row * p.e.N + col, col, y[j]);
+            const f32x4 z = acc[i0 + i][j];
+            uint2 sl;
+            if constexpr (PK || QK) y[j] = make_uint2(pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]));  // a gradient: nothing to add
+            else finish4<ACT, SLOPE>(p.e, z, b[j], r[i][j], y[j], sl);
+            if constexpr (SLOPE) {
+              put(j, sl);
+              __builtin_amdgcn_sched_barrier(0);  // (four elements' intermediate values at a time: more would not fit)
+            }
           }
+          const int row = wrow + (i0 + i) * 16;
+          if constexpr (SLOPE) send(std::integral_constant<int, 8>(), p.e.slope, slope_pitch(p.e.N), row);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) put(j, y[j]);
+          if (p.e.vec == 8) send(std::integral_constant<int, 8>(), p.e.C, p.e.N, row);
+          else if (p.e.vec == 4) send(std::integral_constant<int, 4>(), p.e.C, p.e.N, row);
+          else if (p.e.vec == 2) send(std::integral_constant<int, 2>(), p.e.C, p.e.N, row);
+          else send(std::integral_constant<int, 1>(), p.e.C, p.e.N, row);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("" ::: "memory");
       }
     }
     pid += p.grid;

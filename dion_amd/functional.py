@@ -105,7 +105,7 @@ def adamw8_update_foreach(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_s
     rounding of the codes; equal seeds give equal results bit for bit.  ``state8_values`` gives the moments back."""
     if not X:
         return
-    ops.adamw8_step(X, [g.contiguous() for g in G], M, M_scales, V, V_scales, state_steps,
+    ops.adamw8_step(X, list(map(Tensor.contiguous, G)), M, M_scales, V, V_scales, state_steps,
                     _device_scalar(lr, X[0].device), _host_float(beta1), _host_float(beta2), weight_decay, float(epsilon),
                     cautious_wd, seed)
 

@@ -7,6 +7,7 @@ There is no CPU implementation behind these functions: CPU tensors raise.
 """
 import functools
 import math
+import operator
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -905,20 +906,25 @@ def dion2_post_masked(X: List[Tensor], M: List[Tensor], U: Tensor, norms: Tensor
 # ---------------------------------------------------------------------------------------------
 # multi-tensor AdamW / Lion for the non-matrix parameter groups
 # ---------------------------------------------------------------------------------------------
-def _pointers(ts: List[Tensor], name: str, dtype: torch.dtype, numels: List[int], index: int, what: str) -> List[int]:
-    """Addresses of a list's tensors: dense, of one dtype, on one device, of the given sizes.  (A step passes hundreds of tensors
-    through here: the properties are read in one go, and looked at one by one only to say what is wrong.)"""
+# A step passes hundreds of tensors through here: a property of all of them is read by one map over the C accessor, and they are
+# looked at one by one only to say what is wrong.
+_numel, _get_device, _is_contiguous, _data_ptr = Tensor.numel, Tensor.get_device, Tensor.is_contiguous, Tensor.data_ptr
+_dtype = operator.attrgetter("dtype")
+
+
+def _pointers(ts: List[Tensor], name: str, dtype: torch.dtype, numels: List[int], index: int, what: str):
+    """Table of the addresses of a list's tensors: dense, of one dtype, on one device, of the given sizes."""
     if len(ts) != len(numels):
         raise ValueError(f"{name}: expected {len(numels)} tensors, got {len(ts)}")
-    seen = [(t.numel(), t.dtype, t.get_device(), t.is_contiguous()) for t in ts]
-    if seen != [(n, dtype, index, True) for n in numels] or not set(map(type, ts)) <= _PLAIN_SET:
+    if not (set(map(type, ts)) <= _PLAIN_SET and set(map(_get_device, ts)) == {index} and set(map(_dtype, ts)) == {dtype} and
+            list(map(_numel, ts)) == numels and all(map(_is_contiguous, ts))):
         for t, n in zip(ts, numels):
             _require_gpu(t, name)
             if t.get_device() != index:
                 raise ValueError(f"{name}: tensors of one call must be on one device, got {t.device} beside device {index}")
             if t.dtype != dtype or not t.is_contiguous() or t.numel() != n:
                 raise ValueError(f"{name}: {what}")
-    return [t.data_ptr() for t in ts]
+    return ptr_table(map(_data_ptr, ts), len(ts))
 
 
 _PLAIN_SET = set(_PLAIN)
@@ -934,24 +940,27 @@ def _mta_tables(X: List[Tensor], G: List[Tensor], states: List[List[Tensor]], st
             _require_gpu(x, "X")
     xdt, index = x0.dtype, x0.get_device()
     sdt = state_dtype or xdt
-    if any(x.dtype != xdt for x in X):
+    if set(map(_dtype, X)) != {xdt}:
         raise TypeError("X: one parameter dtype per call")
-    if any(g.dtype != gdt for g in G):
+    if set(map(_dtype, G)) != {gdt}:
         raise TypeError("G: one gradient dtype per call")
-    sizes = [x.numel() for x in X]
+    sizes = list(map(_numel, X))
     dense = "X / G must be contiguous and of equal size"
-    tabs = [ptr_table(_pointers(X, "X", xdt, sizes, index, dense)), ptr_table(_pointers(G, "G", gdt, sizes, index, dense))]
+    tabs = [_pointers(X, "X", xdt, sizes, index, dense), _pointers(G, "G", gdt, sizes, index, dense)]
     for name, st in zip("MV", states):
-        tabs.append(ptr_table(_pointers(st, name, sdt, sizes, index, "optimizer state must be contiguous GPU tensors shaped "
-                                        f"like X, in the dtype of X ({sdt})")))
-    return tabs, (_lib.ctypes.c_int64 * n)(*sizes), _dtype_code(G[0], "G"), _dtype_code(x0, "X")
+        tabs.append(_pointers(st, name, sdt, sizes, index, "optimizer state must be contiguous GPU tensors shaped "
+                              f"like X, in the dtype of X ({sdt})"))
+    return tabs, sizes, _dtype_code(G[0], "G"), _dtype_code(x0, "X")
 
 
-def _check_steps(steps: List[Tensor]) -> List[int]:
-    for s in steps:
-        if s.dtype != torch.float32 or s.numel() != 1 or not s.is_cuda:
-            raise TypeError("steps must be 0-d float32 GPU tensors")
-    return [s.data_ptr() for s in steps]
+def _size_table(sizes: List[int]):
+    return (_lib.ctypes.c_int64 * len(sizes))(*sizes)
+
+
+def _step_pointers(steps: List[Tensor]):
+    if set(map(_dtype, steps)) != {torch.float32} or set(map(_numel, steps)) != {1} or min(map(_get_device, steps)) < 0:
+        raise TypeError("steps must be 0-d float32 GPU tensors")
+    return ptr_table(map(_data_ptr, steps), len(steps))
 
 
 def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor], steps: List[Tensor],
@@ -961,8 +970,10 @@ def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor
     are 0-d float32 device counters (one per tensor; tensors may share one), advanced on the device.  ``M`` and ``V``
     have the dtype of ``X``, or are float32 beside bfloat16 parameters."""
     wide = len(M) > 0 and M[0].dtype == torch.float32 and X[0].dtype == torch.bfloat16
-    (xp, gp, mp, vp), numels, gcode, xcode = _mta_tables(X, G, [M, V], torch.float32 if wide else None)
-    sp = ptr_table(_check_steps(steps))
+    (xp, gp, mp, vp), sizes, gcode, xcode = _mta_tables(X, G, [M, V], torch.float32 if wide else None)
+    if len(steps) != len(X):
+        raise ValueError(f"steps: expected {len(X)} counters, got {len(steps)}")
+    sp, numels = _step_pointers(steps), _size_table(sizes)
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     lib = _lib.load()
     rest = (sp, numels, len(X), lr_p, float(beta1), float(beta2), float(epsilon), wd_p, wd_h, int(bool(cautious_wd)),
@@ -992,15 +1003,15 @@ def adamw8_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: Lis
     n = len(X)
     if any(len(t) != n for t in (G, M, M_scales, V, V_scales, steps)):
         raise ValueError("adamw8_step: all lists must have one tensor for every parameter")
-    (xp, gp), numels, gcode, xcode = _mta_tables(X, G, [])
-    sizes, index = list(numels), X[0].get_device()
-    blocks = [state8_blocks(k) for k in sizes]
+    (xp, gp), sizes, gcode, xcode = _mta_tables(X, G, [])
+    index, numels = X[0].get_device(), _size_table(sizes)
+    blocks = [-(-k // STATE8_BLOCK) for k in sizes]
     tabs = []
     for name, dtype, codes, scales in (("M", torch.int8, M, M_scales), ("V", torch.uint8, V, V_scales)):
-        tabs.append(ptr_table(_pointers(codes, name, dtype, sizes, index, f"codes must be contiguous {dtype} tensors shaped like X")))
-        tabs.append(ptr_table(_pointers(scales, name + "_scales", torch.float32, blocks, index,
-                                        f"one contiguous float32 scale for every {STATE8_BLOCK} elements of X")))
-    tabs.append(ptr_table(_check_steps(steps)))
+        tabs.append(_pointers(codes, name, dtype, sizes, index, f"codes must be contiguous {dtype} tensors shaped like X"))
+        tabs.append(_pointers(scales, name + "_scales", torch.float32, blocks, index,
+                              f"one contiguous float32 scale for every {STATE8_BLOCK} elements of X"))
+    tabs.append(_step_pointers(steps))
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     with _device_of(X[0]):
         check(_lib.load().dion_adamw8_step(xp, xcode, gp, gcode, *tabs, numels, n, lr_p, float(beta1), float(beta2),
@@ -1038,7 +1049,8 @@ def state8_values(codes: Tensor, scales: Tensor, dtype: torch.dtype = torch.floa
 def lion_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Tensor, beta1: float, beta2: float,
               weight_decay, cautious_wd: bool = False) -> None:
     """One fused Lion step over tensors of any sizes (dion/scalar_opts.py:68-118, :271-325)."""
-    (xp, gp, mp), numels, gcode, scode = _mta_tables(X, G, [M])
+    (xp, gp, mp), sizes, gcode, scode = _mta_tables(X, G, [M])
+    numels = _size_table(sizes)
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     lib = _lib.load()
     check(lib.dion_lion_step(xp, gp, gcode, mp, scode, numels, len(X), lr_p, float(beta1), float(beta2), wd_p, wd_h,
