@@ -2018,8 +2018,9 @@ extern "C" int dion_linear_backward(const void* dy, int64_t lddy, const void* sl
   if (tokens == 0) {
     // sums over nothing
     const int64_t all = (int64_t)fan_out * fan_in;
-    for (int64_t at = 0; dw && at < all; at += 1 << 30)
-      HIP_TRY(launch_lin_sum(nullptr, 0, (int)(all - at < (1 << 30) ? all - at : 1 << 30), (bf16_t*)dw + at, 0, st), who);
+    constexpr int kRun = 1 << 26;  // (a launch has fewer than 2^32 threads, sixteen of them an element)
+    for (int64_t at = 0; dw && at < all; at += kRun)
+      HIP_TRY(launch_lin_sum(nullptr, 0, (int)(all - at < kRun ? all - at : kRun), (bf16_t*)dw + at, 0, st), who);
     if (db) HIP_TRY(launch_lin_sum(nullptr, 0, fan_out, db, dt(db_dtype), st), who);
     return DION_OK;
   }

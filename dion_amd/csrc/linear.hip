@@ -24,8 +24,8 @@ static __device__ __forceinline__ float rcp_fast(float v) { return __builtin_amd
 template <int ACT>
 static __device__ __forceinline__ float activate(float z, float& slope) {
   if constexpr (ACT == kActRelu) {
-    slope = z > 0.f ? 1.f : 0.f;
-    return z < 0.f ? 0.f : z;  // (NaN stays)
+    slope = z <= 0.f ? 0.f : 1.f;  // (where z is NaN the gradient goes on, and the value stays NaN)
+    return z < 0.f ? 0.f : z;
   } else if constexpr (ACT == kActReluSquared) {
     const float r = z < 0.f ? 0.f : z;
     slope = 2.f * r;

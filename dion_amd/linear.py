@@ -10,19 +10,15 @@ from torch.autograd.function import once_differentiable
 from . import ops
 
 
-def _rows(t: Optional[Tensor]) -> Optional[Tensor]:
-    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
-
-
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation, residual):
         need = ctx.needs_input_grad
-        y, slope = ops.linear_forward(_rows(x), weight, bias, activation, _rows(residual), need[0] or need[1] or need[2])
+        y, slope = ops.linear_forward(x, weight, bias, activation, residual, need[0] or need[1] or need[2])
         ctx.save_for_backward(x if need[1] else None, weight, slope)
-        ctx.activation, ctx.lead = activation, x.shape[:-1]
+        ctx.activation = activation
         ctx.bias_dtype = bias.dtype if bias is not None and need[2] else None
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
+        return y
 
     @staticmethod
     @once_differentiable
@@ -31,11 +27,24 @@ class _Linear(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if need[0] or need[1] or ctx.bias_dtype is not None:
-            dx, dw, db = ops.linear_backward(_rows(dy), slope, ctx.activation, _rows(x), weight, need[0], need[1],
-                                             ctx.bias_dtype)
-            if dx is not None and len(ctx.lead) != 1:
-                dx = dx.view(*ctx.lead, weight.shape[1])
+            dx, dw, db = ops.linear_backward(dy, slope, ctx.activation, x, weight, need[0], need[1], ctx.bias_dtype)
         return dx, dw, db, None, dy if need[4] else None
+
+
+# A leaf's accumulation node runs on the stream on which it was made and lives as long as a graph that holds it.  Recorded by a
+# capture, a backward pass that meets a node of another stream makes that stream wait inside the capture, and torch then ends the
+# process.  So a node keeps the stream of the first product that it is seen in, and a capture on another one is refused
+# before its backward pass.
+_ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros((), requires_grad=True)).node)
+_STREAM = "dion_amd.linear: stream"
+
+
+def _check_capture(y: Tensor) -> None:
+    stream, capturing = ops._stream_handle(y.device), torch.cuda.is_current_stream_capturing()
+    for node, _index in y.grad_fn.next_functions:
+        if isinstance(node, _ACCUMULATE) and node.metadata.setdefault(_STREAM, stream) != stream and capturing:
+            raise RuntimeError("linear: captured while a result of an earlier product with the same leaf, on another stream, still "
+                               "has its graph; delete or detach that result first")
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
@@ -47,10 +56,13 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     Differentiable once with respect to every tensor.  For the backward pass it keeps ``x``, the weight and, with an
     activation, its slopes in 16 bits an element; the gradient that reaches ``z = x W^T + b`` is rounded to bfloat16 for the two
     products, not for the bias.  Any sizes and strides; rows that are not whole 16-byte chunks (feature counts that are not
-    multiples of 8) are copied first."""
-    ops.check_linear(x, weight, bias, activation, residual)
+    multiples of 8) are copied first.  ``weight`` and ``x`` must not change between the two passes (autograd raises).
+
+    Both passes can be captured into a graph, together, while no result of an earlier call on the same leaves on another
+    stream has its autograd graph: that is refused (RuntimeError)."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
-        return _Linear.apply(x, weight, bias, activation, residual)
-    y, _slope = ops.linear_forward(_rows(x), weight, bias, activation, _rows(residual), False)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
+        y = _Linear.apply(x, weight, bias, activation, residual)
+        _check_capture(y)
+        return y
+    return ops.linear_forward(x, weight, bias, activation, residual, False)[0]

@@ -957,9 +957,11 @@ def _size_table(sizes: List[int]):
     return (_lib.ctypes.c_int64 * len(sizes))(*sizes)
 
 
-def _step_pointers(steps: List[Tensor]):
+def _step_pointers(steps: List[Tensor], index: int):
     if set(map(_dtype, steps)) != {torch.float32} or set(map(_numel, steps)) != {1} or min(map(_get_device, steps)) < 0:
         raise TypeError("steps must be 0-d float32 GPU tensors")
+    if set(map(_get_device, steps)) != {index}:
+        raise ValueError(f"steps must be on the device of X, {index}")
     return ptr_table(map(_data_ptr, steps), len(steps))
 
 
@@ -973,7 +975,7 @@ def adamw_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], V: List[Tensor
     (xp, gp, mp, vp), sizes, gcode, xcode = _mta_tables(X, G, [M, V], torch.float32 if wide else None)
     if len(steps) != len(X):
         raise ValueError(f"steps: expected {len(X)} counters, got {len(steps)}")
-    sp, numels = _step_pointers(steps), _size_table(sizes)
+    sp, numels = _step_pointers(steps, X[0].get_device()), _size_table(sizes)
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     lib = _lib.load()
     rest = (sp, numels, len(X), lr_p, float(beta1), float(beta2), float(epsilon), wd_p, wd_h, int(bool(cautious_wd)),
@@ -997,7 +999,7 @@ def adamw8_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: Lis
                 epsilon: float, cautious_wd: bool = False, seed: int = 0) -> None:
     """``adamw_step`` with moments in 8 bits: ``M`` int8 and ``V`` uint8 codes shaped like ``X``, ``*_scales`` float32, one
     for every 128 elements (``state8_blocks``).  Codes are rounded up or down at random, without bias, by numbers that depend on
-    ``seed``, the step counter and the element alone."""
+    ``seed``, the step counter and the element alone.  No tensor may overlap another one of the call."""
     if not X:
         return
     n = len(X)
@@ -1005,13 +1007,15 @@ def adamw8_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], M_scales: Lis
         raise ValueError("adamw8_step: all lists must have one tensor for every parameter")
     (xp, gp), sizes, gcode, xcode = _mta_tables(X, G, [])
     index, numels = X[0].get_device(), _size_table(sizes)
+    if len(set(xp)) != n and len({x.data_ptr() for x in X if x.numel()}) != sum(k > 0 for k in sizes):
+        raise ValueError("adamw8_step: a parameter is in X twice")
     blocks = [-(-k // STATE8_BLOCK) for k in sizes]
     tabs = []
     for name, dtype, codes, scales in (("M", torch.int8, M, M_scales), ("V", torch.uint8, V, V_scales)):
         tabs.append(_pointers(codes, name, dtype, sizes, index, f"codes must be contiguous {dtype} tensors shaped like X"))
         tabs.append(_pointers(scales, name + "_scales", torch.float32, blocks, index,
                               f"one contiguous float32 scale for every {STATE8_BLOCK} elements of X"))
-    tabs.append(_step_pointers(steps))
+    tabs.append(_step_pointers(steps, index))
     lr_p, wd_p, wd_h = _scalar_args(lr, weight_decay, X[0].device)
     with _device_of(X[0]):
         check(_lib.load().dion_adamw8_step(xp, xcode, gp, gcode, *tabs, numels, n, lr_p, float(beta1), float(beta2),
@@ -1086,23 +1090,45 @@ def _check_linear(name: str, t: Tensor, shape, index: int, fp32: bool = False) -
         raise ValueError(f"linear: {name} is on {t.device}, x on device {index}")
 
 
-def check_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
-                 residual: Optional[Tensor]) -> None:
-    """Raises for what ``linear_forward`` does not take (``x`` of any number of dimensions)."""
+def _check_weight(t: Tensor, name: str, weight: Tensor, side: int, activation: Optional[str]) -> int:
+    """A weight and the tensor whose last dimension fits its dimension ``side``; returns their device's index."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
-    xs, ws = x.shape, weight.shape
-    if len(ws) != 2 or len(xs) < 1 or xs[-1] != ws[1]:
-        raise ValueError(f"linear: x of shape {tuple(xs)} does not fit a weight of shape {tuple(ws)}")
+    ts, ws = t.shape, weight.shape
+    if len(ws) != 2 or len(ts) < 1 or ts[-1] != ws[side]:
+        raise ValueError(f"linear: {name} of shape {tuple(ts)} does not fit a weight of shape {tuple(ws)}")
     if ws[0] == 0 or ws[1] == 0:
         raise ValueError(f"linear: empty weight of shape {tuple(ws)}")
-    index = x.get_device()
-    _check_linear("x", x, xs, index)
+    index = t.get_device()
+    _check_linear(name, t, ts, index)
     _check_linear("weight", weight, ws, index)
+    return index
+
+
+def _check_linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
+                          residual: Optional[Tensor]) -> None:
+    index, xs, ws = _check_weight(x, "x", weight, 1, activation), x.shape, weight.shape
     if bias is not None:
         _check_linear("bias", bias, ws[:1], index, fp32=True)
     if residual is not None:
         _check_linear("residual", residual, xs[:-1] + ws[:1], index)
+
+
+def _check_linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
+                           weight: Tensor, need_dw: bool, bias_dtype: Optional[torch.dtype]) -> None:
+    index, lead, ws = _check_weight(dy, "dy", weight, 0, activation), dy.shape[:-1], weight.shape
+    if (slope is None) != (activation is None):
+        raise ValueError(f"linear: activation {activation!r} goes with{'out' if activation is None else ''} slopes")
+    if slope is not None:
+        want = (lead.numel(), -(-ws[0] // 8) * 8)
+        if slope.get_device() != index or slope.dtype != torch.int16 or tuple(slope.shape) != want or not slope.is_contiguous():
+            raise ValueError(f"linear: expected the slopes that the forward pass kept, int16 of shape {want} on device {index}")
+    if need_dw:
+        if x is None:
+            raise ValueError("linear: the gradient of the weight needs x")
+        _check_linear("x", x, lead + ws[1:], index)
+    if bias_dtype not in (None, torch.bfloat16, torch.float32):
+        raise TypeError(f"linear: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1120,18 +1146,24 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _flat(t: Tensor) -> Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
 def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
                    residual: Optional[Tensor], keep_slope: bool) -> Tuple[Tensor, Optional[Tensor]]:
-    """``act(x W^T + b) + residual`` of 2D ``x`` and ``residual``, and with ``keep_slope`` act' at every element, in the 16
-    bits that ``linear_backward`` reads."""
-    act = ACTIVATIONS[activation]
-    tokens, fan_out = x.shape[0], weight.shape[0]
+    """``act(x W^T + b) + residual``, and with ``keep_slope`` and an activation act' at every element, in the 16 bits that
+    ``linear_backward`` reads."""
+    _check_linear_forward(x, weight, bias, activation, residual)
+    act, lead = ACTIVATIONS[activation], x.shape[:-1]
+    x, fan_out = _flat(x), weight.shape[0]
+    tokens = x.shape[0]
     with _device_of(x):
         y = torch.empty(tokens, fan_out, dtype=torch.bfloat16, device=x.device)
         # (in whole 16-byte chunks)
         slope = torch.empty(tokens, -(-fan_out // 8) * 8, dtype=torch.int16, device=x.device) if keep_slope and act else None
         (x, ldx), (w, ldw) = _rows(x), _rows(weight)
-        r, ldr = (None, 0) if residual is None else _rows(residual)
+        r, ldr = (None, 0) if residual is None else _rows(_flat(residual))
         b = None if bias is None else bias.contiguous()
         copies = (0 if _whole_chunks(x, ldx) else _lib.DION_LINEAR_COPY_X) | (0 if _whole_chunks(w, ldw) else _lib.DION_LINEAR_COPY_W)
         ws, nbytes = _linear_space(tokens, weight, False, act, copies)
@@ -1139,7 +1171,7 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation
                                               DION_BF16 if b is None else _dtype_code(b, "bias"), act, _ptr(r), ldr,
                                               y.data_ptr(), _ptr(slope), tokens, weight.shape[1], fan_out, _ptr(ws), nbytes,
                                               _stream_handle(x.device)), "linear")
-    return y, slope
+    return (y if len(lead) == 1 else y.view(*lead, fan_out)), slope
 
 
 def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
@@ -1147,13 +1179,15 @@ def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[st
                     bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients ``(dx, dW, db)`` of ``linear_forward``, None where not asked for (``bias_dtype`` None: no ``db``).  ``x`` is
     read for ``dW``, the weight for ``dx``."""
-    act = ACTIVATIONS[activation]
+    _check_linear_backward(dy, slope, activation, x, weight, need_dw, bias_dtype)
+    act, lead = ACTIVATIONS[activation], dy.shape[:-1]
     fan_out, fan_in = weight.shape
+    dy = _flat(dy)
     tokens = dy.shape[0]
     with _device_of(dy):
         dy, lddy = _rows(dy)
         copies = 0 if _whole_chunks(dy, lddy) else _lib.DION_LINEAR_COPY_DY
-        xr, ldx = _rows(x) if need_dw else (None, 0)
+        xr, ldx = _rows(_flat(x)) if need_dw else (None, 0)
         w, ldw = _rows(weight) if need_dx else (None, 0)
         if need_dw and not _whole_chunks(xr, ldx):
             copies |= _lib.DION_LINEAR_COPY_X
@@ -1167,4 +1201,6 @@ def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[st
         check(_lib.load().dion_linear_backward(dy.data_ptr(), lddy, _ptr(slope), act, _ptr(xr), ldx, _ptr(w), ldw, _ptr(dx),
                                                _ptr(dw), _ptr(db), DION_BF16 if db is None else _dtype_code(db, "bias"), tokens,
                                                fan_in, fan_out, _ptr(ws), nbytes, _stream_handle(dy.device)), "linear backward")
+    if need_dx and len(lead) != 1:
+        dx = dx.view(*lead, fan_in)
     return dx, dw, db

@@ -172,6 +172,9 @@ class OrthoOptimizer(Optimizer):
             for key, dtype in self._adamw_state_dtypes(bits).items():
                 state[key] = (torch.zeros(ops.state8_blocks(param.numel()), dtype=dtype, device=param.device)
                               if key.endswith("_scale") else torch.zeros_like(param, dtype=dtype))
+        elif state["momentum"].dtype != (torch.int8 if bits == 8 else torch.float32):
+            raise ValueError(f"state_bits={bits}: this parameter's moments are {state['momentum'].dtype}; the option is set when a "
+                             "group is made, or comes with the checkpoint")
         return self._get_or_initialize_state(param, "adamw")
 
     # ------------------------------------------------- live hyper-parameters

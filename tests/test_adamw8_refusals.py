@@ -83,3 +83,15 @@ def test_group_option_is_checked_and_creates_state():
         make(algorithm="adamw", state_bits=8).load_state_dict(saved)
     plain = make(algorithm="adamw")
     assert plain.state[plain.param_groups[1]["params"][0]]["momentum"].dtype == torch.bfloat16
+
+
+def test_group_option_stays_what_it_was():
+    from dion import Muon
+
+    p = torch.nn.Parameter(torch.zeros(130, dtype=torch.bfloat16))
+    for before, after in ((None, 8), (None, 32), (8, 32), (32, 8)):
+        option = {} if before is None else {"state_bits": before}
+        opt = Muon([{"params": [p], "algorithm": "adamw", **option}], lr=0.1)
+        opt.param_groups[0]["state_bits"] = after
+        with pytest.raises(ValueError, match="moments are"):
+            opt._adamw_state(p, after)

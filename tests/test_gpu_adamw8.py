@@ -264,3 +264,21 @@ def test_group_option_state_dict_and_graph(bits, dtype):
         graph.step()
         torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(params, third))
+
+
+def test_a_parameter_twice_and_counters_of_another_kind_are_refused():
+    from dion_amd.functional import adamw8_update_foreach
+
+    x, g = torch.zeros(300, device=DEV), torch.zeros(300, device=DEV)
+    state = lambda: (torch.zeros(300, dtype=torch.int8, device=DEV), torch.zeros(3, device=DEV),  # noqa: E731
+                     torch.zeros(300, dtype=torch.uint8, device=DEV), torch.zeros(3, device=DEV))
+    lists = [list(t) for t in zip(state(), state())]
+    steps = [torch.zeros((), device=DEV) for _ in range(2)]
+    with pytest.raises(ValueError, match="twice"):
+        adamw8_update_foreach([x, x], [g, g], *lists, 0.1, 0.9, 0.95, 0.0, state_steps=steps)
+    with pytest.raises(TypeError, match="steps"):
+        adamw8_update_foreach([x, x.clone()], [g, g], *lists, 0.1, 0.9, 0.95, 0.0, state_steps=[steps[0], torch.zeros(())])
+    none = torch.zeros(0, device=DEV)  # (two empty parameters share an address, and nothing else)
+    empty = [[t[:0], t[:0]] for t in state()]
+    adamw8_update_foreach([none, none.clone()], [none, none], *empty, 0.1, 0.9, 0.95, 0.0, state_steps=steps)
+    assert [float(s) for s in steps] == [1.0, 1.0]

@@ -297,3 +297,122 @@ def test_a_block_is_trained_through_products_and_step():
         before = [p.detach().clone() for p in (emb, up, down, bu, bd)]
         opt.step()
         assert all(p.isfinite().all() and not torch.equal(p, q) for p, q in zip((emb, up, down, bu, bd), before))
+
+
+def test_no_tokens_and_a_weight_past_one_launch():
+    """2^28 and more elements of a gradient of zeros."""
+    from dion_amd import linear
+
+    x = torch.zeros(0, 16400, device=DEV, dtype=torch.bfloat16)
+    w = torch.ones(16400, 16400, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    (g,) = torch.autograd.grad(linear(x, w), w, torch.zeros(0, 16400, device=DEV, dtype=torch.bfloat16))
+    assert g.shape == w.shape and not bool(g.any())
+
+
+@pytest.mark.parametrize("k,n,act", [(8192, 64, None), (64, 8192, "gelu")])
+def test_more_elements_than_32_bits_count(k, n, act):
+    """Operands and results of 4.9 GB: the last rows, which alone carry a gradient, against the formulas."""
+    from dion_amd import linear
+
+    t, tail = 300000, 200
+    x, w, b, _r, dy = make(tail, k, n, torch.bfloat16, False, seed=3)
+    big = torch.ones(t, k, device=DEV, dtype=torch.bfloat16)
+    big[-tail:] = x
+    dys = torch.zeros(t, n, device=DEV, dtype=torch.bfloat16)
+    dys[-tail:] = dy
+    leaves = [p.requires_grad_() for p in (big, w, b)]
+    y = linear(*leaves, activation=act)
+    dx, dw, db = torch.autograd.grad(y, leaves, dys)
+    want = expected(x, w.detach(), b.detach(), act, None, dy)
+    check(y[-tail:], want["y"], "y")
+    check(dx[-tail:], want["dx"], "dx")
+    check(dw, want["dw"], "dw")
+    check(db, want["db"], "db", extra=2.0 ** -8)
+    assert torch.equal(y[0], y[t - tail - 1]) and not bool(dx[:-tail].any())
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_nan_reaches_the_gradients(act):
+    """A row of x that is NaN: its row of dx and all of dW are NaN (with relu, whose derivative is a number there, the gradient goes
+    on instead of ending); the other rows are as without it."""
+    from dion_amd import linear
+
+    x, w, b, _r, dy = make(40, 64, 48, torch.bfloat16, False, seed=9)
+    bad = x.clone()
+    bad[7] = float("nan")
+    grads = []
+    for v in (x, bad):
+        leaves = [p.detach().requires_grad_() for p in (v, w, b)]
+        y = linear(*leaves, activation=act)
+        grads.append((y, *torch.autograd.grad(y, leaves, dy)))
+    (y0, dx0, _, _), (y1, dx1, dw1, db1) = grads
+    rest = torch.arange(40, device=DEV) != 7
+    assert torch.equal(y0[rest], y1[rest]) and torch.equal(dx0[rest], dx1[rest])
+    assert bool(y1[7].isnan().all()) and bool(dw1.isnan().all())
+    if act in (None, "relu"):
+        assert torch.equal(dx1[7], linear(dy[7], w.t().contiguous()))
+    else:
+        assert bool(dx1[7].isnan().all()) and bool(db1.isnan().all())
+
+
+def test_a_captured_pass_through_autograd():
+    """Forward and backward through autograd, recorded and replayed; not while an eager graph of the same leaves lives, whose
+    stream the recorded pass would have to wait for."""
+    from dion_amd import linear
+
+    x, w, b, r, dy = make(160, 264, 1000, torch.float32, True, seed=4)
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+
+    def both():
+        y = linear(*leaves[:3], activation="gelu", residual=leaves[3])
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device=DEV))
+        eager = [t.clone() for t in both()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager)), k
+
+    alive = linear(x.detach(), leaves[1])
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="still has its graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            linear(x.detach(), leaves[1])
+    del alive
+    graph2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2):
+        again = both()
+    graph2.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(again, both()))
+
+
+def test_operator_calls_are_checked():
+    """The calls below the autograd function refuse what does not fit instead of reading past it."""
+    from dion_amd import ops
+
+    x, w, _b, _r, dy = make(12, 40, 24, None, False)
+    y, slope = ops.linear_forward(x, w, None, "silu", None, True)
+    good = dict(dy=dy, slope=slope, activation="silu", x=x, weight=w, need_dx=True, need_dw=True, bias_dtype=torch.float32)
+    ops.linear_backward(**good)
+    for bad in ({"dy": dy[:, :16]}, {"x": x[:8]}, {"x": None}, {"slope": None}, {"slope": slope[:8]}, {"activation": None},
+                {"slope": slope.view(torch.uint8)}, {"weight": w[:16]}):
+        with pytest.raises(ValueError, match="linear"):
+            ops.linear_backward(**{**good, **bad})
+    for bad in ({"dy": dy.float()}, {"x": x.half()}, {"bias_dtype": torch.float64}):
+        with pytest.raises(TypeError):
+            ops.linear_backward(**{**good, **bad})
+    with pytest.raises(ValueError, match="does not fit"):
+        ops.linear_forward(x, w[:, :32], None, None, None, False)
+    with pytest.raises(ValueError, match="residual"):
+        ops.linear_forward(x, w, None, None, y[:8], False)
