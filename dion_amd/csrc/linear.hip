@@ -9,6 +9,12 @@
 // kept in fp16 (eleven bits); those of the squared relu, 2 max(z, 0), have no sign and no bound, and are kept as seven bits of
 // exponent and nine of mantissa, from 2^-63 to where z^2 leaves fp32.  bf16's eight bits would add an error of the size of
 // the rounding of dz itself; so it stays an eighth (a quarter) of that, for the same bytes.
+//
+// Large products are bound by the matrix units at the clock the power limit leaves (a 256-wide slab takes 1.37 us of ordinary
+// values, 1.06 of zeros) and by the output, which all CUs write at once when a round of tiles ends (134 MB of 8192 x 8192 with
+// a reduction of 64, where little else is left: 39 us, with an activation's slopes 63). us, y with nothing in the epilogue / dx
+// / dW: 8192 x 2048 x 8192 (tokens, fan-in, fan-out) 205 / 193 / 195, 16384 x 4096 x 14336 1349 / 1334 / 1715, 4096 x 2048 x
+// 2048 31.7 / 30.8 / 33.1; 8192 x 8192 x 8192 757 / 755 / 776, 1.45 PFLOP/s.
 #include <atomic>
 
 #include "gemm_tile.h"
@@ -231,6 +237,11 @@ struct LinTileParams {
 // XOR swizzles keep the LDS writes and the fragment reads free of bank conflicts.  The MFMA operands are swapped (B
 // fragment first), so that a lane's four sums are neighbours of one row of C: 8-byte accesses to C, the addend and the slopes.
 // SPLIT: the sums of a part go to p.part as fp32, and lin_join_kernel finishes them.
+// What the steps to this form measured, us, 8192 x 2048 x 8192 with the squared relu and its slopes: a workgroup per tile, sums
+// through LDS to the activation 329; activation in the registers of the sums 293; one workgroup per CU that walks its tiles,
+// results through LDS in lines 255. Tiles of 256 x 128 whose fragments are a slab ahead: 4096 x 2048 x 2048 37 to 32, dW of it
+// 48 to 34. Four wavefronts of 128 x 128 instead of eight gain nothing in the loop (1.34 to 1.41 us a slab against 1.37) and
+// lose in the epilogue; neither staggered starts of the workgroups nor non-temporal stores make the rounds' ends cheaper.
 template <class Cfg, bool PK, bool QK, int ACT, bool SLOPE, bool SPLIT>
 __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParams p) {
   constexpr int BM = Cfg::BM, BN = Cfg::BN, BK = Cfg::BK, TM = Cfg::TM, TN = Cfg::TN, ST = Cfg::ST, HALVES = Cfg::HALVES;
@@ -314,7 +325,8 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
       soff = 0;
       KT_in = t.KT;
       k_in = t.part * p.slabs * BK;
-      auto begin = [&](const bf16_t* base, bool kmajor, int extent, int at, int ld, const char*& from, int& end, int& recs, int& in) __attribute__((always_inline)) {
+      auto begin = [&](const bf16_t* base, bool kmajor, int extent, int at, int ld, const char*& from, int& end, int& recs,
+                       int& in) __attribute__((always_inline)) {
         from = (const char*)(base + (kmajor ? (int64_t)k_in * ld + at : (int64_t)at * ld + k_in));
         // (K-major: rows from the tile's last slab on; all of a slab's rows are there before it)
         const int64_t n = (int64_t)(kmajor ? p.K - k_in - (t.KT - 1) * BK : extent - at) * ld * 2;
@@ -605,7 +617,8 @@ __global__ __launch_bounds__(Cfg::NT, 2) void lin_tile_kernel(const LinTileParam
   }
 }
 
-// Adds the parts of a split reduction, in their order, and finishes: four elements per thread.
+// Adds the parts of a split reduction, in their order, and finishes: four elements per thread.  Ten parts of 32 x 2048 4.4 us,
+// of which 2 are the launch; the parts come from L2 and the memory-side cache.
 __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, const float* __restrict__ part, int splits) {
   const int per_row = (p.N + 3) / 4;
   const int64_t all = (int64_t)p.M * per_row, one = (int64_t)p.M * p.N;
@@ -630,7 +643,8 @@ __global__ __launch_bounds__(256) void lin_join_kernel(const LinEpilogue p, cons
 // Up to 32 rows of x and a weight of a few megabytes: latency is what counts.  A workgroup takes 16 rows of W, its wavefronts an
 // equal run of the reduction each; fragments go from memory to registers with no LDS between (a lane's chunk is its MFMA operand
 // as it lies), the next U steps' while the MFMAs of these run.  MFMA row: a row of W; column: a token (past the last one, the
-// last one again).  The wavefronts' sums meet in LDS and are added in their order.
+// last one again).  The wavefronts' sums meet in LDS and are added in their order.  Bound by the weight's bytes: one token of 4096 to 14336
+// 24.4 us (4.8 TB/s, the weight from HBM), of 768 to 768 4.7 us (launch, one way to memory, LDS).
 template <int TB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void lin_few_kernel(const LinEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
                                                              const bf16_t* __restrict__ w, int64_t ldw, int K) {
@@ -696,6 +710,8 @@ constexpr int kPrepCols = 256;  // columns of a workgroup: 32 threads of eight, 
 static int sum_rows(int rows) { return (rows + 1023) / 1024 * 8; }
 int lin_sum_parts(int rows) { return (rows + sum_rows(rows) - 1) / sum_rows(rows); }
 
+// One pass for what the products cannot read as it lies: dz, its column sums, and rows that are not whole chunks.  HBM: 6 bytes an
+// element with slopes, 8192 x 8192 92 us (4.4 TB/s); 4 bytes for a copy, 2 for sums alone (4096 x 2048 4.7 us).
 // SLOPE: src is dy, and dz = dy * act'(z) goes on.  W: elements of src that are read at once; 8: every row is whole chunks.
 template <bool SLOPE, bool DST, bool SUM, int W>
 __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restrict__ src, int64_t ld,
@@ -752,7 +768,7 @@ __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restri
   }
 }
 
-// out[c] = sum of partial[0 .. parts)[c]: 16 columns of a workgroup, sixteen threads a column.
+// out[c] = sum of partial[0 .. parts)[c]: 16 columns of a workgroup, sixteen threads a column.  3 us: a launch and eight loads in a row.
 __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* out,
                                                       int out_dtype) {
   __shared__ float sums[16][17];
@@ -773,11 +789,17 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// How a product runs: on which tiles, and in how many parts of the reduction: what is estimated to take least.  A round of the
-// 256 CUs takes so much a slab and so much for itself (first loads, epilogue).  Measured, us, reductions of 1024 / 8192: one
-// round of 128-wide tiles 12.9 / 63, of 256 x 128 21 / 122, of 256-wide 34 / 224; of 64 128-wide tiles the slab costs 0.37 instead of
-// 0.45 (the clock, on this power-limited part, and L2).  Splitting pays where a round is not full: 32 tokens of 2048 x 8192, 16
-// tiles, in 1 / 4 / 16 parts 46 / 16.8 / 10.8 us with the kernel that joins them.
+// How a product runs: on which tiles, and in how many parts of the reduction: what is estimated to take least.  us:
+//   a round of the 256 CUs: so much a slab and so much for itself (first loads, epilogue).  Measured over reductions of 1024 / 8192,
+//     128-wide tiles 12.9 / 63, 256 x 128 21 / 122, 256-wide 34 / 224; from HBM full 128-wide tiles, which read the most, take 0.62 a
+//     slab (512 tokens of 4096 x 14336, weights not cached: two parts of them 78, four of 256 x 128 63), from caches 0.45;
+//   never less than the bytes at what so many CUs draw from HBM: 4096 x 14336 and one to sixteen tokens in 160 / 256 parts of
+//     tiles 28.8 / 25.6, 14336 x 4096 and 128 tokens in 112 / 224 45 / 37;
+//   the kernel that joins the parts: 3 and the sums both ways (32 tokens of 2048 x 8192, 16 tiles, in 1 / 4 / 16 parts 46 / 16.8 /
+//     13.4).
+// lin_few_kernel takes so long per 512 of the reduction, its tokens and a workgroup per CU.  Few / tiles at 1, 8, 16, 32 tokens of
+// a weight from HBM: 768 x 768 3.8, 4.1, 4.2, 5.2 / 7.1 to 7.7; 4096 x 4096 8.6, 10.0, 11.9, 16.4 / 11.8 to 12.7; 4096 x 14336
+// 23.5, 28.5, 34.8, 50.3 / 25.2 to 25.9; 50304 x 768 15.5, 20.0, 24.5, 57 / 20.4 to 21.7.
 enum LinTile { kLinFew, kLin128, kLinWide, kLin256 };
 struct LinPlan {
   LinTile tile;
@@ -787,18 +809,20 @@ static LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
   const int KT = (K + 63) / 64;
   LinPlan best{kLin128, 1, KT};
   double least = 1e30;
-  const double streaming = 4.0 + 2.0 * ((double)M * K + (double)N * K + (double)M * N) / 5e6;
+  const double bytes = 2.0 * ((double)M * K + (double)N * K + (double)M * N);
   for (int t = kLin128; t <= kLin256; ++t) {
     const int bm = t == kLin128 ? 128 : 256, bn = t == kLin256 ? 256 : 128;
-    const double slab = t == kLin256 ? 1.65 : t == kLinWide ? 0.9 : 0.45, fixed = t == kLin256 ? 8.0 : t == kLinWide ? 5.0 : 4.5;
+    const double slab = t == kLin256 ? 1.65 : t == kLinWide ? 0.9 : M > 64 && bytes > 64e6 ? 0.55 : 0.45;
+    const double fixed = t == kLin256 ? 8.0 : t == kLinWide ? 5.0 : 4.5;
     const int64_t tiles = (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     for (int s = 1; s <= 16 && s <= KT; ++s) {
       const int slabs = (KT + s - 1) / s;
       const int parts = (KT + slabs - 1) / slabs;
       if (parts != s) continue;
       double us = (double)((tiles * parts + 255) / 256) * (slabs * slab + fixed);
+      const double streaming = 3.0 + bytes / (tiles * parts >= 256 ? 6.1e6 : tiles * parts > 128 ? 5.1e6 : 3.0e6);
       if (us < streaming) us = streaming;
-      if (parts > 1) us += 2.5 + (double)M * N * parts * 8.0 / 4e6;
+      if (parts > 1) us += 3.0 + (double)M * N * parts * 8.0 / 6e6;
       if (us < least) {
         least = us;
         best = {(LinTile)t, parts, slabs};

@@ -443,8 +443,8 @@ enum { DION_ACT_NONE, DION_ACT_RELU, DION_ACT_RELU_SQUARED, DION_ACT_GELU, DION_
 size_t dion_linear_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int activation, int copies);
 
 /* y = act(x w^T + bias) + residual.  bias, residual may be null.  slope (null, or [tokens][fan_out rounded up to 8] of 16 bits,
- * 16-byte aligned; not without an activation): act' at every element, for dion_linear_backward -- fp16, of the squared relu seven bits of exponent and
- * nine of mantissa.  Neither y nor slope may overlap an operand, but y may be the residual where that is dense. */
+ * 16-byte aligned; not without an activation): act' at every element, for dion_linear_backward -- fp16, of the squared relu seven
+ * bits of exponent and nine of mantissa.  Neither y nor slope may overlap an operand, but y may be the residual where that is dense. */
 int dion_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_dtype,
                         int activation, const void* residual, int64_t ldr, void* y, void* slope, int tokens, int fan_in,
                         int fan_out, void* workspace, size_t workspace_bytes, void* stream);
@@ -487,8 +487,8 @@ int dion_adamw_fp32_state_step(const uint64_t* X_ptrs, int x_dtype, const uint64
  * m and in v, by u = ((h + j 0x9E3779B9) mod 2^32 >> 8) 2^-24 for element 8 i + j of a tensor, h = mix(key ^ i), key =
  * mix(mix(seed) + step) (mix: adamw8.hip):  c = floor(m / s + u);  k = floor(t), t = sqrt(v) / q, or one more where
  * u (2 k + 1) < t^2 - k^2.  v > 0 keeps k >= 1.  Zeroed codes and scales are the state before the first step.  First moments of a
- * block whose largest is below 1e-30, and second ones below fp32's normal numbers, become zero; a value that is not finite makes the scale of
- * its block NaN.  Codes, parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
+ * block whose largest is below 1e-30, and second ones below fp32's normal numbers, become zero; a value that is not finite makes
+ * the scale of its block NaN.  No tensor of a call may overlap another.  Codes, parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
 int dion_adamw8_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype, const uint64_t* M_ptrs,
                      const uint64_t* M_scale_ptrs, const uint64_t* V_ptrs, const uint64_t* V_scale_ptrs,
                      const uint64_t* step_ptrs, const int64_t* numels, int n, const float* lr_dev, float beta1,
