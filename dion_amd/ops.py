@@ -62,7 +62,8 @@ _SAME_DEVICE = _SameDevice()
 
 def _device_of(t: Tensor):
     """Context in which the current device is that of ``t``."""
-    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    index = t.get_device()
+    return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 _workspaces = {}
@@ -958,9 +959,10 @@ def _size_table(sizes: List[int]):
 
 
 def _step_pointers(steps: List[Tensor], index: int):
-    if set(map(_dtype, steps)) != {torch.float32} or set(map(_numel, steps)) != {1} or min(map(_get_device, steps)) < 0:
+    devices = set(map(_get_device, steps))
+    if set(map(_dtype, steps)) != {torch.float32} or set(map(_numel, steps)) != {1} or min(devices) < 0:
         raise TypeError("steps must be 0-d float32 GPU tensors")
-    if set(map(_get_device, steps)) != {index}:
+    if devices != {index}:
         raise ValueError(f"steps must be on the device of X, {index}")
     return ptr_table(map(_data_ptr, steps), len(steps))
 
@@ -1067,27 +1069,34 @@ def lion_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Tensor, bet
 ACTIVATIONS = {None: 0, "relu": 1, "relu_squared": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
 
 
-def _rows(t: Tensor) -> Tuple[Tensor, int]:
-    """A 2D tensor whose rows are dense and do not overlap (itself, or a copy), and the elements between them."""
-    rows, cols = t.shape
-    if t.stride(1) != 1 and cols > 1 or rows > 1 and t.stride(0) < cols:
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else cols)
-
-
-def _whole_chunks(t: Tensor, ld: int) -> bool:
-    return t.data_ptr() % 16 == 0 and ld % 8 == 0 and t.shape[1] % 8 == 0 and ld <= 1 << 21
+def _rows(t: Optional[Tensor], copy: int = 0) -> Tuple[Optional[Tensor], Optional[int], int, int]:
+    """A tensor (of any number of dimensions) as rows that are dense and do not overlap: itself, a view or a copy, which has to
+    live as long as its address is used; their address; the elements between them; ``copy`` if they are not whole 16-byte
+    chunks, else 0."""
+    if t is None:
+        return None, None, 0, 0
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    (rows, cols), (ld, inner) = t.shape, t.stride()
+    if inner != 1 and cols > 1 or rows > 1 and ld < cols:
+        t, ld = t.contiguous(), cols
+    elif rows <= 1:
+        ld = cols
+    address = t.data_ptr()
+    return t, address, ld, 0 if address % 16 == 0 and ld % 8 == 0 and cols % 8 == 0 and ld <= 1 << 21 else copy
 
 
 def _check_linear(name: str, t: Tensor, shape, index: int, fp32: bool = False) -> None:
-    if type(t) not in _PLAIN or not t.is_cuda:
-        _require_gpu(t, name)
+    if (type(t) in _PLAIN_SET and t.get_device() == index >= 0 and t.shape == shape and
+            (t.dtype == torch.bfloat16 or fp32 and t.dtype == torch.float32)):
+        return
+    _require_gpu(t, name)
     if t.dtype != torch.bfloat16 and not (fp32 and t.dtype == torch.float32):
         raise TypeError(f"linear: {name} must be torch.bfloat16{' or torch.float32' if fp32 else ''}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"linear: expected {name} of shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.get_device() != index:
-        raise ValueError(f"linear: {name} is on {t.device}, x on device {index}")
+        raise ValueError(f"linear: {name} is on {t.device}, another tensor on device {index}")
 
 
 def _check_weight(t: Tensor, name: str, weight: Tensor, side: int, activation: Optional[str]) -> int:
@@ -1146,31 +1155,26 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _flat(t: Tensor) -> Tensor:
-    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-
-
 def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
                    residual: Optional[Tensor], keep_slope: bool) -> Tuple[Tensor, Optional[Tensor]]:
     """``act(x W^T + b) + residual``, and with ``keep_slope`` and an activation act' at every element, in the 16 bits that
     ``linear_backward`` reads."""
     _check_linear_forward(x, weight, bias, activation, residual)
     act, lead = ACTIVATIONS[activation], x.shape[:-1]
-    x, fan_out = _flat(x), weight.shape[0]
-    tokens = x.shape[0]
+    fan_out, fan_in = weight.shape
     with _device_of(x):
-        y = torch.empty(tokens, fan_out, dtype=torch.bfloat16, device=x.device)
-        # (in whole 16-byte chunks)
-        slope = torch.empty(tokens, -(-fan_out // 8) * 8, dtype=torch.int16, device=x.device) if keep_slope and act else None
-        (x, ldx), (w, ldw) = _rows(x), _rows(weight)
-        r, ldr = (None, 0) if residual is None else _rows(_flat(residual))
+        x, px, ldx, copy_x = _rows(x, _lib.DION_LINEAR_COPY_X)
+        w, pw, ldw, copy_w = _rows(weight, _lib.DION_LINEAR_COPY_W)
+        r, pr, ldr, _ = _rows(residual)
         b = None if bias is None else bias.contiguous()
-        copies = (0 if _whole_chunks(x, ldx) else _lib.DION_LINEAR_COPY_X) | (0 if _whole_chunks(w, ldw) else _lib.DION_LINEAR_COPY_W)
-        ws, nbytes = _linear_space(tokens, weight, False, act, copies)
-        check(_lib.load().dion_linear_forward(x.data_ptr(), ldx, w.data_ptr(), ldw, _ptr(b),
-                                              DION_BF16 if b is None else _dtype_code(b, "bias"), act, _ptr(r), ldr,
-                                              y.data_ptr(), _ptr(slope), tokens, weight.shape[1], fan_out, _ptr(ws), nbytes,
-                                              _stream_handle(x.device)), "linear")
+        tokens = x.shape[0]
+        y = x.new_empty((tokens, fan_out))
+        # (in whole 16-byte chunks)
+        slope = x.new_empty((tokens, -(-fan_out // 8) * 8), dtype=torch.int16) if keep_slope and act else None
+        ws, nbytes = _linear_space(tokens, weight, False, act, copy_x | copy_w)
+        check(_lib.load().dion_linear_forward(px, ldx, pw, ldw, _ptr(b), DION_BF16 if b is None else _dtype_code(b, "bias"),
+                                              act, pr, ldr, y.data_ptr(), _ptr(slope), tokens, fan_in, fan_out, _ptr(ws),
+                                              nbytes, _stream_handle(x.device)), "linear")
     return (y if len(lead) == 1 else y.view(*lead, fan_out)), slope
 
 
@@ -1182,25 +1186,18 @@ def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[st
     _check_linear_backward(dy, slope, activation, x, weight, need_dw, bias_dtype)
     act, lead = ACTIVATIONS[activation], dy.shape[:-1]
     fan_out, fan_in = weight.shape
-    dy = _flat(dy)
-    tokens = dy.shape[0]
     with _device_of(dy):
-        dy, lddy = _rows(dy)
-        copies = 0 if _whole_chunks(dy, lddy) else _lib.DION_LINEAR_COPY_DY
-        xr, ldx = _rows(_flat(x)) if need_dw else (None, 0)
-        w, ldw = _rows(weight) if need_dx else (None, 0)
-        if need_dw and not _whole_chunks(xr, ldx):
-            copies |= _lib.DION_LINEAR_COPY_X
-        if need_dx and not _whole_chunks(w, ldw):
-            copies |= _lib.DION_LINEAR_COPY_W
-        ws, nbytes = _linear_space(tokens, weight, True, act, copies)
-        new = lambda *shape, dtype=torch.bfloat16: torch.empty(shape, dtype=dtype, device=dy.device)  # noqa: E731
-        dx = new(tokens, fan_in) if need_dx else None
-        dw = new(fan_out, fan_in) if need_dw else None
-        db = new(fan_out, dtype=bias_dtype) if bias_dtype is not None else None
-        check(_lib.load().dion_linear_backward(dy.data_ptr(), lddy, _ptr(slope), act, _ptr(xr), ldx, _ptr(w), ldw, _ptr(dx),
-                                               _ptr(dw), _ptr(db), DION_BF16 if db is None else _dtype_code(db, "bias"), tokens,
-                                               fan_in, fan_out, _ptr(ws), nbytes, _stream_handle(dy.device)), "linear backward")
+        dy, pdy, lddy, copy_dy = _rows(dy, _lib.DION_LINEAR_COPY_DY)
+        x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
+        w, pw, ldw, copy_w = _rows(weight if need_dx else None, _lib.DION_LINEAR_COPY_W)
+        tokens = dy.shape[0]
+        ws, nbytes = _linear_space(tokens, weight, True, act, copy_x | copy_w | copy_dy)
+        dx = dy.new_empty((tokens, fan_in)) if need_dx else None
+        dw = dy.new_empty((fan_out, fan_in)) if need_dw else None
+        db = dy.new_empty((fan_out,), dtype=bias_dtype) if bias_dtype is not None else None
+        check(_lib.load().dion_linear_backward(pdy, lddy, _ptr(slope), act, px, ldx, pw, ldw, _ptr(dx), _ptr(dw), _ptr(db),
+                                               DION_BF16 if db is None else _dtype_code(db, "bias"), tokens, fan_in, fan_out,
+                                               _ptr(ws), nbytes, _stream_handle(dy.device)), "linear backward")
     if need_dx and len(lead) != 1:
         dx = dx.view(*lead, fan_in)
     return dx, dw, db
