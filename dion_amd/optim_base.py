@@ -64,7 +64,11 @@ class LiveScalars:
 
 class OrthoOptimizer(Optimizer):
     """Base class: orchestration, state and validation.  Subclasses implement
-    ``_shape_group_phases`` (a generator: work before / during / after the orthogonalization)."""
+    ``_shape_group_phases`` (a generator: work before / during / after the orthogonalization).
+
+    An ``algorithm="adamw"`` group of any of them may hold ``state_bits``: 8 keeps both moments in 8 bits, with a float32 scale
+    for every 128 elements, rounded at random without bias (``state_seed``, 0 by default); 32 keeps them in float32 beside
+    bfloat16 parameters; without it they have the parameters' dtype."""
 
     def __init__(self, params, distributed_mesh, algo_name: str, defaults: dict,
                  use_gram_newton_schulz: bool = False, use_triton: bool = False,
@@ -130,6 +134,8 @@ class OrthoOptimizer(Optimizer):
     def add_param_group(self, param_group: dict) -> None:
         """torch calls this from ``Optimizer.__init__`` for every group and users call it later; only a
         late group needs its state and device scalars made here (construction does it for all at once)."""
+        if "state_bits" in param_group:  # (refused before the group is added)
+            self._state_bits({**self.defaults, **param_group})
         super().add_param_group(param_group)
         if not getattr(self, "_constructed", False):
             return

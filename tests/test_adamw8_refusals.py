@@ -95,3 +95,16 @@ def test_group_option_stays_what_it_was():
         opt.param_groups[0]["state_bits"] = after
         with pytest.raises(ValueError, match="moments are"):
             opt._adamw_state(p, after)
+
+
+def test_a_refused_group_is_not_added():
+    from dion import Muon
+
+    opt = Muon([torch.nn.Parameter(torch.zeros(8, 8))], lr=0.1)
+    for kw in ({"algorithm": "adamw", "state_bits": 16}, {"state_bits": 8}):
+        with pytest.raises(ValueError, match="state_bits"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(8))], **kw})
+    assert len(opt.param_groups) == 1
+    p = torch.nn.Parameter(torch.zeros(8))
+    opt.add_param_group({"params": [p], "algorithm": "adamw", "state_bits": 8})
+    assert opt.state[p]["momentum"].dtype == torch.int8
