@@ -25,16 +25,16 @@ namespace dion {
 // ---------------------------------------------------------------------------------------------- activations
 static __device__ __forceinline__ float rcp_fast(float v) { return __builtin_amdgcn_rcpf(v); }
 
-// act(z), and act'(z) in `slope`.  Exponentials and quotients by the hardware's approximations (1 ulp): the result is rounded
-// to bf16, the slope to eleven bits.
+// act(z), and act'(z) in `slope`, for slope_pack2.  Exponentials and quotients by the hardware's approximations (1 ulp): the
+// result is rounded to bf16, the slope to eleven bits.
 template <int ACT>
 static __device__ __forceinline__ float activate(float z, float& slope) {
   if constexpr (ACT == kActRelu) {
     slope = z <= 0.f ? 0.f : 1.f;  // (where z is NaN the gradient goes on, and the value stays NaN)
     return z < 0.f ? 0.f : z;
   } else if constexpr (ACT == kActReluSquared) {
-    const float r = z < 0.f ? 0.f : z;
-    slope = 2.f * r;
+    const float r = z <= 0.f ? 0.f : z;  // (never -0, which has no code; NaN stays)
+    slope = r;  // (half of it: slope_pack2 doubles)
     return r * r;
   } else if constexpr (ACT == kActSilu) {
     const float s = rcp_fast(1.f + __expf(-z));
@@ -73,12 +73,12 @@ static __device__ __forceinline__ uint32_t slope_pack2(float a, float b) {
   if constexpr (ACT != kActReluSquared) {
     return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
   } else {
-    // Rounded to nine bits of mantissa; code 0 is zero (and 2^-63 and below), 0xffff NaN and everything past 2^65.
-    auto code = [](float s) {
-      const uint32_t c = (__float_as_uint(s) + 0x2000u) >> 14;
-      return min(c > (64u << 9) ? c - (64u << 9) : 0u, 0xffffu);
+    // Doubled and rounded to nine bits of mantissa; code 0 is zero (and 2^-63 and below), 0xffff NaN and everything past 2^65.
+    auto code = [](float half) {  // in the upper bits
+      const uint32_t twice = __builtin_elementwise_add_sat(__float_as_uint(half), 0x802000u);  // (a NaN may have a sign)
+      return min(__builtin_elementwise_sub_sat(twice, 64u << 23), 0x3fffffffu);
     };
-    return code(a) | code(b) << 16;
+    return code(a) >> 14 | (code(b) << 2 & 0xffff0000u);
   }
 }
 static __device__ __forceinline__ float slope_unpack(int act, uint16_t c) {
@@ -711,9 +711,10 @@ static int sum_rows(int rows) { return (rows + 1023) / 1024 * 8; }
 int lin_sum_parts(int rows) { return (rows + sum_rows(rows) - 1) / sum_rows(rows); }
 
 // One pass for what the products cannot read as it lies: dz, its column sums, and rows that are not whole chunks.  HBM: 6 bytes an
-// element with slopes, 8192 x 8192 92 us (4.4 TB/s); 4 bytes for a copy, 2 for sums alone (4096 x 2048 4.7 us).
+// element with slopes, 8192 x 8192 72 us (5.6 TB/s); 4 bytes for a copy, 2 for sums alone (4096 x 2048 4.7 us).
 // SLOPE: src is dy, and dz = dy * act'(z) goes on.  W: elements of src that are read at once; 8: every row is whole chunks.
-template <bool SLOPE, bool DST, bool SUM, int W>
+// NT: non-temporal loads of dy and the slopes, which nothing reads again.
+template <bool SLOPE, bool DST, bool SUM, int W, bool NT>
 __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restrict__ src, int64_t ld,
                                                           const uint16_t* __restrict__ slope, int act, int rows, int cols,
                                                           bf16_t* __restrict__ dst, float* __restrict__ partial, int per) {
@@ -728,7 +729,9 @@ __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restri
       const bf16_t* q = src + (int64_t)r * ld + c0;
       float v[8];
       if constexpr (W == 8) {
-        st_load8<bf16_t>(q, 0, v);
+        const u32x4_t w = NT ? __builtin_nontemporal_load((const u32x4_t*)q) : *(const u32x4_t*)q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
       } else if constexpr (W == 2) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {  // (an even number of columns)
@@ -741,7 +744,8 @@ __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restri
         for (int e = 0; e < 8; ++e) v[e] = c0 + e < cols ? bf16_to_f32(q[e]) : 0.f;
       }
       if constexpr (SLOPE) {
-        const u32x4_t s = *(const u32x4_t*)(slope + (int64_t)r * padded + c0);
+        const u32x4_t* sp = (const u32x4_t*)(slope + (int64_t)r * padded + c0);
+        const u32x4_t s = NT ? __builtin_nontemporal_load(sp) : *sp;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float f = slope_unpack(act, (uint16_t)(s[e >> 1] >> (16 * (e & 1))));
@@ -960,13 +964,21 @@ static hipError_t launch_prepare(const bf16_t* src, int64_t ld, const uint16_t* 
                                  float* partial, hipStream_t st) {
   const dim3 grid((cols + kPrepCols - 1) / kPrepCols, lin_sum_parts(rows));
   const uint64_t bytes = (uint64_t)src | (uint64_t)cols * 2 | (uint64_t)ld * 2;
-  auto go = [&](auto wc) {
-    hipLaunchKernelGGL((lin_prepare_kernel<SLOPE, DST, SUM, decltype(wc)::value>), grid, dim3(256), 0, st, src, ld, slope, act, rows,
-                       cols, dst, partial, sum_rows(rows));
+  auto go = [&](auto wc, auto ntc) {
+    hipLaunchKernelGGL((lin_prepare_kernel<SLOPE, DST, SUM, decltype(wc)::value, decltype(ntc)::value>), grid, dim3(256), 0, st, src, ld,
+                       slope, act, rows, cols, dst, partial, sum_rows(rows));
   };
-  if (bytes % 16 == 0) go(std::integral_constant<int, 8>());
-  else if (bytes % 4 == 0) go(std::integral_constant<int, 2>());
-  else go(std::integral_constant<int, 1>());
+  if constexpr (SLOPE) {
+    // From 30 MB of dy, slopes and dz on.  us without / with, dz alone and with its sums: 777 x 2736 5.0 / 5.2 and 4.5 / 4.8,
+    // 4096 x 2048 12.3 / 11.9 and 12.0 / 10.2, 4096 x 14336 69 / 67 and 70 / 66, 8192 x 8192 84 / 69 and 83 / 67.
+    if (bytes % 16 == 0 && (int64_t)rows * cols >= (5 << 20)) {
+      go(std::integral_constant<int, 8>(), std::true_type());
+      return hipGetLastError();
+    }
+  }
+  if (bytes % 16 == 0) go(std::integral_constant<int, 8>(), std::false_type());
+  else if (bytes % 4 == 0) go(std::integral_constant<int, 2>(), std::false_type());
+  else go(std::integral_constant<int, 1>(), std::false_type());
   return hipGetLastError();
 }
 
