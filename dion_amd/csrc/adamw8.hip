@@ -12,9 +12,11 @@
 // less than half a code (1 / 127 of v near the top of a block, more below) for beta2 = 0.99: rounded to nearest, v would
 // never move.  u in [0, 1) comes from a hash of (seed, step counter, element / 8), spread over the eight elements by a
 // Weyl sequence: the noise of an element is independent from step to step, and a run repeats bit for bit.
-// A second moment above zero (the normal numbers of fp32) keeps a code of at least 1: m may outlive it, and
-// nothing may then be divided by epsilon.  First moments of a block whose largest is below 1e-30 are dropped (127 / max would
-// overflow).  A block with a value that is not finite gets a scale of NaN, so that it shows in every later step.
+// m / s + u is a sum in fp32, exact for m = 0; of u's 24 bits 17 count beside a code of 64 and more.
+// A second moment above zero (the normal numbers of fp32) keeps a code of at least 1, and beside one of zero the first moment is
+// dropped: no first moment may be divided by epsilon alone in a later step.  First moments of a block whose largest is below 1e-30
+// are dropped too (127 / max would overflow).  A block with a value that is not finite gets a scale of NaN, so that it shows in
+// every later step.
 //
 // Bound by HBM: fp32 parameters, bf16 gradients 14.1 bytes per element (26 with fp32 states): X both ways 8, G 2, codes 4,
 // scales 0.125. That leaves about a hundred vector instructions an element (seventy with bf16 parameters), which a plain
@@ -204,12 +206,13 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adam8Tensors a, int n, cons
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float u = (float)((h + (uint32_t)e * 0x9E3779B9u) >> 8) * 0x1p-24f;
-      // m / s + u, plus 128: an unsigned code (a scale of zero or NaN has an inverse of zero)
-      const float c = floorf(fmaf(mv[e], minv, u + 128.0f));
+      const float least = __builtin_amdgcn_fmed3f(rt[e] * 0x1p127f, 0.0f, 1.0f);  // 1 where v > 0, else 0
+      // (a scale of zero or NaN has an inverse of zero; 128 is added to the code, where it is exact: added to u it would round
+      // the last of u's values up to a code of 1 for m = 0)
+      const float c = fmaf(floorf(fmaf(mv[e], minv, u)), least, 128.0f);
       mo[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(c, 1.0f, 255.0f), e & 3, mo[e >> 2]);
       const float t = rt[e] * rinv, k = floorf(t);
       const float up = fmaf(u, fmaf(2.0f, k, 1.0f), k * k) < t * t ? k + 1.0f : k;
-      const float least = __builtin_amdgcn_fmed3f(rt[e] * 0x1p127f, 0.0f, 1.0f);  // 1 where v > 0
       vo[e >> 2] = __builtin_amdgcn_cvt_pk_u8_f32(__builtin_amdgcn_fmed3f(up, least, 255.0f), e & 3, vo[e >> 2]);
     }
     mo ^= 0x80808080u;

@@ -486,9 +486,10 @@ int dion_adamw_fp32_state_step(const uint64_t* X_ptrs, int x_dtype, const uint64
  * The update is computed in fp32 from the decoded moments; the new ones are rounded up or down at random, without bias in
  * m and in v, by u = ((h + j 0x9E3779B9) mod 2^32 >> 8) 2^-24 for element 8 i + j of a tensor, h = mix(key ^ i), key =
  * mix(mix(seed) + step) (mix: adamw8.hip):  c = floor(m / s + u);  k = floor(t), t = sqrt(v) / q, or one more where
- * u (2 k + 1) < t^2 - k^2.  v > 0 keeps k >= 1.  Zeroed codes and scales are the state before the first step.  First moments of a
- * block whose largest is below 1e-30, and second ones below fp32's normal numbers, become zero; a value that is not finite makes
- * the scale of its block NaN.  No tensor of a call may overlap another.  Codes, parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
+ * u (2 k + 1) < t^2 - k^2 (sums in fp32).  v > 0 keeps k >= 1; beside v = 0, c = 0.  Zeroed codes and scales are the state
+ * before the first step.  First moments of a block whose largest is below 1e-30, and second ones below fp32's normal numbers,
+ * become zero; a value that is not finite makes the scale of its block NaN.  No tensor of a call may overlap another.  Codes,
+ * parameters and gradients may lie anywhere; 16-byte aligned (codes 8) they are moved in whole lines. */
 int dion_adamw8_step(const uint64_t* X_ptrs, int x_dtype, const uint64_t* G_ptrs, int g_dtype, const uint64_t* M_ptrs,
                      const uint64_t* M_scale_ptrs, const uint64_t* V_ptrs, const uint64_t* V_scale_ptrs,
                      const uint64_t* step_ptrs, const int64_t* numels, int n, const float* lr_dev, float beta1,
