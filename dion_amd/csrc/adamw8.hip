@@ -129,7 +129,10 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adam8Tensors a, int n, cons
   u32x2_t mr, vr;
   float s_old = 0.f, q_old = 0.f;
   auto fetch = [&](int64_t e0) {
-    if (e0 >= numel) return;
+    if (e0 >= numel) {  // (the last round's scales, which may be NaN, are another block's)
+      s_old = q_old = 0.f;
+      return;
+    }
     s_old = ms[e0 >> 7];
     q_old = vs[e0 >> 7];
     if (!vec || e0 + 8 > numel) return;
