@@ -5,6 +5,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -47,19 +48,28 @@ def _check_capture(y: Tensor) -> None:
                                "has its graph; delete or detach that result first")
 
 
+# The kernels have no tangents, and a tensor can have one without requires_grad.
+def _refuse_tangents(*operands: Optional[Tensor]) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
+        raise NotImplementedError("linear: forward-mode derivatives are not supported")
+
+
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
            residual: Optional[Tensor] = None) -> Tensor:
     """``act(x W^T + b) + residual``: ``x [..., fan_in]``, ``weight [fan_out, fan_in]``, ``residual [..., fan_out]`` bfloat16,
     ``bias [fan_out]`` bfloat16 or float32; returns bfloat16 ``[..., fan_out]``.  ``activation``: None, "relu", "relu_squared",
     "gelu" (by the error function), "gelu_tanh" or "silu".  Sums are float32, and the result is rounded once.
 
-    Differentiable once with respect to every tensor.  For the backward pass it keeps ``x``, the weight and, with an
-    activation, its slopes in 16 bits an element; the gradient that reaches ``z = x W^T + b`` is rounded to bfloat16 for the two
-    products, not for the bias.  Any sizes and strides; rows that are not whole 16-byte chunks (feature counts that are not
-    multiples of 8) are copied first.  ``weight`` and ``x`` must not change between the two passes (autograd raises).
+    Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
+    the backward pass it keeps ``x``, the weight and, with an activation, its slopes in 16 bits an element; the gradient that
+    reaches ``z = x W^T + b`` is rounded to bfloat16 for the two products, not for the bias.  Any sizes and strides; rows that are
+    not whole 16-byte chunks (feature counts that are not multiples of 8) are copied first.  ``weight`` and ``x`` must not
+    change between the two passes (autograd raises).
 
     Both passes can be captured into a graph, together, while no result of an earlier call on the same leaves on another
     stream has its autograd graph: that is refused (RuntimeError)."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         y = _Linear.apply(x, weight, bias, activation, residual)
