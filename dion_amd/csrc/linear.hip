@@ -57,9 +57,11 @@ static __device__ __forceinline__ float activate(float z, float& slope) {
     slope = cdf + z * 0.39894228f * e;
     return z * cdf;
   } else if constexpr (ACT == kActGeluTanh) {
-    const float u = 0.79788456f * z * (1.f + 0.044715f * z * z);
+    // (past |z| = 100, where s is 0 or 1, the square stands still: none that leaves fp32 meets 1 - s = 0)
+    const float zz = fminf(z * z, 1e4f);
+    const float u = 0.79788456f * z * (1.f + 0.044715f * zz);
     const float s = rcp_fast(1.f + __expf(-2.f * u));  // (1 + tanh u) / 2
-    slope = s + 2.f * z * s * (1.f - s) * 0.79788456f * (1.f + 0.134145f * z * z);
+    slope = s + z * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * zz);
     return z * s;
   } else {
     slope = 1.f;
