@@ -16,7 +16,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, activation, residual):
         need = ctx.needs_input_grad
         y, slope = ops.linear_forward(x, weight, bias, activation, residual, need[0] or need[1] or need[2])
-        ctx.save_for_backward(x if need[1] else None, weight, slope)
+        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, slope)
         ctx.activation = activation
         ctx.bias_dtype = bias.dtype if bias is not None and need[2] else None
         return y
@@ -61,10 +61,11 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     "gelu" (by the error function), "gelu_tanh" or "silu".  Sums are float32, and the result is rounded once.
 
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
-    the backward pass it keeps ``x``, the weight and, with an activation, its slopes in 16 bits an element; the gradient that
-    reaches ``z = x W^T + b`` is rounded to bfloat16 for the two products, not for the bias.  Any sizes and strides; rows that are
-    not whole 16-byte chunks (feature counts that are not multiples of 8) are copied first.  ``weight`` and ``x`` must not
-    change between the two passes (autograd raises).
+    the backward pass it keeps ``x`` where the weight needs a gradient, the weight where ``x`` does and, with an activation, its
+    slopes in 16 bits an element; what it keeps must not change between the two passes (autograd raises).  The gradient that
+    reaches ``z = x W^T + b`` is rounded to bfloat16 for the two products, not for the bias.  Any sizes and strides, up to
+    2^21 - 8 features and 2^30 tokens; rows that are not whole 16-byte chunks (feature counts that are not multiples of 8) are
+    copied first.
 
     Both passes can be captured into a graph, together, while no result of an earlier call on the same leaves on another
     stream has its autograd graph: that is refused (RuntimeError)."""

@@ -1099,10 +1099,14 @@ def _check_linear(name: str, t: Tensor, shape, index: int, fp32: bool = False) -
         raise ValueError(f"linear: {name} is on {t.device}, another tensor on device {index}")
 
 
-def _check_weight(t: Tensor, name: str, weight: Tensor, side: int, activation: Optional[str]) -> int:
-    """A weight and the tensor whose last dimension fits its dimension ``side``; returns their device's index."""
+def _check_activation(activation: Optional[str]) -> None:
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
+
+
+def _check_weight(t: Tensor, name: str, weight: Tensor, side: int, activation: Optional[str]) -> int:
+    """A weight and the tensor whose last dimension fits its dimension ``side``; returns their device's index."""
+    _check_activation(activation)
     ts, ws = t.shape, weight.shape
     if len(ws) != 2 or len(ts) < 1 or ts[-1] != ws[side]:
         raise ValueError(f"linear: {name} of shape {tuple(ts)} does not fit a weight of shape {tuple(ws)}")
@@ -1124,20 +1128,34 @@ def _check_linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], act
 
 
 def _check_linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
-                           weight: Tensor, need_dw: bool, bias_dtype: Optional[torch.dtype]) -> None:
-    index, lead, ws = _check_weight(dy, "dy", weight, 0, activation), dy.shape[:-1], weight.shape
+                           weight: Optional[Tensor], need_dx: bool, need_dw: bool,
+                           bias_dtype: Optional[torch.dtype]) -> Tuple[int, int]:
+    """Returns the weight's shape.  (Without a weight its rows' length is that of ``x``, and 1 where only ``db`` is asked for.)"""
+    ds = dy.shape
+    if need_dw and x is None:
+        raise ValueError("linear: the gradient of the weight needs x")
+    if weight is not None:
+        index, (fan_out, fan_in) = _check_weight(dy, "dy", weight, 0, activation), weight.shape
+    else:
+        _check_activation(activation)
+        if need_dx:
+            raise ValueError("linear: the gradient of x needs the weight")
+        index = dy.get_device()
+        _check_linear("dy", dy, ds, index)
+        if len(ds) < 1 or ds[-1] == 0 or need_dw and (x.dim() < 1 or x.shape[-1] == 0):
+            raise ValueError(f"linear: dy of shape {tuple(ds)} belongs to no weight")
+        fan_out, fan_in = ds[-1], x.shape[-1] if need_dw else 1
     if (slope is None) != (activation is None):
         raise ValueError(f"linear: activation {activation!r} goes with{'out' if activation is None else ''} slopes")
     if slope is not None:
-        want = (lead.numel(), -(-ws[0] // 8) * 8)
+        want = (ds[:-1].numel(), -(-fan_out // 8) * 8)
         if slope.get_device() != index or slope.dtype != torch.int16 or tuple(slope.shape) != want or not slope.is_contiguous():
             raise ValueError(f"linear: expected the slopes that the forward pass kept, int16 of shape {want} on device {index}")
     if need_dw:
-        if x is None:
-            raise ValueError("linear: the gradient of the weight needs x")
-        _check_linear("x", x, lead + ws[1:], index)
+        _check_linear("x", x, ds[:-1] + (fan_in,), index)
     if bias_dtype not in (None, torch.bfloat16, torch.float32):
         raise TypeError(f"linear: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
+    return fan_out, fan_in
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1145,10 +1163,11 @@ def _linear_bytes(tokens: int, fan_in: int, fan_out: int, backward: bool, act: i
     return _lib.load().dion_linear_workspace_bytes(tokens, fan_in, fan_out, int(backward), act, copies)
 
 
-def _linear_space(tokens: int, weight: Tensor, backward: bool, act: int, copies: int) -> Tuple[Optional[Tensor], int]:
+def _linear_space(tokens: int, fan_in: int, fan_out: int, device: torch.device, backward: bool, act: int,
+                  copies: int) -> Tuple[Optional[Tensor], int]:
     # (the caching allocator's: a captured graph has its own, and no two calls in flight share one)
-    nbytes = _linear_bytes(tokens, weight.shape[1], weight.shape[0], backward, act, copies)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=weight.device) if nbytes else None), nbytes
+    nbytes = _linear_bytes(tokens, fan_in, fan_out, backward, act, copies)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None), nbytes
 
 
 def _ptr(t: Optional[Tensor]):
@@ -1171,7 +1190,7 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation
         y = x.new_empty((tokens, fan_out))
         # (in whole 16-byte chunks)
         slope = x.new_empty((tokens, -(-fan_out // 8) * 8), dtype=torch.int16) if keep_slope and act else None
-        ws, nbytes = _linear_space(tokens, weight, False, act, copy_x | copy_w)
+        ws, nbytes = _linear_space(tokens, fan_in, fan_out, x.device, False, act, copy_x | copy_w)
         check(_lib.load().dion_linear_forward(px, ldx, pw, ldw, _ptr(b), DION_BF16 if b is None else _dtype_code(b, "bias"),
                                               act, pr, ldr, y.data_ptr(), _ptr(slope), tokens, fan_in, fan_out, _ptr(ws),
                                               nbytes, _stream_handle(x.device)), "linear")
@@ -1179,19 +1198,18 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation
 
 
 def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
-                    weight: Tensor, need_dx: bool, need_dw: bool,
+                    weight: Optional[Tensor], need_dx: bool, need_dw: bool,
                     bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients ``(dx, dW, db)`` of ``linear_forward``, None where not asked for (``bias_dtype`` None: no ``db``).  ``x`` is
-    read for ``dW``, the weight for ``dx``."""
-    _check_linear_backward(dy, slope, activation, x, weight, need_dw, bias_dtype)
+    read for ``dW``, the weight for ``dx``; either may be None without."""
+    fan_out, fan_in = _check_linear_backward(dy, slope, activation, x, weight, need_dx, need_dw, bias_dtype)
     act, lead = ACTIVATIONS[activation], dy.shape[:-1]
-    fan_out, fan_in = weight.shape
     with _device_of(dy):
         dy, pdy, lddy, copy_dy = _rows(dy, _lib.DION_LINEAR_COPY_DY)
         x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
         w, pw, ldw, copy_w = _rows(weight if need_dx else None, _lib.DION_LINEAR_COPY_W)
         tokens = dy.shape[0]
-        ws, nbytes = _linear_space(tokens, weight, True, act, copy_x | copy_w | copy_dy)
+        ws, nbytes = _linear_space(tokens, fan_in, fan_out, dy.device, True, act, copy_x | copy_w | copy_dy)
         dx = dy.new_empty((tokens, fan_in)) if need_dx else None
         dw = dy.new_empty((fan_out, fan_in)) if need_dw else None
         db = dy.new_empty((fan_out,), dtype=bias_dtype) if bias_dtype is not None else None
