@@ -34,18 +34,39 @@ class _Linear(torch.autograd.Function):
 
 # A leaf's accumulation node runs on the stream on which it was made and lives as long as a graph that holds it.  Recorded by a
 # capture, a backward pass that meets a node of another stream makes that stream wait inside the capture, and torch then ends the
-# process.  So a node keeps the stream of the first product that it is seen in, and a capture on another one is refused
-# before its backward pass.
+# process.  torch does not say which stream that is, so a node keeps the stream of the first product that it is seen in: as a
+# leaf among the operands, or below a weight or bias that is a cast or view of one.  A capture looks at every node below its result and
+# is refused before its backward pass where one has another stream.
 _ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros((), requires_grad=True)).node)
-_STREAM = "dion_amd.linear: stream"
+_STREAM, _CHECKED = "dion_amd.linear: stream", "dion_amd.linear: captured on"
 
 
-def _check_capture(y: Tensor) -> None:
-    stream, capturing = ops._stream_handle(y.device), torch.cuda.is_current_stream_capturing()
-    for node, _index in y.grad_fn.next_functions:
-        if isinstance(node, _ACCUMULATE) and node.metadata.setdefault(_STREAM, stream) != stream and capturing:
+def _check_leaves(nodes: list, device: torch.device, stream: int, capturing: bool) -> None:
+    seen = set()
+    while nodes:
+        node = nodes.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        if not isinstance(node, _ACCUMULATE):
+            if not capturing or node.metadata.get(_CHECKED) != stream:
+                nodes.extend(below for below, _index in node.next_functions)
+        elif node.variable.device == device and node.metadata.setdefault(_STREAM, stream) != stream and capturing:
             raise RuntimeError("linear: captured while a result of an earlier product with the same leaf, on another stream, still "
                                "has its graph; delete or detach that result first")
+
+
+def _check_capture(y: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
+    stream = ops._stream_handle(y.device)
+    with ops._device_of(y):
+        capturing = torch.cuda.is_current_stream_capturing()
+    if capturing:
+        _check_leaves([y.grad_fn], y.device, stream, True)
+        y.grad_fn.metadata[_CHECKED] = stream  # (the next product above it goes no further than this)
+        return
+    nodes = [node for node, _index in y.grad_fn.next_functions if isinstance(node, _ACCUMULATE)]
+    nodes += [t.grad_fn for t in (weight, bias) if t is not None and t.grad_fn is not None]
+    _check_leaves(nodes, y.device, stream, False)
 
 
 # The kernels have no tangents, and a tensor can have one without requires_grad.
@@ -68,12 +89,14 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     copied first.
 
     Both passes can be captured into a graph, together, while no result of an earlier call on the same leaves on another
-    stream has its autograd graph: that is refused (RuntimeError)."""
+    stream has its autograd graph: that is refused (RuntimeError), for leaves among the operands and below a weight or bias that is
+    a cast or a view.  A leaf that another operation has used on another stream, and whose result still has its graph, is not
+    noticed: torch ends the process in the backward pass of such a capture, as it does without this product."""
     if forward_ad._current_level >= 0:
         _refuse_tangents(x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         y = _Linear.apply(x, weight, bias, activation, residual)
-        _check_capture(y)
+        _check_capture(y, weight, bias)
         return y
     return ops.linear_forward(x, weight, bias, activation, residual, False)[0]
