@@ -8,11 +8,11 @@
 // the codes is fp32 with fused multiply-adds; root and quotient are the hardware's (1 ulp each).
 //
 // Rounding to a code is up or down at random, unbiased in m and in v:  c = floor(m / s + u),  k = floor(t) or one more
-// with probability (t^2 - floor(t)^2) / (2 floor(t) + 1), t = sqrt(v) / q.  A step changes v by 1 - beta2 of the difference to g^2,
-// less than half a code (1 / 127 of v near the top of a block, more below) for beta2 = 0.99: rounded to nearest, v would
-// never move.  u in [0, 1) comes from a hash of (seed, step counter, element / 8), spread over the eight elements by a
+// with probability (t^2 - floor(t)^2) / (2 floor(t) + 1), t = sqrt(v) / q.  A step without a gradient takes 1 - beta2 off v, and half a
+// code is 1 / k of v at code k: rounded to nearest, v would stand still at codes below 1 / (1 - beta2), which is 20 for beta2 = 0.95,
+// 100 for 0.99 and all of them from 0.9961 on.  u in [0, 1) comes from a hash of (seed, step counter, element / 8), spread over the eight elements by a
 // Weyl sequence: the noise of an element is independent from step to step, and a run repeats bit for bit.
-// m / s + u is a sum in fp32, exact for m = 0; of u's 24 bits 17 count beside a code of 64 and more.
+// m / s + u is a sum in fp32, exact for m = 0; beside a code of 64 and more 17 of u's 24 bits count (a mean off by 2^-18 of a code).
 // A second moment above zero (the normal numbers of fp32) keeps a code of at least 1, and beside one of zero the first moment is
 // dropped: no first moment may be divided by epsilon alone in a later step.  First moments of a block whose largest is below 1e-30
 // are dropped too (127 / max would overflow).  A block with a value that is not finite gets a scale of NaN, so that it shows in
@@ -23,7 +23,8 @@
 // translation of the formulas takes up. us of the update alone, 2 x (50304 x 768) with fp32 parameters and bf16 gradients / 2 x
 // (32000 x 4096) in fp32 / 2 x (32003 x 1001) in bf16, cautious: that translation 259 / 885 / 205; half the vector instructions
 // (packed conversions, clamps by medians, the hardware's root and quotient) 212 / 810 / 130; two rounds a workgroup past the
-// caches 203 / 780 / 129. That is 5.4 TB/s for the first two, 5.0 for the third, which is half in the caches.
+// caches 203 / 780 / 129. Codes whose offset is added behind the rounding, and none beside v = 0: 205 / 789 / 130, which is 5.3, 5.4
+// and 5.0 TB/s (the third is half in the caches).
 #include "elementwise.h"
 
 namespace dion {
