@@ -38,22 +38,29 @@ class _Linear(torch.autograd.Function):
 # leaf among the operands, or below a weight or bias that is a cast or view of one.  A capture looks at every node below its result and
 # is refused before its backward pass where one has another stream.
 _ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros((), requires_grad=True)).node)
-_STREAM, _CHECKED = "dion_amd.linear: stream", "dion_amd.linear: captured on"
+_STREAM, _EAGER, _CAPTURED = ("dion_amd.linear: " + key for key in ("stream", "leaves noted on", "leaves captured on"))
+
+
+def _below(node) -> list:
+    return [below for below, _index in node.next_functions]
 
 
 def _check_leaves(nodes: list, device: torch.device, stream: int, capturing: bool) -> None:
-    seen = set()
+    """Looks at every leaf below ``nodes``; a node that an earlier call has looked below is passed by."""
+    done, seen = _CAPTURED if capturing else _EAGER, set()
     while nodes:
         node = nodes.pop()
         if node is None or node in seen:
             continue
-        seen.add(node)
         if not isinstance(node, _ACCUMULATE):
-            if not capturing or node.metadata.get(_CHECKED) != stream:
-                nodes.extend(below for below, _index in node.next_functions)
+            if node.metadata.get(done) != stream:
+                seen.add(node)
+                nodes.extend(_below(node))
         elif node.variable.device == device and node.metadata.setdefault(_STREAM, stream) != stream and capturing:
             raise RuntimeError("linear: captured while a result of an earlier product with the same leaf, on another stream, still "
                                "has its graph; delete or detach that result first")
+    for node in seen:  # (only here: none of them stays marked where one was refused)
+        node.metadata[done] = stream
 
 
 def _check_capture(y: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
@@ -61,12 +68,11 @@ def _check_capture(y: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
     with ops._device_of(y):
         capturing = torch.cuda.is_current_stream_capturing()
     if capturing:
-        _check_leaves([y.grad_fn], y.device, stream, True)
-        y.grad_fn.metadata[_CHECKED] = stream  # (the next product above it goes no further than this)
-        return
-    nodes = [node for node, _index in y.grad_fn.next_functions if isinstance(node, _ACCUMULATE)]
-    nodes += [t.grad_fn for t in (weight, bias) if t is not None and t.grad_fn is not None]
-    _check_leaves(nodes, y.device, stream, False)
+        nodes = [y.grad_fn]
+    else:
+        nodes = [node for node in _below(y.grad_fn) if isinstance(node, _ACCUMULATE)]
+        nodes += [t.grad_fn for t in (weight, bias) if t is not None and t.grad_fn is not None]
+    _check_leaves(nodes, y.device, stream, capturing)
 
 
 # The kernels have no tangents, and a tensor can have one without requires_grad.

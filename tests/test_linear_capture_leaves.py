@@ -1,5 +1,6 @@
 """Which leaves of a product's graph are looked at before a capture goes on, on the host: the products are stood in for by torch's own."""
 import contextlib
+import sys
 
 import pytest
 import torch
@@ -79,3 +80,18 @@ def test_a_graph_that_was_made_eagerly_and_is_used_in_a_capture(product):
     product(x, half)
     with pytest.raises(RuntimeError, match="still has its graph"):
         product(x, half, captured=True)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_node_is_looked_at_once(product, monkeypatch, captured):
+    """Weights that one deep graph makes, and products along a residual stream: what a call looks at is what is new in it."""
+    module, looked = sys.modules["dion_amd.linear"], []
+    below = module._below
+    monkeypatch.setattr(module, "_below", lambda node: looked.append(1) or below(node))
+    made = torch.ones(16, 16).requires_grad_()
+    for _ in range(300):
+        made = made * 1.0
+    h = torch.ones(4, 16, dtype=torch.bfloat16)
+    for _ in range(40):
+        h = h + product(h.relu(), made.bfloat16(), captured=captured)
+    assert h.requires_grad and 300 <= len(looked) <= 300 + 40 * 8
