@@ -11,7 +11,8 @@ from .newton_schulz import (  # noqa: F401
     zeropower_via_newtonschulz5,
 )
 
-from .linear import linear  # noqa: E402,F401
+from .linear import gated_linear, linear  # noqa: E402,F401
+from .layers import embedding, layer_norm  # noqa: E402,F401
 from .hip_graph import CudaGraphOptimizer, HipGraphOptimizer  # noqa: E402,F401
 from .optimizers import Dion2, Dion3, Muon, NorDion2, NorMuon  # noqa: E402,F401
 
@@ -23,7 +24,10 @@ __all__ = [
     "Dion3",
     "HipGraphOptimizer",
     "CudaGraphOptimizer",
+    "embedding",
+    "gated_linear",
     "gram_newton_schulz",
+    "layer_norm",
     "linear",
     "newton_schulz_triton",
     "ns_line_1",

@@ -6,7 +6,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libdion_hip.so")
-SOURCES = ["gemm_nt.hip", "elementwise.hip", "select_scope.hip", "ns_small.hip", "scalar_opts.hip", "adamw8.hip", "linear.hip", "capi.hip"]
+SOURCES = ["gemm_nt.hip", "elementwise.hip", "select_scope.hip", "ns_small.hip", "scalar_opts.hip", "adamw8.hip", "linear.hip", "gated.hip", "layer_norm.hip",
+           "embedding.hip", "capi.hip"]
 
 # -packed-fp32-ops off: keep hipcc from forming v_pk_*_f32 out of scalar float code.
 HIPCC_FLAGS = [

@@ -14,9 +14,9 @@ LIB_PATH = os.path.join(_HERE, "libdion_hip.so")
 DION_BF16 = 0
 DION_F32 = 1
 DION_NS_GRAM = 1
-DION_LINEAR_COPY_X, DION_LINEAR_COPY_W, DION_LINEAR_COPY_DY = 1, 2, 4
+DION_LINEAR_COPY_X, DION_LINEAR_COPY_W, DION_LINEAR_COPY_DY, DION_GATED_COPY_UP = 1, 2, 4, 8
 DION_NS_STATIC_SCRATCH_BYTES = 64 << 20
-ABI_VERSION = 15  # dion_abi_version() of the library these signatures describe
+ABI_VERSION = 16  # dion_abi_version() of the library these signatures describe
 
 _u64p = ctypes.POINTER(ctypes.c_uint64)
 _i64p = ctypes.POINTER(ctypes.c_int64)
@@ -108,6 +108,23 @@ SIGNATURES = {
                                     c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "dion_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                      c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dion_gated_kept_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dion_gated_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "dion_gated_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int,
+                                   c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dion_gated_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
+                                    c_void_p, c_size_t, c_void_p]),
+    "dion_layer_norm_forward": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                                        c_void_p, c_int, c_int, c_float, c_void_p]),
+    "dion_layer_norm_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "dion_layer_norm_backward": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dion_embedding_forward": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_void_p, c_int,
+                                       c_void_p]),
+    "dion_embedding_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dion_embedding_backward": (c_int, [c_void_p, c_int, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_float, c_int64,
+                                        c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "dion_adamw_step": (c_int, [_u64p, _u64p, c_int, _u64p, _u64p, c_int, _u64p, _i64p, c_int, c_void_p, c_float,
                                 c_float, c_float, c_void_p, c_float, c_int, c_void_p]),
     "dion_adamw_fp32_state_step": (c_int, [_u64p, c_int, _u64p, c_int, _u64p, _u64p, _u64p, _i64p, c_int, c_void_p,

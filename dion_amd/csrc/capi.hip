@@ -9,6 +9,7 @@
 
 #include "../../include/dion_hip.h"
 #include "elementwise.h"
+#include "layers.h"
 #include "linear.h"
 
 using namespace dion;
@@ -38,7 +39,7 @@ static inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 static inline bool aligned16(uint64_t p) { return (p & 15) == 0; }
 
 extern "C" const char* dion_last_error(void) { return g_err; }
-extern "C" int dion_abi_version(void) { return 15; }
+extern "C" int dion_abi_version(void) { return 16; }
 
 // ---------------------------------------------------------------------------------------------
 // Kernel-level GEMMs
@@ -2086,5 +2087,395 @@ extern "C" int dion_linear_backward(const void* dy, int64_t lddy, const void* sl
     p.C = (bf16_t*)dw;
     HIP_TRY(launch_lin_product(p, st), who);
   }
+  return DION_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gated projections
+// ---------------------------------------------------------------------------------------------
+struct GatedSpace {
+  size_t x, wg, wu, dz, sums, scratch, total;
+};
+static GatedSpace gated_space(int tokens, int fan_in, int fan_out, int backward, int copies) {
+  GatedSpace s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  const int kp = round8(fan_in), np = round8(fan_out);
+  s.x = take(copies & DION_LINEAR_COPY_X ? (size_t)tokens * kp * 2 : 0);
+  s.wg = take(copies & DION_LINEAR_COPY_W ? (size_t)fan_out * kp * 2 : 0);
+  s.wu = take(copies & DION_GATED_COPY_UP ? (size_t)fan_out * kp * 2 : 0);
+  s.dz = s.sums = at;
+  size_t scratch = 0;
+  auto most = [&](size_t bytes) { scratch = bytes > scratch ? bytes : scratch; };  // (products run one after the other)
+  if (backward && tokens > 0) {
+    s.dz = take((size_t)tokens * 2 * np * 2);
+    s.sums = take((size_t)lin_sum_parts(tokens) * 2 * fan_out * sizeof(float));
+    most(pair_product_scratch(tokens, fan_in, fan_out));
+    most(lin_product_scratch(np + fan_out, fan_in, tokens, 1, 1));
+    most(lin_product_scratch(fan_out, fan_in, tokens, 1, 1));
+  } else if (tokens > 0) {
+    most(gated_product_scratch(tokens, fan_out, fan_in));
+  }
+  s.scratch = take(scratch);
+  s.total = at;
+  return s;
+}
+
+static int check_gated(const char* who, int tokens, int fan_in, int fan_out) {
+  if (int rc = check_linear(who, tokens, fan_in, fan_out, 0)) return rc;
+  if (fan_out > kLinMaxLd / 2 - 8) return fail(DION_E_INVALID, "%s: more than 2^20 - 8 columns of h", who);
+  return DION_OK;
+}
+static bool bad_dtype(int dtype) { return dtype != DION_BF16 && dtype != DION_F32; }
+static int check_space(const char* who, const void* workspace, size_t have, size_t need) {
+  if (need > 0 && (!workspace || have < need || !aligned16((uint64_t)(uintptr_t)workspace)))
+    return fail(DION_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, need, have);
+  return DION_OK;
+}
+
+static int check_kept(const char* who, const void* kept, int kept_bits) {
+  if (kept_bits != 24 && kept_bits != 32) return fail(DION_E_INVALID, "%s: %d bits kept", who, kept_bits);
+  if (!aligned16((uint64_t)(uintptr_t)kept)) return fail(DION_E_INVALID, "%s: kept is not 16-byte aligned", who);
+  return DION_OK;
+}
+
+extern "C" size_t dion_gated_kept_bytes(int tokens, int fan_out, int kept_bits) {
+  if (check_gated("dion_gated_kept_bytes", tokens, 1, fan_out) || check_kept("dion_gated_kept_bytes", nullptr, kept_bits)) return 0;
+  return gated_kept_bytes(tokens, fan_out, kept_bits == 32);
+}
+
+extern "C" size_t dion_gated_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int copies) {
+  if (check_gated("dion_gated_workspace_bytes", tokens, fan_in, fan_out)) return 0;
+  return gated_space(tokens, fan_in, fan_out, backward, copies).total;
+}
+
+// A copy of an operand in whole chunks where it is none: p and ld become the copy's.
+static hipError_t lin_copy(bool copy, const void** p, int64_t* ld, int rows, int cols, void* to, hipStream_t st) {
+  if (!copy) return hipSuccess;
+  if (hipError_t e = launch_lin_prepare((const bf16_t*)*p, *ld, nullptr, 0, rows, cols, (bf16_t*)to, nullptr, st)) return e;
+  *p = to;
+  *ld = round8(cols);
+  return hipSuccess;
+}
+
+extern "C" int dion_gated_forward(const void* x, int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up,
+                                  const void* bias_gate, int bias_gate_dtype, const void* bias_up, int bias_up_dtype,
+                                  int activation, void* h, void* kept, int kept_bits, int tokens, int fan_in, int fan_out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dion_gated_forward";
+  if (int rc = check_gated(who, tokens, fan_in, fan_out)) return rc;
+  if (activation < 0 || activation >= kActCount) return fail(DION_E_INVALID, "%s: activation %d", who, activation);
+  if ((bias_gate && bad_dtype(bias_gate_dtype)) || (bias_up && bad_dtype(bias_up_dtype)))
+    return fail(DION_E_INVALID, "%s: type of a bias", who);
+  if (tokens == 0) return DION_OK;
+  if (int rc = check_lin_rows(who, "x", x, ldx, tokens, fan_in)) return rc;
+  if (int rc = check_lin_rows(who, "w_gate", w_gate, ld_gate, fan_out, fan_in)) return rc;
+  if (int rc = check_lin_rows(who, "w_up", w_up, ld_up, fan_out, fan_in)) return rc;
+  if (!h) return fail(DION_E_INVALID, "%s: h is null", who);
+  if ((uintptr_t)h & 1) return fail(DION_E_INVALID, "%s: h is not 2-byte aligned", who);
+  if (kept)
+    if (int rc = check_kept(who, kept, kept_bits)) return rc;
+  const int copies = (lin_whole(x, ldx, fan_in) ? 0 : DION_LINEAR_COPY_X) | (lin_whole(w_gate, ld_gate, fan_in) ? 0 : DION_LINEAR_COPY_W) |
+                     (lin_whole(w_up, ld_up, fan_in) ? 0 : DION_GATED_COPY_UP);
+  const GatedSpace s = gated_space(tokens, fan_in, fan_out, 0, copies);
+  if (int rc = check_space(who, workspace, workspace_bytes, s.total)) return rc;
+  char* ws = (char*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_X, &x, &ldx, tokens, fan_in, ws + s.x, st), who);
+  HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_W, &w_gate, &ld_gate, fan_out, fan_in, ws + s.wg, st), who);
+  HIP_TRY(lin_copy(copies & DION_GATED_COPY_UP, &w_up, &ld_up, fan_out, fan_in, ws + s.wu, st), who);
+  GatedProduct p;
+  memset(&p, 0, sizeof(p));
+  p.X = (const bf16_t*)x;
+  p.Wg = (const bf16_t*)w_gate;
+  p.Wu = (const bf16_t*)w_up;
+  p.ldx = ldx;
+  p.ldg = ld_gate;
+  p.ldu = ld_up;
+  p.M = tokens;
+  p.N = fan_out;
+  p.K = fan_in;
+  p.H = (bf16_t*)h;
+  p.act = activation;
+  p.bg = bias_gate;
+  p.bu = bias_up;
+  p.bg_dtype = dt(bias_gate_dtype);
+  p.bu_dtype = dt(bias_up_dtype);
+  p.kept = kept;
+  p.wide = kept_bits == 32;
+  p.scratch = (float*)(ws + s.scratch);
+  HIP_TRY(launch_gated_product(p, st), who);
+  return DION_OK;
+}
+
+extern "C" int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kept_bits, const void* x, int64_t ldx,
+                                   const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate, void* dw_up,
+                                   void* db_gate, int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in,
+                                   int fan_out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "dion_gated_backward";
+  if (int rc = check_gated(who, tokens, fan_in, fan_out)) return rc;
+  if ((db_gate && bad_dtype(db_gate_dtype)) || (db_up && bad_dtype(db_up_dtype)))
+    return fail(DION_E_INVALID, "%s: type of a bias", who);
+  hipStream_t st = (hipStream_t)stream;
+  const int np = round8(fan_out);
+  if (tokens == 0) {  // sums over nothing
+    const int64_t all = (int64_t)fan_out * fan_in;
+    constexpr int kRun = 1 << 26;  // (a launch has fewer than 2^32 threads, sixteen of them an element)
+    for (void* dw : {dw_gate, dw_up})
+      for (int64_t at = 0; dw && at < all; at += kRun)
+        HIP_TRY(launch_lin_sum(nullptr, 0, (int)(all - at < kRun ? all - at : kRun), (bf16_t*)dw + at, 0, st), who);
+    if (db_gate) HIP_TRY(launch_lin_sum(nullptr, 0, fan_out, db_gate, dt(db_gate_dtype), st), who);
+    if (db_up) HIP_TRY(launch_lin_sum(nullptr, 0, fan_out, db_up, dt(db_up_dtype), st), who);
+    return DION_OK;
+  }
+  const bool dw = dw_gate || dw_up;
+  if (int rc = check_lin_rows(who, "dh", dh, ld_dh, tokens, fan_out)) return rc;
+  if (!kept) return fail(DION_E_INVALID, "%s: kept is null", who);
+  if (int rc = check_kept(who, kept, kept_bits)) return rc;
+  if (dw)
+    if (int rc = check_lin_rows(who, "x", x, ldx, tokens, fan_in)) return rc;
+  if (dx) {
+    if (int rc = check_lin_rows(who, "w_gate", w_gate, ld_gate, fan_out, fan_in)) return rc;
+    if (int rc = check_lin_rows(who, "w_up", w_up, ld_up, fan_out, fan_in)) return rc;
+  }
+  const int copies = (dw && !lin_whole(x, ldx, fan_in) ? DION_LINEAR_COPY_X : 0) |
+                     (dx && !lin_whole(w_gate, ld_gate, fan_in) ? DION_LINEAR_COPY_W : 0) |
+                     (dx && !lin_whole(w_up, ld_up, fan_in) ? DION_GATED_COPY_UP : 0);
+  const GatedSpace s = gated_space(tokens, fan_in, fan_out, 1, copies);
+  if (int rc = check_space(who, workspace, workspace_bytes, s.total)) return rc;
+  char* ws = (char*)workspace;
+  if (!dx && !dw && !db_gate && !db_up) return DION_OK;
+  bf16_t* dz = (bf16_t*)(ws + s.dz);
+  const int parts = lin_sum_parts(tokens);
+  float *sums_gate = (float*)(ws + s.sums), *sums_up = sums_gate + (size_t)parts * fan_out;
+  const bool sums = db_gate || db_up;
+  HIP_TRY(launch_gated_dz((const bf16_t*)dh, ld_dh, kept, kept_bits == 32, tokens, fan_out, dx || dw ? dz : nullptr,
+                          sums ? sums_gate : nullptr, sums ? sums_up : nullptr, st), who);
+  if (db_gate) HIP_TRY(launch_lin_sum(sums_gate, parts, fan_out, db_gate, dt(db_gate_dtype), st), who);
+  if (db_up) HIP_TRY(launch_lin_sum(sums_up, parts, fan_out, db_up, dt(db_up_dtype), st), who);
+  HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_X, &x, &ldx, tokens, fan_in, ws + s.x, st), who);
+  HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_W, &w_gate, &ld_gate, fan_out, fan_in, ws + s.wg, st), who);
+  HIP_TRY(lin_copy(copies & DION_GATED_COPY_UP, &w_up, &ld_up, fan_out, fan_in, ws + s.wu, st), who);
+  if (dx) {
+    PairProduct p;
+    p.P = dz;
+    p.P2 = dz + np;
+    p.Q = (const bf16_t*)w_gate;
+    p.Q2 = (const bf16_t*)w_up;
+    p.ldp = 2 * np;
+    p.ldq = ld_gate;
+    p.ldq2 = ld_up;
+    p.M = tokens;
+    p.N = fan_in;
+    p.K = fan_out;
+    p.C = (bf16_t*)dx;
+    p.scratch = (float*)(ws + s.scratch);
+    HIP_TRY(launch_pair_product(p, st), who);
+  }
+  LinProduct p;
+  memset(&p, 0, sizeof(p));
+  p.scratch = (float*)(ws + s.scratch);
+  p.ldp = 2 * np;
+  p.p_kmajor = p.q_kmajor = 1;
+  p.N = fan_in;
+  p.K = tokens;
+  p.Q = (const bf16_t*)x;
+  p.ldq = ldx;
+  const bool behind = dw_gate && dw_up && (char*)dw_up == (char*)dw_gate + (size_t)np * fan_in * 2;
+  if (dw_gate) {
+    p.P = dz;
+    p.M = behind ? np + fan_out : fan_out;
+    p.C = (bf16_t*)dw_gate;
+    HIP_TRY(launch_lin_product(p, st), who);
+  }
+  if (dw_up && !behind) {
+    p.P = dz + np;
+    p.M = fan_out;
+    p.C = (bf16_t*)dw_up;
+    HIP_TRY(launch_lin_product(p, st), who);
+  }
+  return DION_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Layer norm, embedding
+// ---------------------------------------------------------------------------------------------
+constexpr int kMostColumns = 1 << 24;
+
+static int check_rows(const char* who, const char* arg, const void* p, int64_t ld, int dtype, int rows, int cols) {
+  if (bad_dtype(dtype)) return fail(DION_E_INVALID, "%s: type of %s", who, arg);
+  if (rows > 0 && !p) return fail(DION_E_INVALID, "%s: %s is null", who, arg);
+  if ((uintptr_t)p % (dtype == DION_F32 ? 4 : 2)) return fail(DION_E_INVALID, "%s: %s is not aligned to its elements", who, arg);
+  if (rows > 1 && ld < cols)
+    return fail(DION_E_INVALID, "%s: rows of %s overlap (%lld elements apart, %d long)", who, arg, (long long)ld, cols);
+  return DION_OK;
+}
+
+static int check_norm(const char* who, int rows, int width) {
+  if (rows < 0 || width < 1 || width > kMostColumns) return fail(DION_E_INVALID, "%s: %d rows of %d", who, rows, width);
+  return DION_OK;
+}
+
+extern "C" int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype,
+                                       const void* bias, int bias_dtype, void* y, int y_dtype, float* mean, float* rstd, int rows,
+                                       int width, float eps, void* stream) {
+  const char* who = "dion_layer_norm_forward";
+  if (int rc = check_norm(who, rows, width)) return rc;
+  if (int rc = check_rows(who, "x", x, ldx, x_dtype, rows, width)) return rc;
+  if (int rc = check_rows(who, "y", y, width, y_dtype, rows, width)) return rc;
+  if (weight)
+    if (int rc = check_rows(who, "weight", weight, width, weight_dtype, 1, width)) return rc;
+  if (bias)
+    if (int rc = check_rows(who, "bias", bias, width, bias_dtype, 1, width)) return rc;
+  if (!mean != !rstd) return fail(DION_E_INVALID, "%s: mean and rstd go together", who);
+  if (!(eps >= 0.f)) return fail(DION_E_INVALID, "%s: eps %g", who, (double)eps);
+  if (rows == 0) return DION_OK;
+  NormArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x;
+  a.ldx = rows > 1 ? ldx : width;
+  a.w = weight;
+  a.b = bias;
+  a.y = y;
+  a.mean = mean;
+  a.rstd = rstd;
+  a.rows = rows;
+  a.width = width;
+  a.x_dtype = dt(x_dtype);
+  a.y_dtype = dt(y_dtype);
+  a.w_dtype = dt(weight_dtype);
+  a.b_dtype = dt(bias_dtype);
+  a.eps = eps;
+  HIP_TRY(launch_norm_forward(a, (hipStream_t)stream), who);
+  return DION_OK;
+}
+
+extern "C" size_t dion_layer_norm_workspace_bytes(int rows, int width) {
+  if (check_norm("dion_layer_norm_workspace_bytes", rows, width)) return 0;
+  return norm_partial_floats(rows, width) * sizeof(float);
+}
+
+extern "C" int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype,
+                                        const void* weight, int weight_dtype, const float* mean, const float* rstd, void* dx,
+                                        void* dweight, void* dbias, int bias_dtype, int rows, int width, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+  const char* who = "dion_layer_norm_backward";
+  if (int rc = check_norm(who, rows, width)) return rc;
+  if (int rc = check_rows(who, "dy", dy, lddy, y_dtype, rows, width)) return rc;
+  if (int rc = check_rows(who, "x", x, ldx, x_dtype, rows, width)) return rc;
+  if (weight)
+    if (int rc = check_rows(who, "weight", weight, width, weight_dtype, 1, width)) return rc;
+  if (dx)
+    if (int rc = check_rows(who, "dx", dx, width, x_dtype, 1, width)) return rc;
+  if (dweight)
+    if (int rc = check_rows(who, "dweight", dweight, width, weight_dtype, 1, width)) return rc;
+  if (dbias)
+    if (int rc = check_rows(who, "dbias", dbias, width, bias_dtype, 1, width)) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  if (rows == 0) {  // sums over nothing
+    if (dweight) HIP_TRY(launch_lin_sum(nullptr, 0, width, dweight, dt(weight_dtype), st), who);
+    if (dbias) HIP_TRY(launch_lin_sum(nullptr, 0, width, dbias, dt(bias_dtype), st), who);
+    return DION_OK;
+  }
+  if (!mean || !rstd) return fail(DION_E_INVALID, "%s: mean or rstd is null", who);
+  if (dweight || dbias)
+    if (int rc = check_space(who, workspace, workspace_bytes, norm_partial_floats(rows, width) * sizeof(float))) return rc;
+  if (!dx && !dweight && !dbias) return DION_OK;
+  NormArgs a;
+  memset(&a, 0, sizeof(a));
+  a.x = x;
+  a.ldx = rows > 1 ? ldx : width;
+  a.w = weight;
+  a.mean = (float*)mean;
+  a.rstd = (float*)rstd;
+  a.rows = rows;
+  a.width = width;
+  a.x_dtype = dt(x_dtype);
+  a.y_dtype = dt(y_dtype);
+  a.w_dtype = dt(weight_dtype);
+  a.b_dtype = dt(bias_dtype);
+  a.dy = dy;
+  a.lddy = rows > 1 ? lddy : width;
+  a.dx = dx;
+  a.partial = (float*)workspace;
+  a.dw = dweight;
+  a.db = dbias;
+  HIP_TRY(launch_norm_backward(a, st), who);
+  return DION_OK;
+}
+
+static int check_embedding(const char* who, int ids_bits, int tokens, int vocab, int width) {
+  if (ids_bits != 32 && ids_bits != 64) return fail(DION_E_INVALID, "%s: ids of %d bits", who, ids_bits);
+  if (tokens < 0 || vocab < 1 || width < 1) return fail(DION_E_INVALID, "%s: %d tokens, table of %d x %d", who, tokens, vocab, width);
+  if (tokens > (1 << 30) || vocab > (1 << 24) || width > kMostColumns)
+    return fail(DION_E_INVALID, "%s: more than 2^30 tokens, 2^24 rows or 2^24 columns", who);
+  return DION_OK;
+}
+static int check_ids(const char* who, const void* ids, int ids_bits, int tokens) {
+  if (tokens > 0 && !ids) return fail(DION_E_INVALID, "%s: ids is null", who);
+  if ((uintptr_t)ids % (ids_bits / 8)) return fail(DION_E_INVALID, "%s: ids is not aligned to its elements", who);
+  return DION_OK;
+}
+
+extern "C" int dion_embedding_forward(const void* ids, int ids_bits, int tokens, const void* w, int64_t ldw, int w_dtype, int vocab,
+                                      int width, float scale, void* y, int y_dtype, void* stream) {
+  const char* who = "dion_embedding_forward";
+  if (int rc = check_embedding(who, ids_bits, tokens, vocab, width)) return rc;
+  if (int rc = check_ids(who, ids, ids_bits, tokens)) return rc;
+  if (int rc = check_rows(who, "w", w, ldw, w_dtype, vocab, width)) return rc;
+  if (int rc = check_rows(who, "y", y, width, y_dtype, tokens, width)) return rc;
+  if (tokens == 0) return DION_OK;
+  EmbeddingArgs a;
+  memset(&a, 0, sizeof(a));
+  a.ids = ids;
+  a.ids64 = ids_bits == 64;
+  a.tokens = tokens;
+  a.vocab = vocab;
+  a.width = width;
+  a.scale = scale;
+  a.w = w;
+  a.ldw = vocab > 1 ? ldw : width;
+  a.w_dtype = dt(w_dtype);
+  a.y = y;
+  a.y_dtype = dt(y_dtype);
+  HIP_TRY(launch_embedding_forward(a, (hipStream_t)stream), who);
+  return DION_OK;
+}
+
+extern "C" size_t dion_embedding_workspace_bytes(int tokens, int vocab, int width) {
+  if (check_embedding("dion_embedding_workspace_bytes", 64, tokens, vocab, width)) return 0;
+  return embedding_space_bytes(tokens, vocab, width);
+}
+
+extern "C" int dion_embedding_backward(const void* ids, int ids_bits, int tokens, const void* dy, int64_t lddy, int y_dtype, int vocab,
+                                       int width, float scale, int64_t padding, void* dw, int w_dtype, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  const char* who = "dion_embedding_backward";
+  if (int rc = check_embedding(who, ids_bits, tokens, vocab, width)) return rc;
+  if (int rc = check_ids(who, ids, ids_bits, tokens)) return rc;
+  if (int rc = check_rows(who, "dy", dy, lddy, y_dtype, tokens, width)) return rc;
+  if (int rc = check_rows(who, "dw", dw, width, w_dtype, vocab, width)) return rc;
+  if (padding >= vocab) return fail(DION_E_INVALID, "%s: padding %lld of %d rows", who, (long long)padding, vocab);
+  if (int rc = check_space(who, workspace, workspace_bytes, embedding_space_bytes(tokens, vocab, width))) return rc;
+  EmbeddingArgs a;
+  memset(&a, 0, sizeof(a));
+  a.ids = ids;
+  a.ids64 = ids_bits == 64;
+  a.tokens = tokens;
+  a.vocab = vocab;
+  a.width = width;
+  a.padding = padding < 0 ? -1 : padding;
+  a.scale = scale;
+  a.y_dtype = dt(y_dtype);
+  a.dy = dy;
+  a.lddy = tokens > 1 ? lddy : width;
+  a.dw = dw;
+  a.w_dtype = dt(w_dtype);
+  a.space = workspace;
+  HIP_TRY(launch_embedding_backward(a, (hipStream_t)stream), who);
   return DION_OK;
 }

@@ -1,0 +1,401 @@
+// Layer norm of rows of x:  m = mean x,  r = 1 / sqrt(mean (x - m)^2 + eps),  xh = (x - m) r,  y = xh w + b,
+// and its gradients, with g = dy w:  dx = r (g - mean g - xh mean(g xh)),  dw = sum over the rows of dy xh,  db = of dy.
+// Rows stay in registers between the two sums of a pass (the variance is that of the centred values: no difference of large
+// numbers), so x and dy are read once.  Sums fp32, in an order that depends on the sizes alone.
+#include "layers.h"
+
+namespace dion {
+
+constexpr int kNormWide = 16384;  // columns past which a row is read again instead of kept
+
+// Weight or bias of the V columns from c on; `none` without.
+template <int V>
+static __device__ __forceinline__ void param(const void* p, int dtype, int c, bool in, float none, float* v) {
+  if (!p) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = none;
+  } else if (dtype) {
+    Piece<float, V> q;
+    q.load((const float*)p + c, in);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = q.get(e);
+  } else {
+    Piece<bf16_t, V> q;
+    q.load((const bf16_t*)p + c, in);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = q.get(e);
+  }
+}
+
+// The sum of v over the G threads of a row; `at`: LDS of the row's wavefronts that nothing else uses before the next barrier but one.
+template <int G>
+static __device__ __forceinline__ float row_sum(float v, float* at) {
+  v = wave_sum(v);
+  if constexpr (G > 64) {
+    if ((threadIdx.x & 63) == 0) at[(threadIdx.x % G) >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < G / 64; ++k) v += at[k];
+  }
+  return v;
+}
+
+// A row by G threads of E elements each: elements (c G + t) V .. + V - 1 are chunk c of thread t.
+template <typename TX, typename TY, int G, int E, int V>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const NormArgs a) {
+  constexpr int NC = E / V, ROWS = (G < 256 ? 256 : G) / G;
+  __shared__ float sums[2][G / 64 + 1];
+  const int t = threadIdx.x % G;
+  const int row = blockIdx.x * ROWS + threadIdx.x / G;
+  if (row >= a.rows) return;  // (whole wavefronts; of a workgroup of one row none)
+  const TX* x = (const TX*)a.x + (int64_t)row * a.ldx;
+  Piece<TX, V> px[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) px[c].load(x + (c * G + t) * V, (c * G + t) * V < a.width);
+  float v[E], s = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) s += v[c * V + e] = px[c].get(e);
+  const float n = 1.f / (float)a.width, mean = row_sum<G>(s, sums[0]) * n;
+  s = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[c * V + e] = (c * G + t) * V < a.width ? v[c * V + e] - mean : 0.f;
+      s += v[c * V + e] * v[c * V + e];
+    }
+  const float rstd = 1.f / sqrtf(row_sum<G>(s, sums[1]) * n + a.eps);
+  if (t == 0 && a.mean) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+  TY* y = (TY*)a.y + (int64_t)row * a.width;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * G + t) * V;
+    if (col >= a.width) continue;
+    float w[V], b[V];
+    param<V>(a.w, a.w_dtype, col, true, 1.f, w);
+    param<V>(a.b, a.b_dtype, col, true, 0.f, b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = fmaf(v[c * V + e] * rstd, w[e], b[e]);
+    Piece<TY, V>::store(y + col, w);
+  }
+}
+
+// The same for rows that registers do not hold, by 1024 threads that read them three times.
+template <typename TX, typename TY>
+__global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const NormArgs a) {
+  __shared__ float sums[2][17];
+  const int64_t row = blockIdx.x;
+  const TX* x = (const TX*)a.x + row * a.ldx;
+  TY* y = (TY*)a.y + row * a.width;
+  float s = 0.f;
+  for (int c = threadIdx.x; c < a.width; c += 1024) s += st_load<TX>(x, c);
+  const float n = 1.f / (float)a.width, mean = row_sum<1024>(s, sums[0]) * n;
+  s = 0.f;
+  for (int c = threadIdx.x; c < a.width; c += 1024) {
+    const float d = st_load<TX>(x, c) - mean;
+    s += d * d;
+  }
+  const float rstd = 1.f / sqrtf(row_sum<1024>(s, sums[1]) * n + a.eps);
+  if (threadIdx.x == 0 && a.mean) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+  for (int c = threadIdx.x; c < a.width; c += 1024) {
+    float w[1], b[1];
+    param<1>(a.w, a.w_dtype, c, true, 1.f, w);
+    param<1>(a.b, a.b_dtype, c, true, 0.f, b);
+    st_store<TY>(y, c, fmaf((st_load<TX>(x, c) - mean) * rstd, w[0], b[0]));
+  }
+}
+
+// dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy: sixteen wavefronts take
+// 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them.
+template <typename TX, typename TY, int G, int E, int V>
+__global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
+  constexpr int NC = E / V, ROWS = 1024 / G;
+  __shared__ float sums[2][16][2];
+  __shared__ float half[ROWS > 1 ? ROWS / 2 * G * E : 1];
+  const int t = threadIdx.x % G, group = threadIdx.x / G, wave = threadIdx.x >> 6;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t first = (int64_t)blockIdx.x * ROWS;
+  const float n = 1.f / (float)a.width;
+  float w[E], dw[E] = {}, db[E] = {};
+#pragma unroll
+  for (int c = 0; c < NC; ++c) param<V>(a.w, a.w_dtype, (c * G + t) * V, (c * G + t) * V < a.width, 1.f, w + c * V);
+  Piece<TX, V> px[NC];
+  Piece<TY, V> pd[NC];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t row) __attribute__((always_inline)) {  // (zeros behind the last row and the last column: they add nothing)
+    const bool in = row < a.rows;
+    const TX* x = (const TX*)a.x + row * a.ldx;
+    const TY* dy = (const TY*)a.dy + row * a.lddy;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = (c * G + t) * V;
+      px[c].load(x + col, in && col < a.width);
+      pd[c].load(dy + col, in && col < a.width);
+    }
+    mean = in ? a.mean[row] : 0.f;
+    rstd = in ? a.rstd[row] : 0.f;
+  };
+  constexpr bool AHEAD = E == 8;  // (sixteen elements a thread leave no registers for the next ones)
+  if constexpr (AHEAD) fetch(first + group);
+  for (int buf = 0; first < a.rows; first += step, buf ^= 1) {  // (the same for the whole workgroup)
+    const int64_t row = first + group;
+    if constexpr (!AHEAD) fetch(row);
+    float xh[E], g[E], s0 = 0.f, s1 = 0.f;
+    const float r = rstd;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int i = c * V + e;
+        xh[i] = (c * G + t) * V < a.width ? (px[c].get(e) - mean) * r : 0.f;
+        const float d = pd[c].get(e);
+        dw[i] = fmaf(d, xh[i], dw[i]);
+        db[i] += d;
+        g[i] = d * w[i];
+        s0 += g[i];
+        s1 = fmaf(g[i], xh[i], s1);
+      }
+    if constexpr (AHEAD) fetch(row + step);
+    if (!a.dx) continue;
+    s0 = wave_sum(s0);
+    s1 = wave_sum(s1);
+    if constexpr (G > 64) {
+      if ((threadIdx.x & 63) == 0) {
+        sums[buf][wave][0] = s0;
+        sums[buf][wave][1] = s1;
+      }
+      __syncthreads();
+      s0 = s1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < G / 64; ++k) {
+        s0 += sums[buf][group * (G / 64) + k][0];
+        s1 += sums[buf][group * (G / 64) + k][1];
+      }
+    }
+    s0 *= n;
+    s1 *= n;
+    if (row < a.rows) {
+      TX* dx = (TX*)a.dx + row * a.width;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int col = (c * G + t) * V;
+        if (col >= a.width) continue;
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = r * (g[c * V + e] - s0 - xh[c * V + e] * s1);
+        Piece<TX, V>::store(dx + col, o);
+      }
+    }
+  }
+  if (!a.partial) return;
+  // The groups' sums meet in LDS, the upper half of them added to the lower one until one is left.
+  auto meet = [&](float* v) __attribute__((always_inline)) {
+    if constexpr (ROWS > 1) {
+#pragma unroll
+      for (int h = ROWS / 2; h > 0; h /= 2) {
+        __syncthreads();
+        if (group >= h && group < 2 * h)
+#pragma unroll
+          for (int i = 0; i < E; ++i) half[((group - h) * E + i) * G + t] = v[i];
+        __syncthreads();
+        if (group < h)
+#pragma unroll
+          for (int i = 0; i < E; ++i) v[i] += half[(group * E + i) * G + t];
+      }
+    }
+  };
+  meet(dw);
+  meet(db);
+  if (group > 0) return;
+  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = (c * G + t) * V;
+    if (col >= a.width) continue;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      out[col + e] = dw[c * V + e];
+      out[a.width + col + e] = db[c * V + e];
+    }
+  }
+}
+
+// dx of rows that registers do not hold.
+template <typename TX, typename TY>
+__global__ __launch_bounds__(1024) void norm_backward_wide_kernel(const NormArgs a) {
+  __shared__ float sums[2][17];
+  const int64_t row = blockIdx.x;
+  const TX* x = (const TX*)a.x + row * a.ldx;
+  const TY* dy = (const TY*)a.dy + row * a.lddy;
+  const float n = 1.f / (float)a.width, mean = a.mean[row], r = a.rstd[row];
+  float s0 = 0.f, s1 = 0.f, w[1];
+  for (int c = threadIdx.x; c < a.width; c += 1024) {
+    param<1>(a.w, a.w_dtype, c, true, 1.f, w);
+    const float g = st_load<TY>(dy, c) * w[0];
+    s0 += g;
+    s1 = fmaf(g, (st_load<TX>(x, c) - mean) * r, s1);
+  }
+  s0 = row_sum<1024>(s0, sums[0]) * n;
+  s1 = row_sum<1024>(s1, sums[1]) * n;
+  TX* dx = (TX*)a.dx + row * a.width;
+  for (int c = threadIdx.x; c < a.width; c += 1024) {
+    param<1>(a.w, a.w_dtype, c, true, 1.f, w);
+    st_store<TX>(dx, c, r * (st_load<TY>(dy, c) * w[0] - s0 - (st_load<TX>(x, c) - mean) * r * s1));
+  }
+}
+
+// ... and the sums of dy xh and dy over a run of `per` rows, a column a thread.
+template <typename TX, typename TY>
+__global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a, int per) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.width) return;
+  const int64_t r0 = (int64_t)blockIdx.y * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
+  float dw = 0.f, db = 0.f;
+#pragma unroll 4
+  for (int64_t r = r0; r < r1; ++r) {
+    const float d = st_load<TY>((const TY*)a.dy + r * a.lddy, c);
+    dw = fmaf(d, (st_load<TX>((const TX*)a.x + r * a.ldx, c) - a.mean[r]) * a.rstd[r], dw);
+    db += d;
+  }
+  float* out = a.partial + (int64_t)blockIdx.y * 2 * a.width;
+  out[c] = dw;
+  out[a.width + c] = db;
+}
+
+// dw and db from the parts' sums: sixteen columns of a workgroup, sixteen threads a column.
+__global__ __launch_bounds__(256) void norm_join_kernel(const NormArgs a, int parts) {
+  __shared__ float sums[16][17];
+  const int tx = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
+  const bool in = c < 2 * a.width;
+  float s = 0.f;
+  if (in)
+#pragma unroll 4
+    for (int k = g; k < parts; k += 16) s += a.partial[(int64_t)k * 2 * a.width + c];
+  sums[g][tx] = s;
+  __syncthreads();
+  if (g == 0 && in) {
+    s = sums[0][tx];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sums[k][tx];
+    void* out = c < a.width ? a.dw : a.db;
+    const int at = c < a.width ? c : c - a.width, dtype = c < a.width ? a.w_dtype : a.b_dtype;
+    if (!out) return;
+    if (dtype) ((float*)out)[at] = s;
+    else ((bf16_t*)out)[at] = f32_to_bf16(s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+// Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows fill.
+static int norm_threads(int width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 2048 ? 256 : width <= 4096 ? 512 : 1024; }
+static int norm_parts(int rows, int width) {
+  if (width > kNormWide) return rows < 128 ? rows : 128;
+  const int at_once = 1024 / norm_threads(width);
+  const int wgs = (rows + at_once - 1) / at_once;
+  return wgs < 256 ? wgs : 256;
+}
+size_t norm_partial_floats(int rows, int width) { return rows > 0 ? (size_t)norm_parts(rows, width) * 2 * width : 0; }
+
+// Elements that one access can move: 8 (4 with fp32 on either side), 2 or 1, by what every row's start is a multiple of.
+static int norm_vec(const NormArgs& a, const void* other, int64_t ldo, int other_dtype) {
+  auto fits = [&](int v) {
+    auto ok = [&](const void* p, int64_t ld, int dtype) {
+      const uint64_t bytes = (uint64_t)v * (dtype ? 4 : 2), line = bytes < 16 ? bytes : 16;
+      return !p || (((uint64_t)p % line) == 0 && (uint64_t)ld * (dtype ? 4 : 2) % line == 0);
+    };
+    return a.width % v == 0 && ok(a.x, a.ldx, a.x_dtype) && ok(other, ldo, other_dtype) && ok(a.w, 0, a.w_dtype) &&
+           ok(a.b, 0, a.b_dtype) && ok(a.dx, a.width, a.x_dtype);
+  };
+  const int most = a.x_dtype || other_dtype ? 4 : 8;
+  return fits(most) ? most : fits(2) ? 2 : 1;
+}
+
+template <typename F>
+static hipError_t norm_types(const NormArgs& a, F&& go) {
+  if (a.x_dtype) {
+    if (a.y_dtype) go((float*)nullptr, (float*)nullptr);
+    else go((float*)nullptr, (bf16_t*)nullptr);
+  } else {
+    if (a.y_dtype) go((bf16_t*)nullptr, (float*)nullptr);
+    else go((bf16_t*)nullptr, (bf16_t*)nullptr);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
+  if (a.rows <= 0 || a.width <= 0 || !a.x || !a.y || !a.mean != !a.rstd) return hipErrorInvalidValue;
+  return norm_types(a, [&](auto* tx, auto* ty) {
+    typedef std::remove_pointer_t<decltype(tx)> TX;
+    typedef std::remove_pointer_t<decltype(ty)> TY;
+    if (a.width > 2 * kNormWide) {
+      hipLaunchKernelGGL((norm_forward_wide_kernel<TX, TY>), dim3(a.rows), dim3(1024), 0, st, a);
+      return;
+    }
+    auto run = [&](auto gc, auto ec, auto vc) {
+      constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value, T = G < 256 ? 256 : G;
+      hipLaunchKernelGGL((norm_forward_kernel<TX, TY, G, E, V>), dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
+    };
+    auto sized = [&](auto vc) {
+      if (a.width <= 512) run(std::integral_constant<int, 64>(), std::integral_constant<int, 8>(), vc);
+      else if (a.width <= 2048) run(std::integral_constant<int, 64>(), std::integral_constant<int, 32>(), vc);
+      else if (a.width <= 8192) run(std::integral_constant<int, 256>(), std::integral_constant<int, 32>(), vc);
+      else run(std::integral_constant<int, 1024>(), std::integral_constant<int, 32>(), vc);
+    };
+    constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
+    const int v = norm_vec(a, a.y, a.width, a.y_dtype);
+    if (v == W) sized(std::integral_constant<int, W>());
+    else if (v == 2) sized(std::integral_constant<int, 2>());
+    else sized(std::integral_constant<int, 1>());
+  });
+}
+
+hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
+  if (a.rows <= 0 || a.width <= 0 || !a.x || !a.dy || !a.mean || !a.rstd || ((a.dw || a.db) && !a.partial)) return hipErrorInvalidValue;
+  NormArgs p = a;
+  p.b = nullptr;  // (not read)
+  if (!a.dw && !a.db) p.partial = nullptr;
+  const int parts = norm_parts(a.rows, a.width);
+  hipError_t e = norm_types(p, [&](auto* tx, auto* ty) {
+    typedef std::remove_pointer_t<decltype(tx)> TX;
+    typedef std::remove_pointer_t<decltype(ty)> TY;
+    if (a.width > kNormWide) {
+      const int per = (a.rows + parts - 1) / parts;
+      if (p.dx) hipLaunchKernelGGL((norm_backward_wide_kernel<TX, TY>), dim3(a.rows), dim3(1024), 0, st, p);
+      if (p.partial)
+        hipLaunchKernelGGL((norm_columns_kernel<TX, TY>), dim3((a.width + 255) / 256, parts), dim3(256), 0, st, p, per);
+      return;
+    }
+    auto run = [&](auto gc, auto ec, auto vc) {
+      constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value;
+      hipLaunchKernelGGL((norm_backward_kernel<TX, TY, G, E, V>), dim3(parts), dim3(1024), 0, st, p);
+    };
+    auto sized = [&](auto vc) {
+      typedef std::integral_constant<int, 8> eight;
+      if (a.width <= 512) run(std::integral_constant<int, 64>(), eight(), vc);
+      else if (a.width <= 1024) run(std::integral_constant<int, 128>(), eight(), vc);
+      else if (a.width <= 2048) run(std::integral_constant<int, 256>(), eight(), vc);
+      else if (a.width <= 4096) run(std::integral_constant<int, 512>(), eight(), vc);
+      else if (a.width <= 8192) run(std::integral_constant<int, 1024>(), eight(), vc);
+      else run(std::integral_constant<int, 1024>(), std::integral_constant<int, 16>(), vc);
+    };
+    constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
+    const int v = norm_vec(p, p.dy, p.lddy, p.y_dtype);
+    if (v == W) sized(std::integral_constant<int, W>());
+    else if (v == 2) sized(std::integral_constant<int, 2>());
+    else sized(std::integral_constant<int, 1>());
+  });
+  if (e != hipSuccess || !p.partial) return e;
+  hipLaunchKernelGGL(norm_join_kernel, dim3((2 * a.width + 15) / 16), dim3(256), 0, st, p, parts);
+  return hipGetLastError();
+}
+
+}  // namespace dion

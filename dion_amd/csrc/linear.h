@@ -1,4 +1,4 @@
-// Launchers of linear.hip (internal; the public surface is include/dion_hip.h).
+// Launchers of linear.hip and gated.hip (internal; the public surface is include/dion_hip.h).
 #pragma once
 #include "common.h"
 
@@ -28,6 +28,14 @@ struct LinProduct {
 };
 constexpr int64_t kLinMaxLd = int64_t(1) << 21;
 
+// How a product runs: on which tiles, and in how many parts of the reduction, of so many slabs of 64.
+enum LinTile { kLinFew, kLin128, kLinWide, kLin256 };
+struct LinPlan {
+  LinTile tile;
+  int splits, slabs;
+};
+LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor);
+
 size_t lin_product_scratch(int M, int N, int K, int p_kmajor, int q_kmajor);
 hipError_t launch_lin_product(const LinProduct& p, hipStream_t st);
 
@@ -37,5 +45,40 @@ int lin_sum_parts(int rows);
 hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slope, int act, int rows, int cols, bf16_t* dst,
                               float* partial, hipStream_t st);
 hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st);
+// C[M][N] = the sum of part[0 .. splits)[M][N], in that order, rounded once.
+hipError_t launch_lin_join(const float* part, int splits, int M, int N, bf16_t* C, hipStream_t st);
+
+// ---- gated.hip: h = act(x Wg^T + bg) * (x Wu^T + bu).  Operands as above; the rows of both weights are as long and as many.
+struct GatedProduct {
+  const bf16_t *X, *Wg, *Wu;
+  int64_t ldx, ldg, ldu;
+  int M, N, K;  // tokens, columns of h, columns of x
+  bf16_t* H;    // [M][N], dense
+  int act;
+  const void *bg, *bu;  // [N] or null
+  int bg_dtype, bu_dtype;
+  void* kept;  // gated_kept_bytes(M, N, wide), 16-byte aligned, or null: what launch_gated_dz reads
+  int wide;    // of 32 bits a value instead of 24
+  float* scratch;  // gated_product_scratch(M, N, K) bytes
+};
+size_t gated_kept_bytes(int M, int N, bool wide);
+size_t gated_product_scratch(int M, int N, int K);
+hipError_t launch_gated_product(const GatedProduct& p, hipStream_t st);
+
+// dz[rows][2 * (cols rounded up to 8)]: the gradients at x Wg^T + bg and, behind them in a row, at x Wu^T + bu, zeros behind column
+// cols; sums_gate, sums_up[lin_sum_parts(rows)][cols]: sums over runs of rows, in fp32, before rounding.  dz or the sums may be null.
+hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool wide, int rows, int cols, bf16_t* dz, float* sums_gate,
+                           float* sums_up, hipStream_t st);
+
+// C[M][N] = P Q + P2 Q2, sums over K each: P, P2 [M][K], ldp elements between rows, Q, Q2 [K][N].
+struct PairProduct {
+  const bf16_t *P, *P2, *Q, *Q2;
+  int64_t ldp, ldq, ldq2;
+  int M, N, K;
+  bf16_t* C;
+  float* scratch;  // pair_product_scratch(M, N, K) bytes
+};
+size_t pair_product_scratch(int M, int N, int K);
+hipError_t launch_pair_product(const PairProduct& p, hipStream_t st);
 
 }  // namespace dion

@@ -1,5 +1,6 @@
-"""The product a weight matrix stands for, with its bias, activation and residual in one kernel, and its gradients: what the
-matrices that the optimizers update compute, and where their gradients come from.
+"""The product a weight matrix stands for, with its bias, activation and residual in one kernel, and both projections of a gated
+feed-forward block with their product in one, and their gradients: what the matrices that the optimizers update compute, and where
+their gradients come from.
 """
 from typing import Optional
 
@@ -45,7 +46,7 @@ def _below(node) -> list:
     return [below for below, _index in node.next_functions]
 
 
-def _check_leaves(nodes: list, device: torch.device, stream: int, capturing: bool) -> None:
+def _check_leaves(nodes: list, device: torch.device, stream: int, capturing: bool, op: str = "linear") -> None:
     """Looks at every leaf below ``nodes``; a node that an earlier call has looked below is passed by."""
     done, seen = _CAPTURED if capturing else _EAGER, set()
     while nodes:
@@ -57,13 +58,13 @@ def _check_leaves(nodes: list, device: torch.device, stream: int, capturing: boo
                 seen.add(node)
                 nodes.extend(_below(node))
         elif node.variable.device == device and node.metadata.setdefault(_STREAM, stream) != stream and capturing:
-            raise RuntimeError("linear: captured while a result of an earlier product with the same leaf, on another stream, still "
+            raise RuntimeError(f"{op}: captured while a result of an earlier call with the same leaf, on another stream, still "
                                "has its graph; delete or detach that result first")
     for node in seen:  # (only here: none of them stays marked where one was refused)
         node.metadata[done] = stream
 
 
-def _check_capture(y: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
+def _check_capture(y: Tensor, *weights: Optional[Tensor], op: str = "linear") -> None:
     stream = ops._stream_handle(y.device)
     with ops._device_of(y):
         capturing = torch.cuda.is_current_stream_capturing()
@@ -71,14 +72,14 @@ def _check_capture(y: Tensor, weight: Tensor, bias: Optional[Tensor]) -> None:
         nodes = [y.grad_fn]
     else:
         nodes = [node for node in _below(y.grad_fn) if isinstance(node, _ACCUMULATE)]
-        nodes += [t.grad_fn for t in (weight, bias) if t is not None and t.grad_fn is not None]
-    _check_leaves(nodes, y.device, stream, capturing)
+        nodes += [t.grad_fn for t in weights if t is not None and t.grad_fn is not None]
+    _check_leaves(nodes, y.device, stream, capturing, op)
 
 
 # The kernels have no tangents, and a tensor can have one without requires_grad.
-def _refuse_tangents(*operands: Optional[Tensor]) -> None:
+def _refuse_tangents(*operands: Optional[Tensor], op: str = "linear") -> None:
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in operands):
-        raise NotImplementedError("linear: forward-mode derivatives are not supported")
+        raise NotImplementedError(f"{op}: forward-mode derivatives are not supported")
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: Optional[str] = None,
@@ -106,3 +107,44 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
         _check_capture(y, weight, bias)
         return y
     return ops.linear_forward(x, weight, bias, activation, residual, False)[0]
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight_gate, weight_up, bias_gate, bias_up, activation):
+        need = ctx.needs_input_grad
+        biases = ((bias_gate, need[3]), (bias_up, need[4]))
+        ctx.bias_dtypes = [b.dtype if b is not None and n else None for b, n in biases]
+        # (sums that are stored as float32 are worth it; whether one is asked for does not change the other gradients)
+        ctx.keep = 32 if any(b is not None and b.dtype == torch.float32 for b, _ in biases) else 24
+        h, kept = ops.gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation, ctx.keep)
+        ctx.save_for_backward(x if need[1] or need[2] else None, weight_gate, weight_up, kept)
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        need = ctx.needs_input_grad
+        return (*ops.gated_backward(dh, ctx.saved_tensors[3], ctx.keep, *ctx.saved_tensors[:3], *need[:3], *ctx.bias_dtypes), None)
+
+
+def gated_linear(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: Optional[Tensor] = None,
+                 bias_up: Optional[Tensor] = None, activation: Optional[str] = "silu") -> Tensor:
+    """Both projections of a gated feed-forward block, ``act(x Wg^T + bg) * (x Wu^T + bu)``: ``x [..., fan_in]``, the weights
+    ``[fan_out, fan_in]`` bfloat16 (the two halves of one tensor, or any two), the biases ``[fan_out]`` bfloat16 or float32;
+    returns bfloat16 ``[..., fan_out]``.  ``activation``: as for ``linear``; None for the product of the projections alone.  Sums are
+    float32, and the result is rounded once.
+
+    Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
+    the backward pass it keeps ``x``, the weights and ``act(g)`` and ``act'(g) u`` in 24 bits each (32 beside a float32
+    bias); the gradients that reach the two projections are rounded to bfloat16 for the products, not for the biases.  The gradients of the two
+    weights, where both are asked for, share an allocation.  Sizes, strides and captures as for ``linear``, up to 2^20 - 8
+    columns of the result."""
+    operands = (x, weight_gate, weight_up, bias_gate, bias_up)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(*operands, op="gated_linear")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        h = _GatedLinear.apply(*operands, activation)
+        _check_capture(h, *operands[1:], op="gated_linear")
+        return h
+    return ops.gated_forward(*operands, activation, 0)[0]

@@ -1219,3 +1219,244 @@ def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[st
     if need_dx and len(lead) != 1:
         dx = dx.view(*lead, fan_in)
     return dx, dw, db
+
+
+# ---------------------------------------------------------------------------------------------
+# gated projections, layer norm, embedding
+# ---------------------------------------------------------------------------------------------
+_BF16, _FLOATS, _IDS = (torch.bfloat16,), (torch.bfloat16, torch.float32), (torch.int64, torch.int32)
+
+
+def _check_operand(op: str, name: str, t: Tensor, shape, index: int, dtypes=_BF16) -> None:
+    if type(t) in _PLAIN_SET and t.get_device() == index >= 0 and t.shape == shape and t.dtype in dtypes:
+        return
+    _require_gpu(t, f"{op}: {name}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{op}: {name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{op}: expected {name} of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.get_device() != index:
+        raise ValueError(f"{op}: {name} is on {t.device}, another tensor on device {index}")
+
+
+def _space(nbytes: int, device: torch.device) -> Optional[Tensor]:
+    # (the caching allocator's: a captured graph has its own, and no two calls in flight share one)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _code(t: Optional[Tensor]) -> int:
+    return DION_F32 if t is not None and t.dtype == torch.float32 else DION_BF16
+
+
+def _viewed(t: Tensor, lead, cols: int) -> Tensor:
+    return t if len(lead) == 1 else t.view(*lead, cols)
+
+
+def _check_gated_weights(op: str, t: Tensor, name: str, gate: Tensor, up: Tensor, side: int) -> int:
+    ts, ws = t.shape, gate.shape
+    if len(ws) != 2 or len(ts) < 1 or ts[-1] != ws[side]:
+        raise ValueError(f"{op}: {name} of shape {tuple(ts)} does not fit weights of shape {tuple(ws)}")
+    if ws[0] == 0 or ws[1] == 0:
+        raise ValueError(f"{op}: empty weights of shape {tuple(ws)}")
+    index = t.get_device()
+    _check_operand(op, name, t, ts, index)
+    _check_operand(op, "weight_gate", gate, ws, index)
+    _check_operand(op, "weight_up", up, ws, index)
+    return index
+
+
+@functools.lru_cache(maxsize=4096)
+def _gated_bytes(tokens: int, fan_in: int, fan_out: int, backward: bool, copies: int) -> int:
+    return _lib.load().dion_gated_workspace_bytes(tokens, fan_in, fan_out, int(backward), copies)
+
+
+@functools.lru_cache(maxsize=4096)
+def _gated_kept(tokens: int, fan_out: int, bits: int) -> int:
+    return _lib.load().dion_gated_kept_bytes(tokens, fan_out, bits)
+
+
+def gated_forward(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: Optional[Tensor], bias_up: Optional[Tensor],
+                  activation: Optional[str], keep: int) -> Tuple[Tensor, Optional[Tensor]]:
+    """``act(x Wg^T + bg) * (x Wu^T + bu)``, and (``keep`` 24 or 32, not 0) two values of so many bits an element, that
+    ``gated_backward`` reads: 32 for the gradients of float32 biases."""
+    op = "gated_linear"
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{op}: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
+    index = _check_gated_weights(op, x, "x", weight_gate, weight_up, 1)
+    fan_out, fan_in = weight_gate.shape
+    for name, b in (("bias_gate", bias_gate), ("bias_up", bias_up)):
+        if b is not None:
+            _check_operand(op, name, b, weight_gate.shape[:1], index, _FLOATS)
+    lead = x.shape[:-1]
+    with _device_of(x):
+        x, px, ldx, copy_x = _rows(x, _lib.DION_LINEAR_COPY_X)
+        g, pg, ldg, copy_g = _rows(weight_gate, _lib.DION_LINEAR_COPY_W)
+        u, pu, ldu, copy_u = _rows(weight_up, _lib.DION_GATED_COPY_UP)
+        bg = None if bias_gate is None else bias_gate.contiguous()
+        bu = None if bias_up is None else bias_up.contiguous()
+        tokens = x.shape[0]
+        h = x.new_empty((tokens, fan_out))
+        kept = x.new_empty((_gated_kept(tokens, fan_out, keep),), dtype=torch.uint8) if keep else None
+        nbytes = _gated_bytes(tokens, fan_in, fan_out, False, copy_x | copy_g | copy_u)
+        ws = _space(nbytes, x.device)
+        check(_lib.load().dion_gated_forward(px, ldx, pg, ldg, pu, ldu, _ptr(bg), _code(bg), _ptr(bu), _code(bu),
+                                             ACTIVATIONS[activation], h.data_ptr(), _ptr(kept), keep, tokens, fan_in, fan_out,
+                                             _ptr(ws), nbytes, _stream_handle(x.device)), op)
+    return _viewed(h, lead, fan_out), kept
+
+
+def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], weight_gate: Tensor, weight_up: Tensor, need_dx: bool,
+                   need_dgate: bool, need_dup: bool, bias_gate_dtype: Optional[torch.dtype],
+                   bias_up_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], ...]:
+    """Gradients ``(dx, dWg, dWu, dbg, dbu)`` of ``gated_forward``, None where not asked for.  ``x`` is read for ``dWg`` and
+    ``dWu``, and may be None without.  Both asked for, they are the two ends of one allocation."""
+    op = "gated_linear"
+    index = _check_gated_weights(op, dh, "dh", weight_gate, weight_up, 0)
+    fan_out, fan_in = weight_gate.shape
+    lead, need_dw = dh.shape[:-1], need_dgate or need_dup
+    if need_dw:
+        if x is None:
+            raise ValueError(f"{op}: the gradients of the weights need x")
+        _check_operand(op, "x", x, lead + (fan_in,), index)
+    if kept is None or kept.get_device() != index or kept.dtype != torch.uint8 or not kept.is_contiguous() or \
+            keep not in (24, 32) or kept.numel() != _gated_kept(lead.numel(), fan_out, keep):
+        raise ValueError(f"{op}: expected what the forward pass kept of {lead.numel()} x {fan_out} elements, in {keep} bits")
+    for t in (bias_gate_dtype, bias_up_dtype):
+        if t is not None and t not in _FLOATS:
+            raise TypeError(f"{op}: a bias must be torch.bfloat16 or torch.float32, got {t}")
+    with _device_of(dh):
+        dh, pdh, lddh, _ = _rows(dh)
+        x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
+        g, pg, ldg, copy_g = _rows(weight_gate if need_dx else None, _lib.DION_LINEAR_COPY_W)
+        u, pu, ldu, copy_u = _rows(weight_up if need_dx else None, _lib.DION_GATED_COPY_UP)
+        tokens = dh.shape[0]
+        nbytes = _gated_bytes(tokens, fan_in, fan_out, True, copy_x | copy_g | copy_u)
+        ws = _space(nbytes, dh.device)
+        dx = dh.new_empty((tokens, fan_in)) if need_dx else None
+        dgate = dup = None
+        if need_dgate and need_dup:  # (one product: the second behind the first, which starts on a multiple of 8 rows)
+            both = dh.new_empty((-(-fan_out // 8) * 8 + fan_out, fan_in))
+            dgate, dup = both[:fan_out], both[-fan_out:]
+        elif need_dgate:
+            dgate = dh.new_empty((fan_out, fan_in))
+        elif need_dup:
+            dup = dh.new_empty((fan_out, fan_in))
+        dbg = dh.new_empty((fan_out,), dtype=bias_gate_dtype) if bias_gate_dtype is not None else None
+        dbu = dh.new_empty((fan_out,), dtype=bias_up_dtype) if bias_up_dtype is not None else None
+        check(_lib.load().dion_gated_backward(pdh, lddh, kept.data_ptr(), keep, px, ldx, pg, ldg, pu, ldu, _ptr(dx),
+                                              _ptr(dgate), _ptr(dup), _ptr(dbg), _code(dbg), _ptr(dbu), _code(dbu), tokens, fan_in,
+                                              fan_out, _ptr(ws), nbytes, _stream_handle(dh.device)), f"{op} backward")
+    return (_viewed(dx, lead, fan_in) if need_dx else None), dgate, dup, dbg, dbu
+
+
+def _check_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> int:
+    xs = x.shape
+    if len(xs) < 1 or xs[-1] == 0:
+        raise ValueError(f"layer_norm: x of shape {tuple(xs)} has no last dimension to normalise")
+    index = x.get_device()
+    _check_operand("layer_norm", "x", x, xs, index, _FLOATS)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _check_operand("layer_norm", name, t, xs[-1:], index, _FLOATS)
+    return index
+
+
+def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float, dtype: Optional[torch.dtype],
+                       keep: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """Layer norm over the last dimension, and with ``keep`` the rows' means and reciprocal deviations, float32 ``[2, rows]``, that
+    ``layer_norm_backward`` reads."""
+    _check_norm(x, weight, bias)
+    dtype = x.dtype if dtype is None else dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"layer_norm: dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+    lead, width = x.shape[:-1], x.shape[-1]
+    with _device_of(x):
+        x, px, ldx, _ = _rows(x)
+        w = None if weight is None else weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        rows = x.shape[0]
+        y = x.new_empty((rows, width), dtype=dtype)
+        stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
+        at = None if stats is None else stats.data_ptr()
+        check(_lib.load().dion_layer_norm_forward(px, ldx, _code(x), _ptr(w), _code(w), _ptr(b), _code(b), y.data_ptr(), _code(y),
+                                                  at, None if at is None else at + 4 * rows, rows, width, eps,
+                                                  _stream_handle(x.device)), "layer_norm")
+    return _viewed(y, lead, width), stats
+
+
+def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor, need_dx: bool, need_dw: bool,
+                        bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients ``(dx, dweight, dbias)`` of ``layer_norm_forward``, None where not asked for (``bias_dtype`` None: no ``dbias``)."""
+    op = "layer_norm"
+    index = _check_norm(x, weight, None)
+    _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
+    lead, width = x.shape[:-1], x.shape[-1]
+    rows = lead.numel()
+    if stats.get_device() != index or stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
+        raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
+    if need_dw and weight is None:
+        raise ValueError(f"{op}: the gradient of the weight needs the weight")
+    if bias_dtype is not None and bias_dtype not in _FLOATS:
+        raise TypeError(f"{op}: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
+    with _device_of(x):
+        dy, pdy, lddy, _ = _rows(dy)
+        x, px, ldx, _ = _rows(x)
+        w = None if weight is None else weight.contiguous()
+        dx = x.new_empty((rows, width)) if need_dx else None
+        dw = w.new_empty((width,)) if need_dw else None
+        db = x.new_empty((width,), dtype=bias_dtype) if bias_dtype is not None else None
+        nbytes = _lib.load().dion_layer_norm_workspace_bytes(rows, width) if need_dw or db is not None else 0
+        ws, at = _space(nbytes, x.device), stats.data_ptr()
+        check(_lib.load().dion_layer_norm_backward(pdy, lddy, _code(dy), px, ldx, _code(x), _ptr(w), _code(w), at, at + 4 * rows,
+                                                   _ptr(dx), _ptr(dw), _ptr(db), _code(db), rows, width, _ptr(ws), nbytes,
+                                                   _stream_handle(x.device)), f"{op} backward")
+    return (_viewed(dx, lead, width) if need_dx else None), dw, db
+
+
+def _check_ids(op: str, ids: Tensor, index: int) -> None:
+    _check_operand(op, "ids", ids, ids.shape, index, _IDS)
+
+
+def embedding_forward(ids: Tensor, weight: Tensor, scale: float, dtype: Optional[torch.dtype]) -> Tensor:
+    """``scale * weight[ids]``; NaN where an id is outside the table."""
+    op = "embedding"
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"{op}: expected a table of two dimensions that is not empty, got {tuple(weight.shape)}")
+    index = weight.get_device()
+    _check_operand(op, "weight", weight, weight.shape, index, _FLOATS)
+    _check_ids(op, ids, index)
+    dtype = weight.dtype if dtype is None else dtype
+    if dtype not in _FLOATS:
+        raise TypeError(f"{op}: dtype must be torch.bfloat16 or torch.float32, got {dtype}")
+    vocab, width = weight.shape
+    with _device_of(weight):
+        w, pw, ldw, _ = _rows(weight)
+        t = ids.contiguous()
+        y = weight.new_empty((*ids.shape, width), dtype=dtype)
+        check(_lib.load().dion_embedding_forward(t.data_ptr(), 64 if t.dtype == torch.int64 else 32, t.numel(), pw, ldw, _code(w),
+                                                 vocab, width, scale, y.data_ptr(), _code(y), _stream_handle(w.device)), op)
+    return y
+
+
+def embedding_backward(dy: Tensor, ids: Tensor, vocab: int, scale: float, padding_idx: Optional[int], dtype: torch.dtype) -> Tensor:
+    """The gradient ``[vocab, width]``, of ``dtype``, of the table of ``embedding_forward``: a row is ``scale`` times the sum of the
+    rows of ``dy`` whose id it is, in their order."""
+    op = "embedding"
+    index = dy.get_device()
+    _check_ids(op, ids, index)
+    if dy.dim() < 1 or dy.shape[-1] == 0:
+        raise ValueError(f"{op}: dy of shape {tuple(dy.shape)} belongs to no table")
+    width = dy.shape[-1]
+    _check_operand(op, "dy", dy, ids.shape + (width,), index, _FLOATS)
+    if dtype not in _FLOATS:
+        raise TypeError(f"{op}: the gradient must be torch.bfloat16 or torch.float32, got {dtype}")
+    with _device_of(dy):
+        dy, pdy, lddy, _ = _rows(dy)
+        t = ids.contiguous()
+        dw = dy.new_empty((vocab, width), dtype=dtype)
+        nbytes = _lib.load().dion_embedding_workspace_bytes(t.numel(), vocab, width)
+        ws = _space(nbytes, dy.device)
+        check(_lib.load().dion_embedding_backward(t.data_ptr(), 64 if t.dtype == torch.int64 else 32, t.numel(), pdy, lddy, _code(dy),
+                                                  vocab, width, scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(),
+                                                  _code(dw), _ptr(ws), nbytes, _stream_handle(dy.device)), f"{op} backward")
+    return dw
