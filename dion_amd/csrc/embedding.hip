@@ -10,7 +10,7 @@
 namespace dion {
 
 constexpr int kRun = 64;         // tokens of a partial sum
-constexpr int kSlice = 512;      // columns of a wavefront: eight a lane
+constexpr int kSlice = 512;      // columns: eight a lane of a wavefront
 constexpr int kIndexRows = 512;  // rows of a workgroup of the index, at most
 constexpr int kIndexWaves = 16;
 
@@ -56,15 +56,17 @@ struct IndexArgs {
   uint32_t *order, *first, *count;  // [tokens], [vocab + 1] (the last one: how many tokens have a gradient), [vocab]
 };
 
-// Workgroup g has the rows v with v % groups = g: row v / groups of its own.  Every workgroup reads all ids, twice: to count its own (by
-// wavefront and row) and those of the workgroups before it, which is where its part of `order` starts; then to place its
-// own.  A wavefront has a run of consecutive tokens and takes 64 of them at a time, equal ids among them together; so the
-// tokens of a row stay in order.
+// Workgroup g has the rows v with v % groups = g: row v / groups of its own.  Every workgroup reads all ids, and counts its own (by
+// wavefront and row) and those of the workgroups before it, which is where its part of `order` starts; then it places its own.  A
+// wavefront has a run of consecutive tokens; it lists those of the workgroup's rows in LDS, in order, and counts and places from
+// there, 64 at a time, equal ones together; so the tokens of a row stay in order.  Where the list is full it reads the ids again
+// instead.  Bound by the instructions that look at an id that is another workgroup's (255 of 256).
 template <typename ID>
 __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const IndexArgs a, int rows) {
-  constexpr int AHEAD = 16;  // ids of a lane on their way
+  constexpr int AHEAD = 16, LIST = 192;  // ids of a lane on their way; tokens in a wavefront's list
   extern __shared__ uint32_t at[];  // [kIndexWaves][rows]: counts, then where a wavefront's next token of the row goes
   __shared__ uint32_t sums[kIndexWaves], before;
+  __shared__ uint2 lists[kIndexWaves][LIST];  // token, row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x, mask = a.groups - 1, shift = __builtin_ctz(a.groups);
   for (int i = threadIdx.x; i < kIndexWaves * rows; i += kIndexWaves * 64) at[i] = 0;
@@ -73,41 +75,71 @@ __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const
   const int batches = (a.tokens + 63) / 64;
   const int b0 = (int)((int64_t)batches * wave / kIndexWaves), b1 = (int)((int64_t)batches * (wave + 1) / kIndexWaves);
   volatile uint32_t* const mine = at + wave * rows;  // (lanes read what others of the wavefront wrote)
-  uint32_t lower = 0;
-  auto scan = [&](auto placec) __attribute__((always_inline)) {
-    constexpr bool PLACE = decltype(placec)::value;
+  uint2* const list = lists[wave];
+  uint32_t lower = 0, listed = 0;  // (both the wavefront's)
+  // Every batch of 64 tokens of this wavefront: f(token of the lane, its row or -1, whether the row is this workgroup's).
+  auto batches_of = [&](auto&& f) __attribute__((always_inline)) {
     for (int b = b0; b < b1; b += AHEAD) {
       ID ids[AHEAD];
+      const int64_t t0 = (int64_t)b * 64 + lane;
+      const ID* p = (const ID*)a.ids + t0;
+      if (b + AHEAD <= b1 && (int64_t)(b + AHEAD) * 64 <= a.tokens) {
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int64_t t = (int64_t)(b + k) * 64 + lane;
-        ids[k] = b + k < b1 && t < a.tokens ? ((const ID*)a.ids)[t] : (ID)-1;
+        for (int k = 0; k < AHEAD; ++k) ids[k] = p[k * 64];
+      } else {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) ids[k] = b + k < b1 && t0 + k * 64 < a.tokens ? p[k * 64] : (ID)-1;
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        const bool valid = ids[k] >= 0 && ids[k] < (ID)a.vocab && ids[k] != (ID)a.padding;
-        const int id = valid ? (int)ids[k] : 0, row = id >> shift;
-        if constexpr (!PLACE) lower += valid && (id & mask) < g;
-        uint64_t left = __ballot(valid && (id & mask) == g);
-        while (left) {  // (every turn takes at least one token out)
-          const int leader = __builtin_ctzll(left);
-          const int r = __builtin_amdgcn_readlane(row, leader);
-          const uint64_t same = __ballot(row == r) & left;
-          if constexpr (PLACE) {
-            const uint32_t to = mine[r];
-            if ((same >> lane) & 1) a.order[to + __popcll(same & ((1ull << lane) - 1))] = (uint32_t)(b + k) * 64 + lane;
-            if (lane == leader) mine[r] = to + __popcll(same);
-          } else if (lane == leader) {
-            mine[r] = mine[r] + __popcll(same);
-          }
-          left &= ~same;
-        }
+        typedef std::make_unsigned_t<ID> U;
+        const bool valid = (U)ids[k] < (U)a.vocab && ids[k] != (ID)a.padding;
+        const uint32_t id = (uint32_t)ids[k];
+        f((uint32_t)t0 + k * 64, id, valid);
       }
     }
   };
-  scan(std::false_type());
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) lower += __shfl_xor(lower, d, 64);
+  // Tokens of the workgroup's rows, at most one a lane, in the lanes' order: counted, or placed.
+  auto take = [&](auto placec, uint32_t token, int row, bool is) __attribute__((always_inline)) {
+    constexpr bool PLACE = decltype(placec)::value;
+    uint64_t left = __ballot(is);
+    while (left) {  // (every turn takes at least one token out)
+      const int leader = __builtin_ctzll(left);
+      const int r = __builtin_amdgcn_readlane(row, leader);
+      const uint64_t same = __ballot(row == r) & left;
+      const uint32_t to = mine[r];
+      if constexpr (PLACE)
+        if ((same >> lane) & 1) a.order[to + __popcll(same & ((1ull << lane) - 1))] = token;
+      if (lane == leader) mine[r] = to + __popcll(same);
+      left &= ~same;
+    }
+  };
+  auto from_list = [&](auto placec) __attribute__((always_inline)) {
+    for (uint32_t i = 0; i < listed; i += 64) {
+      const bool is = i + lane < listed;
+      const uint2 e = is ? list[i + lane] : make_uint2(0, 0);
+      take(placec, e.x, (int)e.y, is);
+    }
+  };
+  auto from_ids = [&](auto placec) __attribute__((always_inline)) {
+    batches_of([&](uint32_t token, uint32_t id, bool valid) __attribute__((always_inline)) {
+      take(placec, token, (int)(id >> shift), valid && (int)(id & mask) == g);
+    });
+  };
+  batches_of([&](uint32_t token, uint32_t id, bool valid) __attribute__((always_inline)) {
+    const int group = (int)(id & mask);
+    lower += (uint32_t)__popcll(__ballot(valid && group < g));
+    const bool is = valid && group == g;
+    const uint64_t here = __ballot(is);
+    if (here) {
+      const uint32_t to = listed + __popcll(here & ((1ull << lane) - 1));
+      if (is && to < LIST) list[to] = make_uint2(token, id >> shift);
+      listed += (uint32_t)__popcll(here);
+    }
+  });
+  const bool fits = listed <= LIST;
+  if (fits) from_list(std::false_type());
+  else from_ids(std::false_type());
   if (lane == 0) atomicAdd(&before, lower);
   __syncthreads();
   // Row r is thread r's: its tokens behind those of the rows before it, a wavefront's behind those of the wavefronts before.
@@ -139,7 +171,8 @@ __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const
     }
   }
   __syncthreads();
-  scan(std::true_type());
+  if (fits) from_list(std::true_type());
+  else from_ids(std::true_type());
 }
 
 // ---- sums
@@ -158,17 +191,17 @@ struct SumArgs {
 // there -- the last one of a row and the first of the next.
 __device__ __forceinline__ int64_t slot(uint32_t p, bool first) { return (int64_t)(p / kRun) * 2 + first; }
 
-// acc += the rows of dy that `order` lists from p on, n <= 64 of them, in that order.
-template <typename TY, int V>
-__device__ __forceinline__ void add_run(const SumArgs& a, uint32_t p, int n, int slice, int lane, float* acc) {
-  constexpr int NC = 8 / V, U = 8;
-  const int col = slice * kSlice + lane * V;
-  const int mine = lane < n ? (int)a.order[p + lane] : 0;
+// A slice is S times 512 columns: of a lane S times eight, in pieces of V that lie 64 V apart.
+// acc += the rows of dy of the n tokens that lanes from.. from + n - 1 hold in `token`, in that order.
+template <typename TY, int V, int S>
+__device__ __forceinline__ void add_rows(const SumArgs& a, int token, int from, int n, int slice, int lane, float* acc) {
+  constexpr int NC = 8 * S / V, U = 8 / S;
+  const int col = slice * (kSlice * S) + lane * V;
   for (int j = 0; j < n; j += U) {
     Piece<TY, V> q[U][NC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t t = (uint32_t)__builtin_amdgcn_readlane(mine, j + u < n ? j + u : n - 1);
+      const int64_t t = (uint32_t)__builtin_amdgcn_readlane(token, from + (j + u < n ? j + u : n - 1));
       const TY* dy = (const TY*)a.dy + t * a.lddy + col;
 #pragma unroll
       for (int c = 0; c < NC; ++c) q[u][c].load(dy + c * 64 * V, j + u < n && col + c * 64 * V < a.width);
@@ -182,18 +215,23 @@ __device__ __forceinline__ void add_run(const SumArgs& a, uint32_t p, int n, int
           for (int e = 0; e < V; ++e) acc[c * V + e] += q[u][c].get(e);
   }
 }
-template <typename T, int V>
+// ... of the n <= 64 that `order` lists from p on.
+template <typename TY, int V, int S>
+__device__ __forceinline__ void add_run(const SumArgs& a, uint32_t p, int n, int slice, int lane, float* acc) {
+  add_rows<TY, V, S>(a, lane < n ? (int)a.order[p + lane] : 0, 0, n, slice, lane, acc);
+}
+template <typename T, int V, int S>
 __device__ __forceinline__ void put_slice(T* row, int slice, int lane, int width, const float* v) {
 #pragma unroll
-  for (int c = 0; c < 8 / V; ++c) {
-    const int col = slice * kSlice + c * 64 * V + lane * V;
+  for (int c = 0; c < 8 * S / V; ++c) {
+    const int col = slice * (kSlice * S) + c * 64 * V + lane * V;
     if (col < width) Piece<T, V>::store(row + col, v + c * V);
   }
 }
 
 constexpr int kUnits = 8;  // rows' slices of a wavefront, far apart: frequent tokens are neighbours in a table
 
-template <typename ID, typename TY, typename TW, int V>
+template <typename ID, typename TY, typename TW, int V, int S>
 __global__ __launch_bounds__(256) void embedding_sums_kernel(const SumArgs a, uint32_t run_wgs, uint32_t stride) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (blockIdx.x < run_wgs) {
@@ -213,49 +251,54 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(const SumArgs a, ui
       starts &= starts - 1;
       const uint32_t q = chunk * kRun + l, f = __builtin_amdgcn_readlane(first, l), m = __builtin_amdgcn_readlane(n, l);
       const uint32_t left = f + m - q;
-      float acc[8] = {};
-      add_run<TY, V>(a, q, left < kRun ? (int)left : kRun, slice, lane, acc);
-      put_slice<float, V>(a.partial + slot(q, q == f) * a.width, slice, lane, a.width, acc);
+      float acc[8 * S] = {};
+      add_run<TY, V, S>(a, q, left < kRun ? (int)left : kRun, slice, lane, acc);
+      put_slice<float, V, S>(a.partial + slot(q, q == f) * a.width, slice, lane, a.width, acc);
     }
     return;
   }
   const uint32_t w0 = (blockIdx.x - run_wgs) * 4 + wave, units = (uint32_t)a.vocab * a.slices;
-  // first and length of this wavefront's rows, one a lane
-  uint32_t first = 0, n = 0;
+  // Lanes 8 k .. 8 k + 7 have the k-th of this wavefront's rows: where its tokens start, how many, and the first eight of them.
+  static_assert(kUnits == 8, "eight lanes a row");
+  uint32_t first = 0, n = 0, token = 0;
   {
-    const uint32_t unit = w0 + lane * stride;
-    if (lane < kUnits && unit < units) {
+    const uint32_t unit = w0 + (lane >> 3) * stride;
+    if (unit < units) {
       first = a.first[unit / a.slices];
       n = a.count[unit / a.slices];
     }
+    if ((uint32_t)(lane & 7) < n) token = a.order[first + (lane & 7)];
   }
   for (int k = 0; k < kUnits; ++k) {
     const uint32_t unit = w0 + k * stride;
     if (unit >= units) break;
     const uint32_t row = unit / a.slices;
     const int slice = (int)(unit - row * a.slices);
-    const uint32_t f = __builtin_amdgcn_readlane(first, k), m = __builtin_amdgcn_readlane(n, k);
+    const uint32_t f = __builtin_amdgcn_readlane(first, 8 * k), m = __builtin_amdgcn_readlane(n, 8 * k);
     if (m > kRun) continue;
-    float acc[8] = {};
+    float acc[8 * S] = {};
     if (m > 0) {
-      add_run<TY, V>(a, f, (int)m, slice, lane, acc);
+      add_rows<TY, V, S>(a, (int)token, 8 * k, m < 8 ? (int)m : 8, slice, lane, acc);
+      if (m > 8) add_run<TY, V, S>(a, f + 8, (int)m - 8, slice, lane, acc);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= a.scale;
+      for (int e = 0; e < 8 * S; ++e) acc[e] *= a.scale;
     }
-    put_slice<TW, V>((TW*)a.dw + (int64_t)row * a.width, slice, lane, a.width, acc);
+    put_slice<TW, V, S>((TW*)a.dw + (int64_t)row * a.width, slice, lane, a.width, acc);
   }
 }
 
 // ---- join
-// The long rows of a workgroup of the index, a slice of their columns: four wavefronts add a quarter of the partial sums each.
+// The long rows of a workgroup of the index, 512 of their columns: eight wavefronts add an eighth of the partial sums each.
+constexpr int kJoinWaves = 8;
+
 template <typename TW, int V>
-__global__ __launch_bounds__(256) void embedding_join_kernel(const SumArgs a, int rows) {
-  __shared__ float quarter[3][kSlice];
+__global__ __launch_bounds__(kJoinWaves * 64) void embedding_join_kernel(const SumArgs a, int rows) {
+  __shared__ float others[kJoinWaves - 1][kSlice];
   __shared__ int longs[kIndexRows], n_long;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slice = blockIdx.y;
   if (threadIdx.x == 0) n_long = 0;
   __syncthreads();
-  for (int r = threadIdx.x; r < rows; r += 256) {
+  for (int r = threadIdx.x; r < rows; r += kJoinWaves * 64) {
     const int64_t v = (int64_t)r * a.groups + blockIdx.x;
     if (v < a.vocab && a.count[v] > kRun) longs[atomicAdd(&n_long, 1)] = (int)v;  // (in any order: each is a row of its own)
   }
@@ -264,11 +307,11 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const SumArgs a, in
   for (int i = 0; i < rows_here; ++i) {
     const int64_t v = longs[i];
     const uint32_t first = a.first[v], runs = (a.count[v] + kRun - 1) / kRun;
-    const uint32_t k0 = (uint32_t)((uint64_t)runs * wave / 4), k1 = (uint32_t)((uint64_t)runs * (wave + 1) / 4);
+    const uint32_t k0 = (uint32_t)((uint64_t)runs * wave / kJoinWaves), k1 = (uint32_t)((uint64_t)runs * (wave + 1) / kJoinWaves);
     constexpr int NC = 8 / V;
     const int col = slice * kSlice + lane * V;
     float acc[8] = {};
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t k = k0; k < k1; ++k) {
       const float* q = a.partial + slot(first + k * kRun, k == 0) * a.width + col;
 #pragma unroll
@@ -281,13 +324,16 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(const SumArgs a, in
     }
     if (wave > 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) quarter[wave - 1][e * 64 + lane] = acc[e];
+      for (int e = 0; e < 8; ++e) others[wave - 1][e * 64 + lane] = acc[e];
     __syncthreads();
     if (wave == 0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        acc[e] = (acc[e] + quarter[0][e * 64 + lane] + quarter[1][e * 64 + lane] + quarter[2][e * 64 + lane]) * a.scale;
-      put_slice<TW, V>((TW*)a.dw + v * a.width, slice, lane, a.width, acc);
+      for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int w = 0; w < kJoinWaves - 1; ++w) acc[e] += others[w][e * 64 + lane];
+        acc[e] *= a.scale;
+      }
+      put_slice<TW, V, 1>((TW*)a.dw + v * a.width, slice, lane, a.width, acc);
     }
     __syncthreads();
   }
@@ -380,26 +426,30 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
   p.vocab = a.vocab;
   p.width = a.width;
   p.groups = ix.groups;
-  p.slices = (a.width + kSlice - 1) / kSlice;
+  const bool whole = a.width % 8 == 0 && embedding_fits(a.dy, a.lddy, a.y_dtype, 8) && embedding_fits(a.dw, a.width, a.w_dtype, 8);
+  const int wide = whole && a.width >= 2 * kSlice ? 2 : 1;  // slices of 1024 columns: half as many ways to memory, one after the other
+  p.slices = (a.width + wide * kSlice - 1) / (wide * kSlice);
   p.scale = a.scale;
   const bool longs = a.tokens > kRun;
   const int64_t units = (int64_t)a.vocab * p.slices, run_units = longs ? ((int64_t)a.tokens + kRun - 1) / kRun * p.slices : 0;
   const int64_t run_wgs = (run_units + 3) / 4, row_wgs = (units + 4 * kUnits - 1) / (4 * kUnits);
-  if (units > kMostUnits || run_units > kMostUnits || p.slices > 65535) return hipErrorInvalidValue;
-  auto go = [&](auto* id, auto* ty, auto* tw, auto vc) {
+  if (units > kMostUnits || run_units > kMostUnits || (a.width + kSlice - 1) / kSlice > 65535) return hipErrorInvalidValue;
+  auto go = [&](auto* id, auto* ty, auto* tw, auto vc, auto sc) {
     typedef std::remove_pointer_t<decltype(id)> ID;
     typedef std::remove_pointer_t<decltype(ty)> TY;
     typedef std::remove_pointer_t<decltype(tw)> TW;
     constexpr int V = decltype(vc)::value;
-    hipLaunchKernelGGL((embedding_sums_kernel<ID, TY, TW, V>), dim3((unsigned)(run_wgs + row_wgs)), dim3(256), 0, st, p,
+    hipLaunchKernelGGL((embedding_sums_kernel<ID, TY, TW, V, decltype(sc)::value>), dim3((unsigned)(run_wgs + row_wgs)), dim3(256), 0, st, p,
                        (uint32_t)run_wgs, (uint32_t)(row_wgs * 4));
     if (longs)
-      hipLaunchKernelGGL((embedding_join_kernel<TW, V>), dim3(ix.groups, p.slices), dim3(256), 0, st, p, rows);
+      hipLaunchKernelGGL((embedding_join_kernel<TW, V>), dim3(ix.groups, (a.width + kSlice - 1) / kSlice), dim3(kJoinWaves * 64), 0, st,
+                         p, rows);
   };
   auto sized = [&](auto* id, auto* ty, auto* tw) {
-    if (a.width % 8 == 0 && embedding_fits(a.dy, a.lddy, a.y_dtype, 8) && embedding_fits(a.dw, a.width, a.w_dtype, 8))
-      go(id, ty, tw, std::integral_constant<int, 8>());
-    else go(id, ty, tw, std::integral_constant<int, 1>());
+    typedef std::integral_constant<int, 1> one;
+    if (wide == 2) go(id, ty, tw, std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
+    else if (whole) go(id, ty, tw, std::integral_constant<int, 8>(), one());
+    else go(id, ty, tw, one(), one());
   };
   auto typed = [&](auto* id) {
     if (a.y_dtype) a.w_dtype ? sized(id, (float*)nullptr, (float*)nullptr) : sized(id, (float*)nullptr, (bf16_t*)nullptr);

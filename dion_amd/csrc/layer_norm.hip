@@ -47,25 +47,25 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const N
   constexpr int NC = E / V, ROWS = (G < 256 ? 256 : G) / G;
   __shared__ float sums[2][G / 64 + 1];
   const int t = threadIdx.x % G;
-  const int row = blockIdx.x * ROWS + threadIdx.x / G;
+  const int row = blockIdx.x * ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / (G / 64);
   if (row >= a.rows) return;  // (whole wavefronts; of a workgroup of one row none)
   const TX* x = (const TX*)a.x + (int64_t)row * a.ldx;
   Piece<TX, V> px[NC];
 #pragma unroll
   for (int c = 0; c < NC; ++c) px[c].load(x + (c * G + t) * V, (c * G + t) * V < a.width);
-  float v[E], s = 0.f;
+  float s = 0.f;  // (E values of x stay as they were read: sixteen bits each, where x is bf16)
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
-    for (int e = 0; e < V; ++e) s += v[c * V + e] = px[c].get(e);
+    for (int e = 0; e < V; ++e) s += px[c].get(e);
   const float n = 1.f / (float)a.width, mean = row_sum<G>(s, sums[0]) * n;
   s = 0.f;
 #pragma unroll
   for (int c = 0; c < NC; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      v[c * V + e] = (c * G + t) * V < a.width ? v[c * V + e] - mean : 0.f;
-      s += v[c * V + e] * v[c * V + e];
+      const float d = px[c].get(e) - mean;
+      s = (c * G + t) * V < a.width ? fmaf(d, d, s) : s;
     }
   const float rstd = 1.f / sqrtf(row_sum<G>(s, sums[1]) * n + a.eps);
   if (t == 0 && a.mean) {
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const N
     param<V>(a.w, a.w_dtype, col, true, 1.f, w);
     param<V>(a.b, a.b_dtype, col, true, 0.f, b);
 #pragma unroll
-    for (int e = 0; e < V; ++e) w[e] = fmaf(v[c * V + e] * rstd, w[e], b[e]);
+    for (int e = 0; e < V; ++e) w[e] = fmaf((px[c].get(e) - mean) * rstd, w[e], b[e]);
     Piece<TY, V>::store(y + col, w);
   }
 }
@@ -121,51 +121,52 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   constexpr int NC = E / V, ROWS = 1024 / G;
   __shared__ float sums[2][16][2];
   __shared__ float half[ROWS > 1 ? ROWS / 2 * G * E : 1];
-  const int t = threadIdx.x % G, group = threadIdx.x / G, wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / (G / 64), t = threadIdx.x % G;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t first = (int64_t)blockIdx.x * ROWS;
   const float n = 1.f / (float)a.width;
+  // Rows on their way: two of eight elements a thread in one access; one in more; none of sixteen elements.
+  constexpr int AHEAD = E > 8 ? 0 : V < 8 ? 1 : 2, SETS = AHEAD > 0 ? AHEAD : 1;
   float w[E], dw[E] = {}, db[E] = {};
 #pragma unroll
   for (int c = 0; c < NC; ++c) param<V>(a.w, a.w_dtype, (c * G + t) * V, (c * G + t) * V < a.width, 1.f, w + c * V);
-  Piece<TX, V> px[NC];
-  Piece<TY, V> pd[NC];
-  float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](int64_t row) __attribute__((always_inline)) {  // (zeros behind the last row and the last column: they add nothing)
+  struct Row {
+    Piece<TX, V> px[NC];
+    Piece<TY, V> pd[NC];
+    float mean, rstd;
+  } sets[SETS];
+  auto fetch = [&](Row& q, int64_t row) __attribute__((always_inline)) {  // (zeros behind the last row and the last column: they add nothing)
     const bool in = row < a.rows;
     const TX* x = (const TX*)a.x + row * a.ldx;
     const TY* dy = (const TY*)a.dy + row * a.lddy;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = (c * G + t) * V;
-      px[c].load(x + col, in && col < a.width);
-      pd[c].load(dy + col, in && col < a.width);
+      q.px[c].load(x + col, in && col < a.width);
+      q.pd[c].load(dy + col, in && col < a.width);
     }
-    mean = in ? a.mean[row] : 0.f;
-    rstd = in ? a.rstd[row] : 0.f;
+    q.mean = in ? a.mean[row] : 0.f;
+    q.rstd = in ? a.rstd[row] : 0.f;
   };
-  constexpr bool AHEAD = E == 8;  // (sixteen elements a thread leave no registers for the next ones)
-  if constexpr (AHEAD) fetch(first + group);
-  for (int buf = 0; first < a.rows; first += step, buf ^= 1) {  // (the same for the whole workgroup)
-    const int64_t row = first + group;
-    if constexpr (!AHEAD) fetch(row);
+  auto one = [&](Row& q, int64_t row, int buf) __attribute__((always_inline)) {
+    if constexpr (AHEAD == 0) fetch(q, row);
     float xh[E], g[E], s0 = 0.f, s1 = 0.f;
-    const float r = rstd;
+    const float r = q.rstd, mean = q.mean;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const int i = c * V + e;
-        xh[i] = (c * G + t) * V < a.width ? (px[c].get(e) - mean) * r : 0.f;
-        const float d = pd[c].get(e);
+        xh[i] = (c * G + t) * V < a.width ? (q.px[c].get(e) - mean) * r : 0.f;
+        const float d = q.pd[c].get(e);
         dw[i] = fmaf(d, xh[i], dw[i]);
         db[i] += d;
         g[i] = d * w[i];
         s0 += g[i];
         s1 = fmaf(g[i], xh[i], s1);
       }
-    if constexpr (AHEAD) fetch(row + step);
-    if (!a.dx) continue;
+    if constexpr (AHEAD > 0) fetch(q, row + AHEAD * step);
+    if (!a.dx) return;
     s0 = wave_sum(s0);
     s1 = wave_sum(s1);
     if constexpr (G > 64) {
@@ -194,6 +195,17 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
         for (int e = 0; e < V; ++e) o[e] = r * (g[c * V + e] - s0 - xh[c * V + e] * s1);
         Piece<TX, V>::store(dx + col, o);
       }
+    }
+  };
+  if constexpr (AHEAD > 0)
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) fetch(sets[k], first + group + k * step);
+  for (int buf = 0; first < a.rows;) {  // (the same for the whole workgroup; rows behind the last one are zeros)
+#pragma unroll
+    for (int k = 0; k < SETS; ++k) {
+      one(sets[k], first + group, buf);
+      first += step;
+      buf ^= 1;
     }
   }
   if (!a.partial) return;
@@ -347,6 +359,7 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
     auto sized = [&](auto vc) {
       if (a.width <= 512) run(std::integral_constant<int, 64>(), std::integral_constant<int, 8>(), vc);
       else if (a.width <= 2048) run(std::integral_constant<int, 64>(), std::integral_constant<int, 32>(), vc);
+      else if (a.width <= 4096) run(std::integral_constant<int, 64>(), std::integral_constant<int, 64>(), vc);
       else if (a.width <= 8192) run(std::integral_constant<int, 256>(), std::integral_constant<int, 32>(), vc);
       else run(std::integral_constant<int, 1024>(), std::integral_constant<int, 32>(), vc);
     };

@@ -6,10 +6,9 @@ from typing import Optional
 import torch
 from torch import Tensor
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from . import ops
-from .linear import _check_capture, _refuse_tangents
+from .linear import _check_capture, _once, _refuse_tangents
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -21,11 +20,12 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.layer_norm_backward(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
+        grads = ops.layer_norm_grads if type(dy) is Tensor else ops.layer_norm_backward
+        return (*grads(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -56,9 +56,10 @@ class _Embedding(torch.autograd.Function):
         return ops.embedding_forward(ids, weight, scale, dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        return None, ops.embedding_backward(dy, ctx.saved_tensors[0], *ctx.table), None, None, None
+        grad = ops.embedding_grad if type(dy) is Tensor else ops.embedding_backward
+        return None, grad(dy, ctx.saved_tensors[0], *ctx.table), None, None, None
 
 
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,

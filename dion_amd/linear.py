@@ -109,6 +109,12 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     return ops.linear_forward(x, weight, bias, activation, residual, False)[0]
 
 
+def _once(backward):
+    """``once_differentiable`` where the pass is recorded for another derivative; otherwise the function itself, which then costs less."""
+    recorded = once_differentiable(backward)
+    return lambda ctx, dy: (recorded if torch.is_grad_enabled() else backward)(ctx, dy)
+
+
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight_gate, weight_up, bias_gate, bias_up, activation):
@@ -122,10 +128,12 @@ class _GatedLinear(torch.autograd.Function):
         return h
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
         need = ctx.needs_input_grad
-        return (*ops.gated_backward(dh, ctx.saved_tensors[3], ctx.keep, *ctx.saved_tensors[:3], *need[:3], *ctx.bias_dtypes), None)
+        x, weight_gate, weight_up, kept = ctx.saved_tensors
+        grads = ops.gated_grads if type(dh) is Tensor else ops.gated_backward
+        return (*grads(dh, kept, ctx.keep, x, weight_gate, weight_up, *need[:3], *ctx.bias_dtypes), None)
 
 
 def gated_linear(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: Optional[Tensor] = None,

@@ -1312,9 +1312,8 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
     ``dWu``, and may be None without.  Both asked for, they are the two ends of one allocation."""
     op = "gated_linear"
     index = _check_gated_weights(op, dh, "dh", weight_gate, weight_up, 0)
-    fan_out, fan_in = weight_gate.shape
-    lead, need_dw = dh.shape[:-1], need_dgate or need_dup
-    if need_dw:
+    (fan_out, fan_in), lead = weight_gate.shape, dh.shape[:-1]
+    if need_dgate or need_dup:
         if x is None:
             raise ValueError(f"{op}: the gradients of the weights need x")
         _check_operand(op, "x", x, lead + (fan_in,), index)
@@ -1324,6 +1323,13 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
     for t in (bias_gate_dtype, bias_up_dtype):
         if t is not None and t not in _FLOATS:
             raise TypeError(f"{op}: a bias must be torch.bfloat16 or torch.float32, got {t}")
+    return gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, need_dup, bias_gate_dtype, bias_up_dtype)
+
+
+def gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, need_dup, bias_gate_dtype, bias_up_dtype):
+    """``gated_backward`` of what the forward pass kept, whose operands it has checked, and a gradient that autograd has."""
+    fan_out, fan_in = weight_gate.shape
+    lead, need_dw = dh.shape[:-1], need_dgate or need_dup
     with _device_of(dh):
         dh, pdh, lddh, _ = _rows(dh)
         x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
@@ -1345,7 +1351,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         dbu = dh.new_empty((fan_out,), dtype=bias_up_dtype) if bias_up_dtype is not None else None
         check(_lib.load().dion_gated_backward(pdh, lddh, kept.data_ptr(), keep, px, ldx, pg, ldg, pu, ldu, _ptr(dx),
                                               _ptr(dgate), _ptr(dup), _ptr(dbg), _code(dbg), _ptr(dbu), _code(dbu), tokens, fan_in,
-                                              fan_out, _ptr(ws), nbytes, _stream_handle(dh.device)), f"{op} backward")
+                                              fan_out, _ptr(ws), nbytes, _stream_handle(dh.device)), "gated_linear backward")
     return (_viewed(dx, lead, fan_in) if need_dx else None), dgate, dup, dbg, dbu
 
 
@@ -1390,26 +1396,37 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: 
     op = "layer_norm"
     index = _check_norm(x, weight, None)
     _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
-    lead, width = x.shape[:-1], x.shape[-1]
-    rows = lead.numel()
+    rows = x.shape[:-1].numel()
     if stats.get_device() != index or stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
     if need_dw and weight is None:
         raise ValueError(f"{op}: the gradient of the weight needs the weight")
     if bias_dtype is not None and bias_dtype not in _FLOATS:
         raise TypeError(f"{op}: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
+    return layer_norm_grads(dy, x, weight, stats, need_dx, need_dw, bias_dtype)
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_bytes(rows: int, width: int) -> int:
+    return _lib.load().dion_layer_norm_workspace_bytes(rows, width)
+
+
+def layer_norm_grads(dy, x, weight, stats, need_dx, need_dw, bias_dtype):
+    """``layer_norm_backward`` of what the forward pass kept, whose operands it has checked, and a gradient that autograd has."""
+    lead, width = x.shape[:-1], x.shape[-1]
     with _device_of(x):
         dy, pdy, lddy, _ = _rows(dy)
         x, px, ldx, _ = _rows(x)
+        rows = x.shape[0]
         w = None if weight is None else weight.contiguous()
         dx = x.new_empty((rows, width)) if need_dx else None
         dw = w.new_empty((width,)) if need_dw else None
         db = x.new_empty((width,), dtype=bias_dtype) if bias_dtype is not None else None
-        nbytes = _lib.load().dion_layer_norm_workspace_bytes(rows, width) if need_dw or db is not None else 0
+        nbytes = _norm_bytes(rows, width) if need_dw or db is not None else 0
         ws, at = _space(nbytes, x.device), stats.data_ptr()
         check(_lib.load().dion_layer_norm_backward(pdy, lddy, _code(dy), px, ldx, _code(x), _ptr(w), _code(w), at, at + 4 * rows,
                                                    _ptr(dx), _ptr(dw), _ptr(db), _code(db), rows, width, _ptr(ws), nbytes,
-                                                   _stream_handle(x.device)), f"{op} backward")
+                                                   _stream_handle(x.device)), "layer_norm backward")
     return (_viewed(dx, lead, width) if need_dx else None), dw, db
 
 
@@ -1450,13 +1467,24 @@ def embedding_backward(dy: Tensor, ids: Tensor, vocab: int, scale: float, paddin
     _check_operand(op, "dy", dy, ids.shape + (width,), index, _FLOATS)
     if dtype not in _FLOATS:
         raise TypeError(f"{op}: the gradient must be torch.bfloat16 or torch.float32, got {dtype}")
+    return embedding_grad(dy, ids, vocab, scale, padding_idx, dtype)
+
+
+@functools.lru_cache(maxsize=4096)
+def _embedding_bytes(tokens: int, vocab: int, width: int) -> int:
+    return _lib.load().dion_embedding_workspace_bytes(tokens, vocab, width)
+
+
+def embedding_grad(dy, ids, vocab, scale, padding_idx, dtype):
+    """``embedding_backward`` of ids that the forward pass has checked and a gradient that autograd has."""
+    width = dy.shape[-1]
     with _device_of(dy):
         dy, pdy, lddy, _ = _rows(dy)
         t = ids.contiguous()
         dw = dy.new_empty((vocab, width), dtype=dtype)
-        nbytes = _lib.load().dion_embedding_workspace_bytes(t.numel(), vocab, width)
+        nbytes = _embedding_bytes(t.numel(), vocab, width)
         ws = _space(nbytes, dy.device)
         check(_lib.load().dion_embedding_backward(t.data_ptr(), 64 if t.dtype == torch.int64 else 32, t.numel(), pdy, lddy, _code(dy),
                                                   vocab, width, scale, -1 if padding_idx is None else padding_idx, dw.data_ptr(),
-                                                  _code(dw), _ptr(ws), nbytes, _stream_handle(dy.device)), f"{op} backward")
+                                                  _code(dw), _ptr(ws), nbytes, _stream_handle(dy.device)), "embedding backward")
     return dw
