@@ -2250,13 +2250,10 @@ extern "C" int dion_gated_backward(const void* dh, int64_t ld_dh, const void* ke
   char* ws = (char*)workspace;
   if (!dx && !dw && !db_gate && !db_up) return DION_OK;
   bf16_t* dz = (bf16_t*)(ws + s.dz);
-  const int parts = lin_sum_parts(tokens);
-  float *sums_gate = (float*)(ws + s.sums), *sums_up = sums_gate + (size_t)parts * fan_out;
-  const bool sums = db_gate || db_up;
-  HIP_TRY(launch_gated_dz((const bf16_t*)dh, ld_dh, kept, kept_bits == 32, tokens, fan_out, dx || dw ? dz : nullptr,
-                          sums ? sums_gate : nullptr, sums ? sums_up : nullptr, st), who);
-  if (db_gate) HIP_TRY(launch_lin_sum(sums_gate, parts, fan_out, db_gate, dt(db_gate_dtype), st), who);
-  if (db_up) HIP_TRY(launch_lin_sum(sums_up, parts, fan_out, db_up, dt(db_up_dtype), st), who);
+  float* const sums = db_gate || db_up ? (float*)(ws + s.sums) : nullptr;
+  HIP_TRY(launch_gated_dz((const bf16_t*)dh, ld_dh, kept, kept_bits == 32, tokens, fan_out, dx || dw ? dz : nullptr, sums, st), who);
+  if (sums)
+    HIP_TRY(launch_lin_sum(sums, lin_sum_parts(tokens), fan_out, db_gate, dt(db_gate_dtype), st, db_up, dt(db_up_dtype)), who);
   HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_X, &x, &ldx, tokens, fan_in, ws + s.x, st), who);
   HIP_TRY(lin_copy(copies & DION_LINEAR_COPY_W, &w_gate, &ld_gate, fan_out, fan_in, ws + s.wg, st), who);
   HIP_TRY(lin_copy(copies & DION_GATED_COPY_UP, &w_up, &ld_up, fan_out, fan_in, ws + s.wu, st), who);

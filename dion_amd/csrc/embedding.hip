@@ -13,6 +13,7 @@ constexpr int kRun = 64;         // tokens of a partial sum
 constexpr int kSlice = 512;      // columns: eight a lane of a wavefront
 constexpr int kIndexRows = 512;  // rows of a workgroup of the index, at most
 constexpr int kIndexWaves = 16;
+constexpr int kIndexLds = 144 * 1024;
 
 static int index_groups(int vocab) {  // a power of two, so that a row's workgroup is its lower bits
   int g = 256;
@@ -22,7 +23,7 @@ static int index_groups(int vocab) {  // a power of two, so that a row's workgro
 
 // ---- y
 // A wavefront takes up to SLICES slices of 64 V columns of a token's row.
-template <typename TW, typename TY, int V>
+template <typename TW, typename TY, int V, bool PAST>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(const EmbeddingArgs a, uint32_t per_row, uint32_t units) {
   constexpr int SLICES = 4;
   const int lane = threadIdx.x & 63;
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const EmbeddingArgs
     float v[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = in ? a.scale * p[s].get(e) : __uint_as_float(0x7fc00000u);
-    Piece<TY, V>::store(y + c, v);
+    Piece<TY, V>::template store<PAST>(y + c, v);
   }
 }
 
@@ -62,11 +63,12 @@ struct IndexArgs {
 // there, 64 at a time, equal ones together; so the tokens of a row stay in order.  Where the list is full it reads the ids again
 // instead.  Bound by the instructions that look at an id that is another workgroup's (255 of 256).
 template <typename ID>
-__global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const IndexArgs a, int rows) {
-  constexpr int AHEAD = 16, LIST = 192;  // ids of a lane on their way; tokens in a wavefront's list
-  extern __shared__ uint32_t at[];  // [kIndexWaves][rows]: counts, then where a wavefront's next token of the row goes
+__global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const IndexArgs a, int rows, int capacity) {
+  constexpr int AHEAD = 16;  // ids of a lane on their way
+  // at [kIndexWaves][rows]: counts, then where a wavefront's next token of the row goes; behind it the lists [kIndexWaves][capacity]:
+  // the row, above it how far the token lies behind the wavefront's first one
+  extern __shared__ uint32_t at[];
   __shared__ uint32_t sums[kIndexWaves], before;
-  __shared__ uint2 lists[kIndexWaves][LIST];  // token, row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = blockIdx.x, mask = a.groups - 1, shift = __builtin_ctz(a.groups);
   for (int i = threadIdx.x; i < kIndexWaves * rows; i += kIndexWaves * 64) at[i] = 0;
@@ -75,7 +77,8 @@ __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const
   const int batches = (a.tokens + 63) / 64;
   const int b0 = (int)((int64_t)batches * wave / kIndexWaves), b1 = (int)((int64_t)batches * (wave + 1) / kIndexWaves);
   volatile uint32_t* const mine = at + wave * rows;  // (lanes read what others of the wavefront wrote)
-  uint2* const list = lists[wave];
+  uint32_t* const list = at + kIndexWaves * rows + wave * capacity;
+  const uint32_t token0 = (uint32_t)b0 * 64;
   uint32_t lower = 0, listed = 0;  // (both the wavefront's)
   // Every batch of 64 tokens of this wavefront: f(token of the lane, its row or -1, whether the row is this workgroup's).
   auto batches_of = [&](auto&& f) __attribute__((always_inline)) {
@@ -117,8 +120,8 @@ __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const
   auto from_list = [&](auto placec) __attribute__((always_inline)) {
     for (uint32_t i = 0; i < listed; i += 64) {
       const bool is = i + lane < listed;
-      const uint2 e = is ? list[i + lane] : make_uint2(0, 0);
-      take(placec, e.x, (int)e.y, is);
+      const uint32_t e = is ? list[i + lane] : 0;
+      take(placec, token0 + e / kIndexRows, (int)(e % kIndexRows), is);
     }
   };
   auto from_ids = [&](auto placec) __attribute__((always_inline)) {
@@ -133,11 +136,11 @@ __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const
     const uint64_t here = __ballot(is);
     if (here) {
       const uint32_t to = listed + __popcll(here & ((1ull << lane) - 1));
-      if (is && to < LIST) list[to] = make_uint2(token, id >> shift);
+      if (is && to < (uint32_t)capacity) list[to] = (token - token0) * kIndexRows + (id >> shift);
       listed += (uint32_t)__popcll(here);
     }
   });
-  const bool fits = listed <= LIST;
+  const bool fits = listed <= (uint32_t)capacity;
   if (fits) from_list(std::false_type());
   else from_ids(std::false_type());
   if (lane == 0) atomicAdd(&before, lower);
@@ -368,6 +371,7 @@ static bool embedding_fits(const void* p, int64_t ld, int dtype, int v) {  // wh
 }
 
 hipError_t launch_embedding_forward(const EmbeddingArgs& a, hipStream_t st) {
+  const bool past = (int64_t)a.tokens * a.width * (a.y_dtype ? 4 : 2) > kPast;
   if (a.tokens <= 0 || a.vocab <= 0 || a.width <= 0 || !a.ids || !a.w || !a.y) return hipErrorInvalidValue;
   hipError_t err = hipSuccess;
   auto go = [&](auto* tw, auto* ty, auto vc) {
@@ -379,7 +383,9 @@ hipError_t launch_embedding_forward(const EmbeddingArgs& a, hipStream_t st) {
       err = hipErrorInvalidValue;
       return;
     }
-    hipLaunchKernelGGL((embedding_rows_kernel<TW, TY, V>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, (uint32_t)per_row,
+    constexpr bool WIDE = V == 8;
+    auto kernel = WIDE && past ? embedding_rows_kernel<TW, TY, V, WIDE> : embedding_rows_kernel<TW, TY, V, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, (uint32_t)per_row,
                        (uint32_t)units);
   };
   auto sized = [&](auto* tw, auto* ty) {
@@ -409,10 +415,19 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
   ix.first = (uint32_t*)(space + s.first);
   ix.count = (uint32_t*)(space + s.count);
   const int rows = (a.vocab + ix.groups - 1) / ix.groups;
-  const size_t lds = (size_t)kIndexWaves * rows * 4;
-  if (a.ids64) hipLaunchKernelGGL((embedding_index_kernel<int64_t>), dim3(ix.groups), dim3(kIndexWaves * 64), lds, st, ix, rows);
-  else hipLaunchKernelGGL((embedding_index_kernel<int32_t>), dim3(ix.groups), dim3(kIndexWaves * 64), lds, st, ix, rows);
-  if (hipError_t e = hipGetLastError()) return e;
+  // Lists for all tokens of a wavefront's run, or what LDS has room for; none where a run is too long for an entry's bits.  65536 tokens, of
+  // which one is 6 %, 50304 rows: 61 us with lists of 192, which that one's workgroup fills and reads the ids again, 24 with these.
+  const int64_t run = ((int64_t)a.tokens + kIndexWaves * 64 - 1) / (kIndexWaves * 64) * 64, room = (kIndexLds / 4 - kIndexWaves * rows) / kIndexWaves;
+  const int capacity = run > (int64_t(1) << 32) / kIndexRows ? 0 : (int)(run < room ? run : room);
+  const size_t lds = ((size_t)rows + capacity) * kIndexWaves * 4;
+  auto index = [&](auto* id) {
+    typedef std::remove_pointer_t<decltype(id)> ID;
+    static std::atomic<uint64_t> attr_done{0};
+    if (hipError_t e = set_max_dynamic_lds_once((const void*)embedding_index_kernel<ID>, kIndexLds, attr_done)) return e;
+    hipLaunchKernelGGL((embedding_index_kernel<ID>), dim3(ix.groups), dim3(kIndexWaves * 64), lds, st, ix, rows, capacity);
+    return hipGetLastError();
+  };
+  if (hipError_t e = a.ids64 ? index((int64_t*)nullptr) : index((int32_t*)nullptr)) return e;
   SumArgs p;
   p.ids = a.ids;
   p.order = ix.order;

@@ -148,8 +148,8 @@ constexpr int kDzCols = 256;  // columns of a workgroup: 32 threads of eight, by
 // W: elements of dh that are read at once; 8: every row is whole chunks.
 template <bool WIDE, bool DST, bool SUM, int W>
 __global__ __launch_bounds__(256) void gated_dz_kernel(const bf16_t* __restrict__ dh, int64_t ld, const char* __restrict__ kept,
-                                                       int rows, int cols, bf16_t* __restrict__ dz, float* __restrict__ sums_gate,
-                                                       float* __restrict__ sums_up, int per) {
+                                                       int rows, int cols, bf16_t* __restrict__ dz, float* __restrict__ partial,
+                                                       int per) {
   __shared__ float sums[2][8][kDzCols];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c0 = blockIdx.x * kDzCols + tx * 8, padded = slope_pitch(cols);
@@ -227,8 +227,8 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const bf16_t* __restrict_
         g += sums[0][k][threadIdx.x];
         u += sums[1][k][threadIdx.x];
       }
-      sums_gate[(int64_t)blockIdx.y * cols + c] = g;
-      sums_up[(int64_t)blockIdx.y * cols + c] = u;
+      partial[(int64_t)blockIdx.y * 2 * cols + c] = g;
+      partial[((int64_t)blockIdx.y * 2 + 1) * cols + c] = u;
     }
   }
 }
@@ -236,8 +236,20 @@ __global__ __launch_bounds__(256) void gated_dz_kernel(const bf16_t* __restrict_
 // ---------------------------------------------------------------------------------------------- host
 size_t gated_kept_bytes(int M, int N, bool wide) { return (size_t)M * kept_pitch(N, wide); }
 
+// Up to 32 tokens: gated_few_kernel where it is estimated to take less than tiles, which pass the weights at 5.4 TB/s and then join the
+// parts of their reductions (8 us).  us, few / tiles, weights from HBM: 4096 x 14336, 1 token 44 / 52, 4 tokens 47 / 52, 16 tokens
+// 68 / 53; 2048 x 8192, 8 tokens 15.6 / 18.1, 24 tokens 39.6 / 19.4.
+static LinPlan gated_plan(int M, int N, int K) {
+  if (M <= 32) {
+    const double wgs = (N + 7) / 8, each = M <= 16 ? 0.74 + 0.03 * (M - 1) : 2.3;
+    const double few = 2.5 + each * (K / 512.0) * (wgs > 256 ? wgs / 256 : 1), tiles = 8.0 + 4.0 * N * K / 5.4e6;
+    if (few < tiles) return {kLinFew, 1, 0};
+  }
+  return lin_plan(M, 2 * N, K, 0, 0, false);
+}
+
 size_t gated_product_scratch(int M, int N, int K) {
-  const LinPlan plan = lin_plan(M, 2 * N, K, 0, 0);
+  const LinPlan plan = gated_plan(M, N, K);
   return plan.splits > 1 ? (size_t)plan.splits * M * N * 2 * sizeof(float) : 0;
 }
 
@@ -280,7 +292,7 @@ hipError_t launch_gated_product(const GatedProduct& p, hipStream_t st) {
   e.bias2 = p.bu;
   e.bias2_dtype = p.bu_dtype;
   e.wide = p.wide;
-  const LinPlan plan = lin_plan(p.M, 2 * p.N, p.K, 0, 0);
+  const LinPlan plan = gated_plan(p.M, p.N, p.K);
   if (plan.tile == kLinFew) {
     const dim3 grid((unsigned)((p.N + 7) / 8));
     auto go = [&](auto tbc, auto wavesc) {
@@ -319,16 +331,16 @@ hipError_t launch_gated_product(const GatedProduct& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool wide, int rows, int cols, bf16_t* dz, float* sums_gate,
-                           float* sums_up, hipStream_t st) {
-  if (rows <= 0 || cols <= 0 || !kept || (!dz && !sums_gate) || !sums_gate != !sums_up || ((uint64_t)dz & 15) || ((uint64_t)kept & 15))
+hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool wide, int rows, int cols, bf16_t* dz, float* sums,
+                           hipStream_t st) {
+  if (rows <= 0 || cols <= 0 || !kept || (!dz && !sums) || ((uint64_t)dz & 15) || ((uint64_t)kept & 15))
     return hipErrorInvalidValue;
   const int parts = lin_sum_parts(rows), per = (rows + 1023) / 1024 * 8;
   const dim3 grid((cols + kDzCols - 1) / kDzCols, parts);
   const uint64_t bytes = (uint64_t)dh | (uint64_t)cols * 2 | (uint64_t)ld * 2;
   auto go = [&](auto widec, auto dstc, auto sumc, auto wc) {
     hipLaunchKernelGGL((gated_dz_kernel<decltype(widec)::value, decltype(dstc)::value, decltype(sumc)::value, decltype(wc)::value>), grid, dim3(256), 0, st, dh,
-                       ld, (const char*)kept, rows, cols, dz, sums_gate, sums_up, per);
+                       ld, (const char*)kept, rows, cols, dz, sums, per);
   };
   auto sized = [&](auto widec, auto dstc, auto sumc) {
     if (bytes % 16 == 0) go(widec, dstc, sumc, std::integral_constant<int, 8>());
@@ -339,7 +351,7 @@ hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool 
     if (wide) sized(std::true_type(), dstc, sumc);
     else sized(std::false_type(), dstc, sumc);
   };
-  if (dz && sums_gate) with(std::true_type(), std::true_type());
+  if (dz && sums) with(std::true_type(), std::true_type());
   else if (dz) with(std::true_type(), std::false_type());
   else with(std::false_type(), std::true_type());
   return hipGetLastError();

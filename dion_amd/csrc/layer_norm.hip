@@ -3,6 +3,7 @@
 // Rows stay in registers between the two sums of a pass (the variance is that of the centred values: no difference of large
 // numbers), so x and dy are read once.  Sums fp32, in an order that depends on the sizes alone.
 #include "layers.h"
+#include "linear.h"
 
 namespace dion {
 
@@ -42,7 +43,7 @@ static __device__ __forceinline__ float row_sum(float v, float* at) {
 }
 
 // A row by G threads of E elements each: elements (c G + t) V .. + V - 1 are chunk c of thread t.
-template <typename TX, typename TY, int G, int E, int V>
+template <typename TX, typename TY, int G, int E, int V, bool PAST>
 __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const NormArgs a) {
   constexpr int NC = E / V, ROWS = (G < 256 ? 256 : G) / G;
   __shared__ float sums[2][G / 64 + 1];
@@ -82,7 +83,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const N
     param<V>(a.b, a.b_dtype, col, true, 0.f, b);
 #pragma unroll
     for (int e = 0; e < V; ++e) w[e] = fmaf((px[c].get(e) - mean) * rstd, w[e], b[e]);
-    Piece<TY, V>::store(y + col, w);
+    Piece<TY, V>::template store<PAST>(y + col, w);
   }
 }
 
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const NormArgs 
 
 // dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy: sixteen wavefronts take
 // 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them.
-template <typename TX, typename TY, int G, int E, int V>
+template <typename TX, typename TY, int G, int E, int V, bool PAST>
 __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   constexpr int NC = E / V, ROWS = 1024 / G;
   __shared__ float sums[2][16][2];
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
         float o[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) o[e] = r * (g[c * V + e] - s0 - xh[c * V + e] * s1);
-        Piece<TX, V>::store(dx + col, o);
+        Piece<TX, V>::template store<PAST>(dx + col, o);
       }
     }
   };
@@ -283,29 +284,6 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a, int
   out[a.width + c] = db;
 }
 
-// dw and db from the parts' sums: sixteen columns of a workgroup, sixteen threads a column.
-__global__ __launch_bounds__(256) void norm_join_kernel(const NormArgs a, int parts) {
-  __shared__ float sums[16][17];
-  const int tx = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
-  const bool in = c < 2 * a.width;
-  float s = 0.f;
-  if (in)
-#pragma unroll 4
-    for (int k = g; k < parts; k += 16) s += a.partial[(int64_t)k * 2 * a.width + c];
-  sums[g][tx] = s;
-  __syncthreads();
-  if (g == 0 && in) {
-    s = sums[0][tx];
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += sums[k][tx];
-    void* out = c < a.width ? a.dw : a.db;
-    const int at = c < a.width ? c : c - a.width, dtype = c < a.width ? a.w_dtype : a.b_dtype;
-    if (!out) return;
-    if (dtype) ((float*)out)[at] = s;
-    else ((bf16_t*)out)[at] = f32_to_bf16(s);
-  }
-}
-
 // ---------------------------------------------------------------------------------------------- host
 // Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows fill.
 static int norm_threads(int width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 2048 ? 256 : width <= 4096 ? 512 : 1024; }
@@ -345,6 +323,7 @@ static hipError_t norm_types(const NormArgs& a, F&& go) {
 
 hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
   if (a.rows <= 0 || a.width <= 0 || !a.x || !a.y || !a.mean != !a.rstd) return hipErrorInvalidValue;
+  const bool past = (int64_t)a.rows * a.width * (a.y_dtype ? 4 : 2) > kPast;
   return norm_types(a, [&](auto* tx, auto* ty) {
     typedef std::remove_pointer_t<decltype(tx)> TX;
     typedef std::remove_pointer_t<decltype(ty)> TY;
@@ -354,7 +333,9 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
     }
     auto run = [&](auto gc, auto ec, auto vc) {
       constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value, T = G < 256 ? 256 : G;
-      hipLaunchKernelGGL((norm_forward_kernel<TX, TY, G, E, V>), dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
+      constexpr bool WIDE = V >= 4;
+      auto kernel = WIDE && past ? norm_forward_kernel<TX, TY, G, E, V, WIDE> : norm_forward_kernel<TX, TY, G, E, V, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
     };
     auto sized = [&](auto vc) {
       if (a.width <= 512) run(std::integral_constant<int, 64>(), std::integral_constant<int, 8>(), vc);
@@ -375,6 +356,7 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
   if (a.rows <= 0 || a.width <= 0 || !a.x || !a.dy || !a.mean || !a.rstd || ((a.dw || a.db) && !a.partial)) return hipErrorInvalidValue;
   NormArgs p = a;
   p.b = nullptr;  // (not read)
+  const bool past = (int64_t)a.rows * a.width * (a.x_dtype ? 4 : 2) > kPast;
   if (!a.dw && !a.db) p.partial = nullptr;
   const int parts = norm_parts(a.rows, a.width);
   hipError_t e = norm_types(p, [&](auto* tx, auto* ty) {
@@ -389,7 +371,9 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
     }
     auto run = [&](auto gc, auto ec, auto vc) {
       constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value;
-      hipLaunchKernelGGL((norm_backward_kernel<TX, TY, G, E, V>), dim3(parts), dim3(1024), 0, st, p);
+      constexpr bool WIDE = V >= 4;
+      auto kernel = WIDE && past ? norm_backward_kernel<TX, TY, G, E, V, WIDE> : norm_backward_kernel<TX, TY, G, E, V, false>;
+      hipLaunchKernelGGL(kernel, dim3(parts), dim3(1024), 0, st, p);
     };
     auto sized = [&](auto vc) {
       typedef std::integral_constant<int, 8> eight;
@@ -407,8 +391,7 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
     else sized(std::integral_constant<int, 1>());
   });
   if (e != hipSuccess || !p.partial) return e;
-  hipLaunchKernelGGL(norm_join_kernel, dim3((2 * a.width + 15) / 16), dim3(256), 0, st, p, parts);
-  return hipGetLastError();
+  return launch_lin_sum(p.partial, parts, a.width, p.dw, p.w_dtype, st, p.db, p.b_dtype);
 }
 
 }  // namespace dion

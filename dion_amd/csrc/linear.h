@@ -34,7 +34,7 @@ struct LinPlan {
   LinTile tile;
   int splits, slabs;
 };
-LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor);
+LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor, bool may_be_few = true);
 
 size_t lin_product_scratch(int M, int N, int K, int p_kmajor, int q_kmajor);
 hipError_t launch_lin_product(const LinProduct& p, hipStream_t st);
@@ -45,6 +45,8 @@ int lin_sum_parts(int rows);
 hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slope, int act, int rows, int cols, bf16_t* dst,
                               float* partial, hipStream_t st);
 hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st);
+// ... of partial[parts][2][cols]: out from the first, out2 from the second; either may be null.
+hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st, void* out2, int out2_dtype);
 // C[M][N] = the sum of part[0 .. splits)[M][N], in that order, rounded once.
 hipError_t launch_lin_join(const float* part, int splits, int M, int N, bf16_t* C, hipStream_t st);
 
@@ -66,9 +68,9 @@ size_t gated_product_scratch(int M, int N, int K);
 hipError_t launch_gated_product(const GatedProduct& p, hipStream_t st);
 
 // dz[rows][2 * (cols rounded up to 8)]: the gradients at x Wg^T + bg and, behind them in a row, at x Wu^T + bu, zeros behind column
-// cols; sums_gate, sums_up[lin_sum_parts(rows)][cols]: sums over runs of rows, in fp32, before rounding.  dz or the sums may be null.
-hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool wide, int rows, int cols, bf16_t* dz, float* sums_gate,
-                           float* sums_up, hipStream_t st);
+// cols; sums[lin_sum_parts(rows)][2][cols]: their sums over runs of rows, in fp32, before rounding.  dz or sums may be null.
+hipError_t launch_gated_dz(const bf16_t* dh, int64_t ld, const void* kept, bool wide, int rows, int cols, bf16_t* dz, float* sums,
+                           hipStream_t st);
 
 // C[M][N] = P Q + P2 Q2, sums over K each: P, P2 [M][K], ldp elements between rows, Q, Q2 [K][N].
 struct PairProduct {

@@ -193,8 +193,9 @@ __global__ __launch_bounds__(256) void lin_prepare_kernel(const bf16_t* __restri
 }
 
 // out[c] = sum of partial[0 .. parts)[c]: 16 columns of a workgroup, sixteen threads a column.  3 us: a launch and eight loads in a row.
+// (out2: of partial[parts][2][cols] the first and the second; `cols` is then that of both.)
 __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ partial, int parts, int cols, void* out,
-                                                      int out_dtype) {
+                                                      int out_dtype, int split, void* out2, int out2_dtype) {
   __shared__ float sums[16][17];
   const int tx = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
   float s = 0.f;
@@ -207,8 +208,11 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
     s = sums[0][tx];
 #pragma unroll
     for (int k = 1; k < 16; ++k) s += sums[k][tx];
-    if (out_dtype) ((float*)out)[c] = s;
-    else ((bf16_t*)out)[c] = f32_to_bf16(s);
+    void* const to = c < split ? out : out2;
+    const int at = c < split ? c : c - split;
+    if (!to) return;
+    if (c < split ? out_dtype : out2_dtype) ((float*)to)[at] = s;
+    else ((bf16_t*)to)[at] = f32_to_bf16(s);
   }
 }
 
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(256) void lin_sum_kernel(const float* __restrict__ 
 // lin_few_kernel takes so long per 512 of the reduction, its tokens and a workgroup per CU.  Few / tiles at 1, 8, 16, 32 tokens of
 // a weight from HBM: 768 x 768 3.8, 4.1, 4.2, 5.2 / 7.1 to 7.7; 4096 x 4096 8.6, 10.0, 11.9, 16.4 / 11.8 to 12.7; 4096 x 14336
 // 23.5, 28.5, 34.8, 50.3 / 25.2 to 25.9; 50304 x 768 15.5, 20.0, 24.5, 57 / 20.4 to 21.7.
-LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
+LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor, bool may_be_few) {
   const int KT = (K + 63) / 64;
   LinPlan best{kLin128, 1, KT};
   double least = 1e30;
@@ -248,7 +252,7 @@ LinPlan lin_plan(int M, int N, int K, int p_kmajor, int q_kmajor) {
       }
     }
   }
-  if (M <= 32 && !p_kmajor && !q_kmajor) {
+  if (M <= 32 && !p_kmajor && !q_kmajor && may_be_few) {
     const double wgs = (N + 15) / 16, each = M <= 16 ? 0.77 + 0.033 * (M - 1) : 1.5;
     if (2.5 + each * (K / 512.0) * (wgs > 256 ? wgs / 256 : 1) < least) return {kLinFew, 1, 0};
   }
@@ -392,7 +396,12 @@ hipError_t launch_lin_prepare(const bf16_t* src, int64_t ld, const uint16_t* slo
 }
 
 hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st) {
-  hipLaunchKernelGGL(lin_sum_kernel, dim3((cols + 15) / 16), dim3(256), 0, st, partial, parts, cols, out, out_dtype);
+  hipLaunchKernelGGL(lin_sum_kernel, dim3((cols + 15) / 16), dim3(256), 0, st, partial, parts, cols, out, out_dtype, cols, nullptr, 0);
+  return hipGetLastError();
+}
+hipError_t launch_lin_sum(const float* partial, int parts, int cols, void* out, int out_dtype, hipStream_t st, void* out2, int out2_dtype) {
+  hipLaunchKernelGGL(lin_sum_kernel, dim3((2 * cols + 15) / 16), dim3(256), 0, st, partial, parts, 2 * cols, out, out_dtype, cols, out2,
+                     out2_dtype);
   return hipGetLastError();
 }
 
