@@ -19,35 +19,30 @@ static __device__ __forceinline__ void gated4_any(const GatedEpilogue& p, int ro
   if (row >= p.M || col >= p.N) return;
   g += bias4(p, col);
   u += bias4(p.bias2, p.bias2_dtype, p.N, col);
-  uint2 h;
-  Kept4 to_gate, to_up;
-  auto finish = [&](auto widec) __attribute__((always_inline)) {
-    constexpr bool WIDE = decltype(widec)::value;
-    switch (p.act) {
-      case kActRelu: gated4<kActRelu, true, WIDE>(g, u, h, to_gate, to_up); break;
-      case kActReluSquared: gated4<kActReluSquared, true, WIDE>(g, u, h, to_gate, to_up); break;
-      case kActGelu: gated4<kActGelu, true, WIDE>(g, u, h, to_gate, to_up); break;
-      case kActGeluTanh: gated4<kActGeluTanh, true, WIDE>(g, u, h, to_gate, to_up); break;
-      case kActSilu: gated4<kActSilu, true, WIDE>(g, u, h, to_gate, to_up); break;
-      default: gated4<kActNone, true, WIDE>(g, u, h, to_gate, to_up); break;
+  f32x4 h, s;  // h, act'(g) u; g becomes act(g)
+  switch (p.act) {
+    case kActRelu: gate4<kActRelu>(g, u, h, s); break;
+    case kActReluSquared: gate4<kActReluSquared>(g, u, h, s); break;
+    case kActGelu: gate4<kActGelu>(g, u, h, s); break;
+    case kActGeluTanh: gate4<kActGeluTanh>(g, u, h, s); break;
+    case kActSilu: gate4<kActSilu>(g, u, h, s); break;
+    default: gate4<kActNone>(g, u, h, s); break;
+  }
+  if (p.slope) {
+    char* k = (char*)p.slope + (int64_t)row * kept_pitch(p.N, p.wide) + (col >> 5) * kept_block(p.wide);
+    const int c = col & 31;
+    const Kept4 to_gate = p.wide ? kept4<true>(s) : kept4<false>(s), to_up = p.wide ? kept4<true>(g) : kept4<false>(g);
+    *(uint2*)(k + 2 * c) = to_gate.high;
+    *(uint2*)(k + 64 + 2 * c) = to_up.high;
+    if (p.wide) {
+      *(uint2*)(k + 128 + 2 * c) = to_gate.low;
+      *(uint2*)(k + 192 + 2 * c) = to_up.low;
+    } else {
+      *(uint32_t*)(k + 128 + c) = to_gate.low.x;
+      *(uint32_t*)(k + 160 + c) = to_up.low.x;
     }
-    if (p.slope) {
-      char* k = (char*)p.slope + (int64_t)row * kept_pitch(p.N, WIDE) + (col >> 5) * kept_block(WIDE);
-      const int c = col & 31;
-      *(uint2*)(k + 2 * c) = to_gate.high;
-      *(uint2*)(k + 64 + 2 * c) = to_up.high;
-      if constexpr (WIDE) {
-        *(uint2*)(k + 128 + 2 * c) = to_gate.low;
-        *(uint2*)(k + 192 + 2 * c) = to_up.low;
-      } else {
-        *(uint32_t*)(k + 128 + c) = to_gate.low.x;
-        *(uint32_t*)(k + 160 + c) = to_up.low.x;
-      }
-    }
-  };
-  if (p.wide) finish(std::true_type());
-  else finish(std::false_type());
-  store4(p, p.C + (int64_t)row * p.N + col, col, h);
+  }
+  store4(p, p.C + (int64_t)row * p.N + col, col, make_uint2(pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])));
 }
 
 // Adds the parts of a split reduction, in their order, and finishes: four elements per thread.
@@ -133,7 +128,7 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(const GatedEpilog
   for (int i = threadIdx.x; i < TB * 32; i += WAVES * 64) {
     const int b = i >> 5, l = i & 31;
     f32x4 g = sums[0][b][l], u = sums[0][b][l + 32];
-#pragma unroll
+#pragma unroll 5  // (all fifteen at once would not fit the registers)
     for (int k = 1; k < WAVES; ++k) {
       g += sums[k][b][l];
       u += sums[k][b][l + 32];

@@ -160,7 +160,7 @@ struct Kept4 {  // of four neighbours
   uint2 high, low;  // (low.x alone: eight bits each)
 };
 template <bool WIDE>
-static __device__ __forceinline__ Kept4 kept4(const float* v) {
+static __device__ __forceinline__ Kept4 kept4(f32x4 v) {
   uint32_t b[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -175,20 +175,27 @@ static __device__ __forceinline__ Kept4 kept4(const float* v) {
     return {high, make_uint2(__builtin_amdgcn_perm(b[1], b[0], 0x0c0c0501) | __builtin_amdgcn_perm(b[3], b[2], 0x05010c0c), 0)};
 }
 
-// Four elements of a row: h, and what is kept for the backward pass.  (Not from h: act(g) may be zero.)
-template <int ACT, bool KEEP, bool WIDE>
-static __device__ __forceinline__ void gated4(f32x4 g, f32x4 u, uint2& h, Kept4& to_gate, Kept4& to_up) {
-  float v[4], s[4], a[4];
+// Four elements of a row from their sums: h = act(g) u, s = act'(g) u, and act(g) in g.
+template <int ACT>
+static __device__ __forceinline__ void gate4(f32x4& g, f32x4 u, f32x4& h, f32x4& s) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    a[e] = activate<ACT>(g[e], s[e]);
-    v[e] = a[e] * u[e];
-    s[e] = (ACT == kActReluSquared ? 2.f * s[e] : s[e]) * u[e];
+    float slope;
+    const float a = activate<ACT>(g[e], slope);
+    h[e] = a * u[e];
+    s[e] = (ACT == kActReluSquared ? 2.f * slope : slope) * u[e];
+    g[e] = a;
   }
+}
+// ... as they are stored: h, and (KEEP) what is kept for the backward pass (not from h: act(g) may be zero).
+template <int ACT, bool KEEP, bool WIDE>
+static __device__ __forceinline__ void gated4(f32x4 g, f32x4 u, uint2& h, Kept4& to_gate, Kept4& to_up) {
+  f32x4 v, s;
+  gate4<ACT>(g, u, v, s);
   h = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
   if constexpr (KEEP) {
     to_gate = kept4<WIDE>(s);
-    to_up = kept4<WIDE>(a);
+    to_up = kept4<WIDE>(g);
   }
 }
 
