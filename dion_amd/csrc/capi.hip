@@ -2131,6 +2131,13 @@ static int check_gated(const char* who, int tokens, int fan_in, int fan_out) {
   return DION_OK;
 }
 static bool bad_dtype(int dtype) { return dtype != DION_BF16 && dtype != DION_F32; }
+// A tensor that may be null: its type, and an address of whole elements.
+static int check_vector(const char* who, const char* arg, const void* p, int dtype) {
+  if (!p) return DION_OK;
+  if (bad_dtype(dtype)) return fail(DION_E_INVALID, "%s: type of %s", who, arg);
+  if ((uintptr_t)p % (dtype == DION_F32 ? 4 : 2)) return fail(DION_E_INVALID, "%s: %s is not aligned to its elements", who, arg);
+  return DION_OK;
+}
 static int check_space(const char* who, const void* workspace, size_t have, size_t need) {
   if (need > 0 && (!workspace || have < need || !aligned16((uint64_t)(uintptr_t)workspace)))
     return fail(DION_E_WORKSPACE, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, need, have);
@@ -2169,14 +2176,14 @@ extern "C" int dion_gated_forward(const void* x, int64_t ldx, const void* w_gate
   const char* who = "dion_gated_forward";
   if (int rc = check_gated(who, tokens, fan_in, fan_out)) return rc;
   if (activation < 0 || activation >= kActCount) return fail(DION_E_INVALID, "%s: activation %d", who, activation);
-  if ((bias_gate && bad_dtype(bias_gate_dtype)) || (bias_up && bad_dtype(bias_up_dtype)))
-    return fail(DION_E_INVALID, "%s: type of a bias", who);
+  if (int rc = check_vector(who, "bias_gate", bias_gate, bias_gate_dtype)) return rc;
+  if (int rc = check_vector(who, "bias_up", bias_up, bias_up_dtype)) return rc;
   if (tokens == 0) return DION_OK;
   if (int rc = check_lin_rows(who, "x", x, ldx, tokens, fan_in)) return rc;
   if (int rc = check_lin_rows(who, "w_gate", w_gate, ld_gate, fan_out, fan_in)) return rc;
   if (int rc = check_lin_rows(who, "w_up", w_up, ld_up, fan_out, fan_in)) return rc;
   if (!h) return fail(DION_E_INVALID, "%s: h is null", who);
-  if ((uintptr_t)h & 1) return fail(DION_E_INVALID, "%s: h is not 2-byte aligned", who);
+  if (int rc = check_vector(who, "h", h, DION_BF16)) return rc;
   if (kept)
     if (int rc = check_kept(who, kept, kept_bits)) return rc;
   const int copies = (lin_whole(x, ldx, fan_in) ? 0 : DION_LINEAR_COPY_X) | (lin_whole(w_gate, ld_gate, fan_in) ? 0 : DION_LINEAR_COPY_W) |
@@ -2218,8 +2225,11 @@ extern "C" int dion_gated_backward(const void* dh, int64_t ld_dh, const void* ke
                                    int fan_out, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "dion_gated_backward";
   if (int rc = check_gated(who, tokens, fan_in, fan_out)) return rc;
-  if ((db_gate && bad_dtype(db_gate_dtype)) || (db_up && bad_dtype(db_up_dtype)))
-    return fail(DION_E_INVALID, "%s: type of a bias", who);
+  if (int rc = check_vector(who, "dx", dx, DION_BF16)) return rc;
+  if (int rc = check_vector(who, "dw_gate", dw_gate, DION_BF16)) return rc;
+  if (int rc = check_vector(who, "dw_up", dw_up, DION_BF16)) return rc;
+  if (int rc = check_vector(who, "db_gate", db_gate, db_gate_dtype)) return rc;
+  if (int rc = check_vector(who, "db_up", db_up, db_up_dtype)) return rc;
   hipStream_t st = (hipStream_t)stream;
   const int np = round8(fan_out);
   if (tokens == 0) {  // sums over nothing
@@ -2324,10 +2334,10 @@ extern "C" int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, 
   if (int rc = check_norm(who, rows, width)) return rc;
   if (int rc = check_rows(who, "x", x, ldx, x_dtype, rows, width)) return rc;
   if (int rc = check_rows(who, "y", y, width, y_dtype, rows, width)) return rc;
-  if (weight)
-    if (int rc = check_rows(who, "weight", weight, width, weight_dtype, 1, width)) return rc;
-  if (bias)
-    if (int rc = check_rows(who, "bias", bias, width, bias_dtype, 1, width)) return rc;
+  if (int rc = check_vector(who, "weight", weight, weight_dtype)) return rc;
+  if (int rc = check_vector(who, "bias", bias, bias_dtype)) return rc;
+  if (int rc = check_vector(who, "mean", mean, DION_F32)) return rc;
+  if (int rc = check_vector(who, "rstd", rstd, DION_F32)) return rc;
   if (!mean != !rstd) return fail(DION_E_INVALID, "%s: mean and rstd go together", who);
   if (!(eps >= 0.f)) return fail(DION_E_INVALID, "%s: eps %g", who, (double)eps);
   if (rows == 0) return DION_OK;
@@ -2364,14 +2374,12 @@ extern "C" int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtyp
   if (int rc = check_norm(who, rows, width)) return rc;
   if (int rc = check_rows(who, "dy", dy, lddy, y_dtype, rows, width)) return rc;
   if (int rc = check_rows(who, "x", x, ldx, x_dtype, rows, width)) return rc;
-  if (weight)
-    if (int rc = check_rows(who, "weight", weight, width, weight_dtype, 1, width)) return rc;
-  if (dx)
-    if (int rc = check_rows(who, "dx", dx, width, x_dtype, 1, width)) return rc;
-  if (dweight)
-    if (int rc = check_rows(who, "dweight", dweight, width, weight_dtype, 1, width)) return rc;
-  if (dbias)
-    if (int rc = check_rows(who, "dbias", dbias, width, bias_dtype, 1, width)) return rc;
+  if (int rc = check_vector(who, "weight", weight, weight_dtype)) return rc;
+  if (int rc = check_vector(who, "dx", dx, x_dtype)) return rc;
+  if (int rc = check_vector(who, "dweight", dweight, weight_dtype)) return rc;
+  if (int rc = check_vector(who, "dbias", dbias, bias_dtype)) return rc;
+  if (int rc = check_vector(who, "mean", mean, DION_F32)) return rc;
+  if (int rc = check_vector(who, "rstd", rstd, DION_F32)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (rows == 0) {  // sums over nothing
     if (dweight) HIP_TRY(launch_lin_sum(nullptr, 0, width, dweight, dt(weight_dtype), st), who);

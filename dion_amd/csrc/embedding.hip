@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const EmbeddingArgs
   TY* y = (TY*)a.y + t * a.width;
   Piece<TW, V> p[SLICES];
 #pragma unroll
-  for (int s = 0; s < SLICES; ++s) p[s].load(w + c0 + s * 64 * V, in && c0 + s * 64 * V < a.width);
+  for (int s = 0; s < SLICES; ++s) p[s].load(w, c0 + s * 64 * V, in && c0 + s * 64 * V < a.width);
 #pragma unroll
   for (int s = 0; s < SLICES; ++s) {
     const int c = c0 + s * 64 * V;
@@ -195,27 +195,41 @@ struct SumArgs {
 __device__ __forceinline__ int64_t slot(uint32_t p, bool first) { return (int64_t)(p / kRun) * 2 + first; }
 
 // A slice is S times 512 columns: of a lane S times eight, in pieces of V that lie 64 V apart.
-// acc += the rows of dy of the n tokens that lanes from.. from + n - 1 hold in `token`, in that order.
+// acc += the rows of dy of the tokens that lanes from.. from + U - 1 hold in `token`, of which n are meant, in that order.
+template <typename TY, int V, int S, int U>
+__device__ __forceinline__ void add_group(const SumArgs& a, int token, int from, int n, int slice, int lane, float* acc) {
+  constexpr int NC = 8 * S / V;
+  const int col = slice * (kSlice * S) + lane * V;
+  Piece<TY, V> q[U][NC];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (u >= n) break;
+    const int64_t t = (uint32_t)__builtin_amdgcn_readlane(token, from + u);
+    const TY* dy = (const TY*)a.dy + t * a.lddy;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) q[u][c].load(dy, col + c * 64 * V, col + c * 64 * V < a.width);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < n)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[c * V + e] += q[u][c].get(e);
+}
+// ... of the n tokens from lane `from` on.  Pieces of eight are few enough to ask for eight tokens' whatever n is; of single
+// elements a row has sixty-four, and what is left of n goes by halves.
 template <typename TY, int V, int S>
 __device__ __forceinline__ void add_rows(const SumArgs& a, int token, int from, int n, int slice, int lane, float* acc) {
-  constexpr int NC = 8 * S / V, U = 8 / S;
-  const int col = slice * (kSlice * S) + lane * V;
-  for (int j = 0; j < n; j += U) {
-    Piece<TY, V> q[U][NC];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t t = (uint32_t)__builtin_amdgcn_readlane(token, from + (j + u < n ? j + u : n - 1));
-      const TY* dy = (const TY*)a.dy + t * a.lddy + col;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) q[u][c].load(dy + c * 64 * V, j + u < n && col + c * 64 * V < a.width);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (j + u < n)
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int e = 0; e < V; ++e) acc[c * V + e] += q[u][c].get(e);
+  constexpr int U = 8 / S;
+  if constexpr (V == 8) {
+    for (int j = 0; j < n; j += U) add_group<TY, V, S, U>(a, token, from + j, n - j < U ? n - j : U, slice, lane, acc);
+  } else {
+    int j = 0;
+    for (; j + 8 <= n; j += 8) add_group<TY, V, S, 8>(a, token, from + j, 8, slice, lane, acc);
+    if (n & 4) add_group<TY, V, S, 4>(a, token, from + j, 4, slice, lane, acc), j += 4;
+    if (n & 2) add_group<TY, V, S, 2>(a, token, from + j, 2, slice, lane, acc), j += 2;
+    if (n & 1) add_group<TY, V, S, 1>(a, token, from + j, 1, slice, lane, acc);
   }
 }
 // ... of the n <= 64 that `order` lists from p on.
@@ -271,6 +285,7 @@ __global__ __launch_bounds__(256) void embedding_sums_kernel(const SumArgs a, ui
       n = a.count[unit / a.slices];
     }
     if ((uint32_t)(lane & 7) < n) token = a.order[first + (lane & 7)];
+    asm volatile("" : "+v"(token));  // (waited for here: in the loop that would be a wait for the last row's stores too)
   }
   for (int k = 0; k < kUnits; ++k) {
     const uint32_t unit = w0 + k * stride;
@@ -316,11 +331,11 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embedding_join_kernel(const S
     float acc[8] = {};
 #pragma unroll 8
     for (uint32_t k = k0; k < k1; ++k) {
-      const float* q = a.partial + slot(first + k * kRun, k == 0) * a.width + col;
+      const float* q = a.partial + slot(first + k * kRun, k == 0) * a.width;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         Piece<float, V> p;
-        p.load(q + c * 64 * V, col + c * 64 * V < a.width);
+        p.load(q, col + c * 64 * V, col + c * 64 * V < a.width);
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[c * V + e] += p.get(e);
       }
@@ -441,7 +456,10 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
   p.vocab = a.vocab;
   p.width = a.width;
   p.groups = ix.groups;
-  const bool whole = a.width % 8 == 0 && embedding_fits(a.dy, a.lddy, a.y_dtype, 8) && embedding_fits(a.dw, a.width, a.w_dtype, 8);
+  auto fits = [&](int v) {
+    return a.width % v == 0 && embedding_fits(a.dy, a.lddy, a.y_dtype, v) && embedding_fits(a.dw, a.width, a.w_dtype, v);
+  };
+  const bool whole = fits(8);
   const int wide = whole && a.width >= 2 * kSlice ? 2 : 1;  // slices of 1024 columns: half as many ways to memory, one after the other
   p.slices = (a.width + wide * kSlice - 1) / (wide * kSlice);
   p.scale = a.scale;
@@ -464,6 +482,7 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
     typedef std::integral_constant<int, 1> one;
     if (wide == 2) go(id, ty, tw, std::integral_constant<int, 8>(), std::integral_constant<int, 2>());
     else if (whole) go(id, ty, tw, std::integral_constant<int, 8>(), one());
+    else if (fits(2)) go(id, ty, tw, std::integral_constant<int, 2>(), one());
     else go(id, ty, tw, one(), one());
   };
   auto typed = [&](auto* id) {

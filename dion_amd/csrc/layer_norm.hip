@@ -17,12 +17,12 @@ static __device__ __forceinline__ void param(const void* p, int dtype, int c, bo
     for (int e = 0; e < V; ++e) v[e] = none;
   } else if (dtype) {
     Piece<float, V> q;
-    q.load((const float*)p + c, in);
+    q.load((const float*)p, c, in);
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = q.get(e);
   } else {
     Piece<bf16_t, V> q;
-    q.load((const bf16_t*)p + c, in);
+    q.load((const bf16_t*)p, c, in);
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = q.get(e);
   }
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void norm_forward_kernel(const N
   const TX* x = (const TX*)a.x + (int64_t)row * a.ldx;
   Piece<TX, V> px[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) px[c].load(x + (c * G + t) * V, (c * G + t) * V < a.width);
+  for (int c = 0; c < NC; ++c) px[c].load(x, (c * G + t) * V, (c * G + t) * V < a.width);
   float s = 0.f;  // (E values of x stay as they were read: sixteen bits each, where x is bf16)
 #pragma unroll
   for (int c = 0; c < NC; ++c)
@@ -138,16 +138,18 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   } sets[SETS];
   auto fetch = [&](Row& q, int64_t row) __attribute__((always_inline)) {  // (zeros behind the last row and the last column: they add nothing)
     const bool in = row < a.rows;
+    if (!in) row = 0;
     const TX* x = (const TX*)a.x + row * a.ldx;
     const TY* dy = (const TY*)a.dy + row * a.lddy;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = (c * G + t) * V;
-      q.px[c].load(x + col, in && col < a.width);
-      q.pd[c].load(dy + col, in && col < a.width);
+      q.px[c].load(x, col, in && col < a.width);
+      q.pd[c].load(dy, col, in && col < a.width);
     }
-    q.mean = in ? a.mean[row] : 0.f;
-    q.rstd = in ? a.rstd[row] : 0.f;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    q.mean = in ? mean : 0.f;
+    q.rstd = in ? rstd : 0.f;
   };
   auto one = [&](Row& q, int64_t row, int buf) __attribute__((always_inline)) {
     if constexpr (AHEAD == 0) fetch(q, row);
@@ -337,11 +339,17 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
       auto kernel = WIDE && past ? norm_forward_kernel<TX, TY, G, E, V, WIDE> : norm_forward_kernel<TX, TY, G, E, V, false>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
     };
+    // Up to 64 elements a thread: rows of up to 4096 columns then need no barrier, and wider ones a workgroup of four wavefronts.  Not
+    // where elements are read one by one.  us, 64 / 32 a thread: 16384 x 4096 56 / 66, 4096 x 16384 64 / 87; one by one, 2492 x
+    // 14459 149 / 99, 2492 x 2731 33 / 16.
     auto sized = [&](auto vc) {
+      constexpr bool SINGLE = decltype(vc)::value == 1;
       if (a.width <= 512) run(std::integral_constant<int, 64>(), std::integral_constant<int, 8>(), vc);
+      else if (a.width <= 1024) run(std::integral_constant<int, 64>(), std::integral_constant<int, 16>(), vc);
       else if (a.width <= 2048) run(std::integral_constant<int, 64>(), std::integral_constant<int, 32>(), vc);
-      else if (a.width <= 4096) run(std::integral_constant<int, 64>(), std::integral_constant<int, 64>(), vc);
+      else if (a.width <= 4096 && !SINGLE) run(std::integral_constant<int, 64>(), std::integral_constant<int, SINGLE ? 32 : 64>(), vc);
       else if (a.width <= 8192) run(std::integral_constant<int, 256>(), std::integral_constant<int, 32>(), vc);
+      else if (a.width <= 16384 && !SINGLE) run(std::integral_constant<int, 256>(), std::integral_constant<int, SINGLE ? 32 : 64>(), vc);
       else run(std::integral_constant<int, 1024>(), std::integral_constant<int, 32>(), vc);
     };
     constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;

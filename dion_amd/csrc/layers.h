@@ -49,22 +49,27 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st);
 // 16384 x 4096 36.3 / 32.2.
 constexpr int64_t kPast = int64_t(32) << 20;
 
-// V elements as one access moves them: zeros, and nothing read, where `in` is false.
+// V elements as one access moves them.
 template <typename T, int V>
 struct Piece {
   static constexpr int BYTES = (int)sizeof(T) * V;
   typedef std::conditional_t<BYTES == 32, f32x4, std::conditional_t<BYTES == 16, u32x4_t, std::conditional_t<BYTES == 8, u32x2_t,
           std::conditional_t<BYTES == 4, uint32_t, uint16_t>>>> raw_t;
-  raw_t r[BYTES == 32 ? 2 : 1];
-  __device__ __forceinline__ void load(const T* p, bool in) {
+  typedef std::conditional_t<BYTES == 2, uint32_t, raw_t> held_t;
+  held_t r[BYTES == 32 ? 2 : 1];
+  // Elements `at` .. of a row, or zeros where `in` is false: then the row's first ones are read.  (A load that is skipped is a branch,
+  // into which the compiler takes what follows from a narrow load, and its wait with it.  us, rows of single bf16 elements, branch /
+  // none: layer norm of 2492 x 2731, forward 41.5 / 33.4; 6465 tokens of 18573 x 2155, sums 345 / 49.)
+  __device__ __forceinline__ void load(const T* row, int at, bool in) {
+    const raw_t* p = (const raw_t*)(row + (in ? at : 0));
 #pragma unroll
     for (int k = 0; k < (BYTES == 32 ? 2 : 1); ++k) {
-      raw_t zero = {};
-      r[k] = in ? ((const raw_t*)p)[k] : zero;
+      const held_t zero = {}, v = (held_t)p[k];
+      r[k] = in ? v : zero;
     }
   }
   __device__ __forceinline__ float get(int e) const {
-    if constexpr (BYTES == 2) return bf16_to_f32(r[0]);
+    if constexpr (BYTES == 2) return __uint_as_float(r[0] << 16);
     else if constexpr (BYTES == 4 && sizeof(T) == 4) return __uint_as_float(r[0]);
     else if constexpr (BYTES == 4) return __uint_as_float(e ? r[0] & 0xffff0000u : r[0] << 16);
     else if constexpr (BYTES == 32) return r[e >> 2][e & 3];

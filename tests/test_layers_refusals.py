@@ -41,13 +41,16 @@ def rows_backward(lib, ids=P, bits=64, t=8, dy=P, ld=64, yt=0, v=100, d=64, pad=
 CASES = {
     gated_forward: ({"t": -1}, {"k": 0}, {"n": 0}, {"n": 1 << 20}, {"k": 1 << 21}, {"t": (1 << 30) + 1}, {"act": 6}, {"act": -1},
                     {"x": None}, {"wg": None}, {"wu": None}, {"h": None}, {"h": P + 1}, {"x": P + 1}, {"ldx": 63}, {"ldg": 63},
-                    {"ldu": 63}, {"bg": P, "bgt": 2}, {"bu": P, "but": -1}, {"kept": P + 8}, {"kept": P, "bits": 16}),
+                    {"ldu": 63}, {"bg": P, "bgt": 2}, {"bu": P, "but": -1}, {"bg": P + 2, "bgt": 1}, {"bu": P + 1}, {"kept": P + 8}, {"kept": P, "bits": 16}),
     gated_backward: ({"t": -1}, {"dh": None}, {"ld": 31}, {"kept": None}, {"kept": P + 2}, {"bits": 16}, {"x": None}, {"wg": None}, {"wu": None},
-                     {"ldx": 8}, {"ldg": 8}, {"ldu": 8}, {"dbg": P, "dbgt": 3}, {"dbu": P, "dbut": 3}, {"n": 1 << 20}),
+                     {"ldx": 8}, {"ldg": 8}, {"ldu": 8}, {"dbg": P, "dbgt": 3}, {"dbu": P, "dbut": 3}, {"n": 1 << 20}, {"dx": P + 1},
+                     {"dg": P + 1}, {"du": P + 1}, {"dbu": P + 2, "dbut": 1}),
     norm_forward: ({"rows": -1}, {"width": 0}, {"width": (1 << 24) + 1}, {"x": None}, {"y": None}, {"ldx": 63}, {"xt": 2}, {"yt": -1},
-                   {"wt": 2}, {"bt": 2}, {"x": P + 1}, {"w": P + 2}, {"mean": P}, {"rstd": P}, {"eps": -1.0}, {"eps": float("nan")}),
+                   {"wt": 2}, {"bt": 2}, {"x": P + 1}, {"w": P + 2}, {"mean": P}, {"rstd": P}, {"mean": P + 2, "rstd": P},
+                   {"eps": -1.0}, {"eps": float("nan")}),
     norm_backward: ({"rows": -1}, {"width": 0}, {"dy": None}, {"x": None}, {"ld": 63}, {"ldx": 63}, {"mean": None}, {"rstd": None},
-                    {"xt": 2}, {"yt": 2}, {"wt": 2}, {"bt": 2}, {"dx": P + 1}, {"dw": P + 2}, {"db": P + 2}),
+                    {"xt": 2}, {"yt": 2}, {"wt": 2}, {"bt": 2}, {"dx": P + 1}, {"dw": P + 2}, {"db": P + 2},
+                    {"rstd": P + 2}),
     rows_forward: ({"bits": 16}, {"t": -1}, {"v": 0}, {"d": 0}, {"v": (1 << 24) + 1}, {"t": (1 << 30) + 1}, {"ids": None}, {"ids": P + 4},
                    {"w": None}, {"y": None}, {"ldw": 63}, {"wt": 2}, {"yt": 2}, {"w": P + 2}),
     rows_backward: ({"bits": 8}, {"t": -1}, {"v": 0}, {"ids": None}, {"dy": None}, {"dw": None}, {"ld": 63}, {"yt": 2}, {"wt": 2},
