@@ -3,7 +3,12 @@
 //   dg = dh u act'(g),  du = dh act(g)   elementwise, from two values of 24 (32) bits an element that the forward pass keeps
 //   dx = dg Wg + du Wu                   one reduction over both (pair form): dx is rounded once and no sum goes through memory
 //   dWg = dg^T x,  dWu = du^T x          one product of linear.hip where the results lie behind one another
-// Operands bf16, sums fp32.  Tiles, ring and epilogue are lin_tile.h's.
+// Operands bf16, sums fp32.  Tiles, ring and epilogue are lin_tile.h's; like linear.hip's products, large ones are bound by the matrix
+// units at the clock the power limit leaves, and by what all CUs store when a round of tiles ends.
+// us: 8192 x 4096 x 14336 (tokens, fan-in, fan-out) forward 1360, 1.41 PFLOP/s; 8192 x 2048 x 5632 forward with what is kept 351 (277 MB
+// of it; 1408 tiles of 256 x 256, 5.5 rounds of the CUs), dz 108, dx 279, dW 322 (704 tiles of 256 x 128, 2.75 rounds); 8192 x 2048
+// x 8192 480, 180, 418, 409, forward without keeping 424 (1.30 PFLOP/s).  Two workgroups a CU of 128 x 128 tiles in a ring of two slots, so
+// that one stores while the other multiplies, take 452 instead of 351 and 571 instead of 424: their operands come twice as often.
 #include "lin_tile.h"
 
 namespace dion {
@@ -45,7 +50,7 @@ static __device__ __forceinline__ void gated4_any(const GatedEpilogue& p, int ro
   store4(p, p.C + (int64_t)row * p.N + col, col, make_uint2(pack_bf16x2(h[0], h[1]), pack_bf16x2(h[2], h[3])));
 }
 
-// Adds the parts of a split reduction, in their order, and finishes: four elements per thread.
+// Adds the parts of a split reduction, in their order, and finishes: four elements per thread.  24 x 8192 in eight parts 4 us.
 __global__ __launch_bounds__(256) void gated_join_kernel(const GatedEpilogue p, const float* __restrict__ part, int splits) {
   const int per_row = (p.N + 3) / 4;
   const int64_t all = (int64_t)p.M * per_row, one = (int64_t)p.M * p.N;
@@ -75,7 +80,8 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const GatedEpilogue p, 
 // ---------------------------------------------------------------------------------------------- few tokens
 // Up to 32 rows of x: a workgroup takes eight rows of each weight, which are the sixteen rows of an MFMA operand, and its wavefronts
 // an equal run of the reduction each; fragments go from memory to registers, the next U steps' while the MFMAs of these run.
-// The wavefronts' sums meet in LDS and are added in their order; rows 0-7 of a product are g's, 8-15 u's.
+// The wavefronts' sums meet in LDS and are added in their order; rows 0-7 of a product are g's, 8-15 u's.  Bound by the weights'
+// bytes: one token of 4096 x 14336 41.5 us (5.7 TB/s, the weights from HBM); of 768 x 2048 4.9 (launch, one way to memory, LDS).
 template <int TB, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(const GatedEpilogue p, const bf16_t* __restrict__ x, int64_t ldx,
                                                                const bf16_t* __restrict__ wg, int64_t ldg,
@@ -140,6 +146,8 @@ __global__ __launch_bounds__(WAVES * 64) void gated_few_kernel(const GatedEpilog
 // ---------------------------------------------------------------------------------------------- gradients at g and u
 constexpr int kDzCols = 256;  // columns of a workgroup: 32 threads of eight, by eight rows
 
+// One pass for both: 12 bytes an element (14 with 32 bits kept), 8192 x 5632 108 us (5.1 TB/s).  Four rows at a time instead of two
+// take 17 us more; results stored around the caches, where the products then do not find them, 19 with these.
 // W: elements of dh that are read at once; 8: every row is whole chunks.
 template <bool WIDE, bool DST, bool SUM, int W>
 __global__ __launch_bounds__(256) void gated_dz_kernel(const bf16_t* __restrict__ dh, int64_t ld, const char* __restrict__ kept,

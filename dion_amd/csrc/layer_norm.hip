@@ -1,7 +1,9 @@
 // Layer norm of rows of x:  m = mean x,  r = 1 / sqrt(mean (x - m)^2 + eps),  xh = (x - m) r,  y = xh w + b,
 // and its gradients, with g = dy w:  dx = r (g - mean g - xh mean(g xh)),  dw = sum over the rows of dy xh,  db = of dy.
 // Rows stay in registers between the two sums of a pass (the variance is that of the centred values: no difference of large
-// numbers), so x and dy are read once.  Sums fp32, in an order that depends on the sizes alone.
+// numbers), so x and dy are read once.  Sums fp32, in an order that depends on the sizes alone.  Bound by HBM.  us, bf16: 16384 x 4096
+// forward 55 (4.9 TB/s), backward 67 (6.0) and 4 for the sums over the workgroups; 4096 x 16384 64 and 114, 65536 x 768 41 and 54;
+// one row of 768 2.4, a launch and one way to memory.
 #include "layers.h"
 #include "linear.h"
 
@@ -116,7 +118,9 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const NormArgs 
 }
 
 // dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy: sixteen wavefronts take
-// 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them.
+// 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them, and one
+// workgroup a CU leaves few parts to add.  us, 16384 x 4096: one row ahead of 16 elements a thread 93, two of eight 87, dx around the
+// caches 75, loads without branches 67.
 template <typename TX, typename TY, int G, int E, int V, bool PAST>
 __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   constexpr int NC = E / V, ROWS = 1024 / G;

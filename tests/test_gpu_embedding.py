@@ -60,7 +60,7 @@ def run_and_check(ids, w, dy, scale=1.0, padding=None):
 
 
 SIZES = [(1, 1, 1), (1, 5, 8), (3, 7, 5), (64, 1, 24), (65, 1, 24), (64, 300, 77), (65, 300, 512), (1000, 3, 520), (1000, 257, 513),
-         (1023, 5000, 64), (1025, 200, 1000), (3000, 131073, 96), (5000, 70, 768), (20000, 1001, 264), (17000, 40000, 128)]
+         (1023, 5000, 64), (1025, 200, 1000), (3000, 131073, 96), (5000, 70, 768), (20000, 1001, 264), (17000, 40000, 128), (700, 90, 1254), (300, 50, 10), (2000, 3, 2050)]
 
 
 @pytest.mark.parametrize("tokens,vocab,d", SIZES)
@@ -70,10 +70,11 @@ def test_sizes_and_types(tokens, vocab, d, table, y, scale, padding):
     run_and_check(ids, *make(ids, vocab, d, table, y), scale, padding)
 
 
-@pytest.mark.parametrize("tokens", [1, 63, 64, 65, 128, 129, 1024, 1025, 4096, 30000])
+@pytest.mark.parametrize("tokens", [1, 63, 64, 65, 128, 129, 1024, 1025, 4096, 30000, 50000])
 @pytest.mark.parametrize("form", ["same", "same_but_one", "two_in_turn", "ascending", "one_workgroup", "blocks_of_65"])
 def test_runs_of_equal_tokens(tokens, form):
-    """Rows whose tokens end and start inside a run, all tokens in one row, and many rows of one workgroup of the index."""
+    """Rows whose tokens end and start inside a run, all tokens in one row, and many rows of one workgroup of the index, with more tokens
+    of a wavefront's run than its list has room for (2147 of 3136, at 50000)."""
     vocab = 40001
     at = torch.arange(tokens, device=DEV)
     ids = {"same": torch.full((tokens,), 33333, device=DEV), "same_but_one": torch.where(at == tokens // 2, 7, 256 * 7),
