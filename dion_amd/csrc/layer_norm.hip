@@ -344,16 +344,16 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
     };
     // Up to 64 elements a thread: rows of up to 4096 columns then need no barrier, and wider ones a workgroup of four wavefronts.  Not
-    // where elements are read one by one.  us, 64 / 32 a thread: 16384 x 4096 56 / 66, 4096 x 16384 64 / 87; one by one, 2492 x
-    // 14459 149 / 99, 2492 x 2731 33 / 16.
+    // where they are read one by one, and in the first case not in pairs.  us, 64 / 32 a thread: 16384 x 4096 56 / 66, 4096 x 16384
+    // 64 / 87; in pairs 4096 x 4094 28 / 20, 2492 x 14458 47 / 59; one by one 2492 x 2731 33 / 16, 2492 x 14459 149 / 99.
     auto sized = [&](auto vc) {
-      constexpr bool SINGLE = decltype(vc)::value == 1;
+      constexpr int V = decltype(vc)::value;
       if (a.width <= 512) run(std::integral_constant<int, 64>(), std::integral_constant<int, 8>(), vc);
       else if (a.width <= 1024) run(std::integral_constant<int, 64>(), std::integral_constant<int, 16>(), vc);
       else if (a.width <= 2048) run(std::integral_constant<int, 64>(), std::integral_constant<int, 32>(), vc);
-      else if (a.width <= 4096 && !SINGLE) run(std::integral_constant<int, 64>(), std::integral_constant<int, SINGLE ? 32 : 64>(), vc);
+      else if (a.width <= 4096 && V >= 4) run(std::integral_constant<int, 64>(), std::integral_constant<int, V >= 4 ? 64 : 32>(), vc);
       else if (a.width <= 8192) run(std::integral_constant<int, 256>(), std::integral_constant<int, 32>(), vc);
-      else if (a.width <= 16384 && !SINGLE) run(std::integral_constant<int, 256>(), std::integral_constant<int, SINGLE ? 32 : 64>(), vc);
+      else if (a.width <= 16384 && V >= 2) run(std::integral_constant<int, 256>(), std::integral_constant<int, V >= 2 ? 64 : 32>(), vc);
       else run(std::integral_constant<int, 1024>(), std::integral_constant<int, 32>(), vc);
     };
     constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;
