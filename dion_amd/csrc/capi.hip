@@ -2220,14 +2220,16 @@ extern "C" int dion_gated_forward(const void* x, int64_t ldx, const void* w_gate
 }
 
 extern "C" int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kept_bits, const void* x, int64_t ldx,
-                                   const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate, void* dw_up,
-                                   void* db_gate, int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in,
+                                   const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate,
+                                   void* dw_up, int dw_behind, void* db_gate, int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in,
                                    int fan_out, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "dion_gated_backward";
   if (int rc = check_gated(who, tokens, fan_in, fan_out)) return rc;
   if (int rc = check_vector(who, "dx", dx, DION_BF16)) return rc;
   if (int rc = check_vector(who, "dw_gate", dw_gate, DION_BF16)) return rc;
   if (int rc = check_vector(who, "dw_up", dw_up, DION_BF16)) return rc;
+  if (dw_behind && (!dw_gate || (uintptr_t)dw_up != (uintptr_t)dw_gate + (size_t)round8(fan_out) * fan_in * 2))
+    return fail(DION_E_INVALID, "%s: dw_up is not %d rows behind dw_gate", who, round8(fan_out));
   if (int rc = check_vector(who, "db_gate", db_gate, db_gate_dtype)) return rc;
   if (int rc = check_vector(who, "db_up", db_up, db_up_dtype)) return rc;
   hipStream_t st = (hipStream_t)stream;
@@ -2292,14 +2294,13 @@ extern "C" int dion_gated_backward(const void* dh, int64_t ld_dh, const void* ke
   p.K = tokens;
   p.Q = (const bf16_t*)x;
   p.ldq = ldx;
-  const bool behind = dw_gate && dw_up && (char*)dw_up == (char*)dw_gate + (size_t)np * fan_in * 2;
   if (dw_gate) {
     p.P = dz;
-    p.M = behind ? np + fan_out : fan_out;
+    p.M = dw_behind ? np + fan_out : fan_out;
     p.C = (bf16_t*)dw_gate;
     HIP_TRY(launch_lin_product(p, st), who);
   }
-  if (dw_up && !behind) {
+  if (dw_up && !dw_behind) {
     p.P = dz + np;
     p.M = fan_out;
     p.C = (bf16_t*)dw_up;

@@ -24,7 +24,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        grads = ops.layer_norm_grads if type(dy) is Tensor else ops.layer_norm_backward
+        grads = ops.layer_norm_grads if ops.plain_on_one_device(dy, x, weight, stats) else ops.layer_norm_backward
         return (*grads(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
 
 
@@ -32,7 +32,8 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
                dtype: Optional[torch.dtype] = None) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension: ``x [..., width]``, ``weight`` and ``bias``
     ``[width]``, bfloat16 or float32 each; the result is of ``dtype`` (None: that of ``x``).  ``var`` is the mean square of the centred
-    values; arithmetic and sums are float32, and the result is rounded once.
+    values; arithmetic and sums are float32, and the result is rounded once (a row whose squares leave float32, with values past 1.8e19,
+    comes out as the bias).
 
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
     the backward pass it keeps ``x``, the weight and two float32 values a row.  Gradients are of their tensor's type, sums of
@@ -58,8 +59,9 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     @_once
     def backward(ctx, dy):
-        grad = ops.embedding_grad if type(dy) is Tensor else ops.embedding_backward
-        return None, grad(dy, ctx.saved_tensors[0], *ctx.table), None, None, None
+        ids = ctx.saved_tensors[0]
+        grad = ops.embedding_grad if ops.plain_on_one_device(dy, ids) else ops.embedding_backward
+        return None, grad(dy, ids, *ctx.table), None, None, None
 
 
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,

@@ -1248,6 +1248,18 @@ def _code(t: Optional[Tensor]) -> int:
     return DION_F32 if t is not None and t.dtype == torch.float32 else DION_BF16
 
 
+def plain_on_one_device(t: Tensor, *others: Optional[Tensor]) -> bool:
+    """Whether a gradient and what a forward pass kept can be read as they are: not where autograd, or a hook on what it saved, has given
+    back a wrapper or a tensor that lies elsewhere."""
+    index = t.get_device()
+    if index < 0 or type(t) not in _PLAIN_SET:
+        return False
+    for o in others:
+        if o is not None and (type(o) not in _PLAIN_SET or o.get_device() != index):
+            return False
+    return True
+
+
 def _viewed(t: Tensor, lead, cols: int) -> Tensor:
     return t if len(lead) == 1 else t.view(*lead, cols)
 
@@ -1340,7 +1352,8 @@ def gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, 
         ws = _space(nbytes, dh.device)
         dx = dh.new_empty((tokens, fan_in)) if need_dx else None
         dgate = dup = None
-        if need_dgate and need_dup:  # (one product: the second behind the first, which starts on a multiple of 8 rows)
+        behind = need_dgate and need_dup
+        if behind:  # (one product: the second behind the first, which starts on a multiple of 8 rows)
             both = dh.new_empty((-(-fan_out // 8) * 8 + fan_out, fan_in))
             dgate, dup = both[:fan_out], both[-fan_out:]
         elif need_dgate:
@@ -1350,7 +1363,7 @@ def gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, 
         dbg = dh.new_empty((fan_out,), dtype=bias_gate_dtype) if bias_gate_dtype is not None else None
         dbu = dh.new_empty((fan_out,), dtype=bias_up_dtype) if bias_up_dtype is not None else None
         check(_lib.load().dion_gated_backward(pdh, lddh, kept.data_ptr(), keep, px, ldx, pg, ldg, pu, ldu, _ptr(dx),
-                                              _ptr(dgate), _ptr(dup), _ptr(dbg), _code(dbg), _ptr(dbu), _code(dbu), tokens, fan_in,
+                                              _ptr(dgate), _ptr(dup), behind, _ptr(dbg), _code(dbg), _ptr(dbu), _code(dbu), tokens, fan_in,
                                               fan_out, _ptr(ws), nbytes, _stream_handle(dh.device)), "gated_linear backward")
     return (_viewed(dx, lead, fan_in) if need_dx else None), dgate, dup, dbg, dbu
 

@@ -470,11 +470,11 @@ int dion_gated_forward(const void* x, int64_t ldx, const void* w_gate, int64_t l
 
 /* dg = dh act'(g) u, du = dh act(g) (rounded to bf16 for the products, not for the biases):  dx = dg w_gate + du w_up,
  * dw_gate = dg^T x,  dw_up = du^T x,  db_gate, db_up = sums over the tokens.  Any of them may be null; x is read for dw_*, the weights
- * for dx.  dw_up fan_out rounded up to 8 rows behind dw_gate: one product instead of two, which also writes what rows lie between
- * them (zeros). */
+ * for dx.  dw_behind: dw_up lies fan_out rounded up to 8 rows behind dw_gate, and the rows between them, which are written (zeros),
+ * belong to the same buffer: one product instead of two. */
 int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kept_bits, const void* x, int64_t ldx,
-                        const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate, void* dw_up, void* db_gate,
-                        int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in, int fan_out, void* workspace,
+                        const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate, void* dw_up,
+                        int dw_behind, void* db_gate, int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in, int fan_out, void* workspace,
                         size_t workspace_bytes, void* stream);
 
 /* --------------------------------------------------------------------------------------------

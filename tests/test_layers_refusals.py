@@ -16,9 +16,9 @@ def gated_forward(lib, x=P, ldx=64, wg=P, ldg=64, wu=P, ldu=64, bg=None, bgt=0, 
     return lib.dion_gated_forward(x, ldx, wg, ldg, wu, ldu, bg, bgt, bu, but, act, h, kept, bits, t, k, n, ws, nbytes, None)
 
 
-def gated_backward(lib, dh=P, ld=32, kept=P, bits=32, x=P, ldx=64, wg=P, ldg=64, wu=P, ldu=64, dx=P, dg=P, du=P, dbg=None, dbgt=0, dbu=None,
-                   dbut=0, t=8, k=64, n=32, ws=None, nbytes=0):
-    return lib.dion_gated_backward(dh, ld, kept, bits, x, ldx, wg, ldg, wu, ldu, dx, dg, du, dbg, dbgt, dbu, dbut, t, k, n, ws, nbytes, None)
+def gated_backward(lib, dh=P, ld=32, kept=P, bits=32, x=P, ldx=64, wg=P, ldg=64, wu=P, ldu=64, dx=P, dg=P, du=P, behind=0, dbg=None, dbgt=0,
+                   dbu=None, dbut=0, t=8, k=64, n=32, ws=None, nbytes=0):
+    return lib.dion_gated_backward(dh, ld, kept, bits, x, ldx, wg, ldg, wu, ldu, dx, dg, du, behind, dbg, dbgt, dbu, dbut, t, k, n, ws, nbytes, None)
 
 
 def norm_forward(lib, x=P, ldx=64, xt=0, w=P, wt=1, b=P, bt=1, y=P, yt=0, mean=None, rstd=None, rows=8, width=64, eps=1e-5):
@@ -44,7 +44,8 @@ CASES = {
                     {"ldu": 63}, {"bg": P, "bgt": 2}, {"bu": P, "but": -1}, {"bg": P + 2, "bgt": 1}, {"bu": P + 1}, {"kept": P + 8}, {"kept": P, "bits": 16}),
     gated_backward: ({"t": -1}, {"dh": None}, {"ld": 31}, {"kept": None}, {"kept": P + 2}, {"bits": 16}, {"x": None}, {"wg": None}, {"wu": None},
                      {"ldx": 8}, {"ldg": 8}, {"ldu": 8}, {"dbg": P, "dbgt": 3}, {"dbu": P, "dbut": 3}, {"n": 1 << 20}, {"dx": P + 1},
-                     {"dg": P + 1}, {"du": P + 1}, {"dbu": P + 2, "dbut": 1}),
+                     {"dg": P + 1}, {"du": P + 1}, {"dbu": P + 2, "dbut": 1}, {"behind": 1}, {"behind": 1, "du": None},
+                     {"behind": 1, "n": 30, "ld": 30, "du": P + 30 * 64 * 2}),
     norm_forward: ({"rows": -1}, {"width": 0}, {"width": (1 << 24) + 1}, {"x": None}, {"y": None}, {"ldx": 63}, {"xt": 2}, {"yt": -1},
                    {"wt": 2}, {"bt": 2}, {"x": P + 1}, {"w": P + 2}, {"mean": P}, {"rstd": P}, {"mean": P + 2, "rstd": P},
                    {"eps": -1.0}, {"eps": float("nan")}),
