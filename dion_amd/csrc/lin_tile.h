@@ -1,5 +1,5 @@
-// What the products of weights share: activations, the tile kernel in its forms, the estimate a product's tiles are chosen by
-// (linear.hip: y = act(x W^T + b) + residual and its gradients; gated.hip: act(x Wg^T + bg) * (x Wu^T + bu) and its own).
+// What the products of weights share: activations, the tile kernel in its forms, and its launch (linear.hip: y = act(x W^T + b) +
+// residual and its gradients; gated.hip: act(x Wg^T + bg) * (x Wu^T + bu) and its own).
 #pragma once
 #include <atomic>
 
