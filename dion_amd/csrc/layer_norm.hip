@@ -117,7 +117,13 @@ __global__ __launch_bounds__(1024) void norm_forward_wide_kernel(const NormArgs 
   }
 }
 
-// dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy: sixteen wavefronts take
+static __device__ __forceinline__ void put(void* p, int dtype, int c, float v) {
+  if (dtype) ((float*)p)[c] = v;
+  else ((bf16_t*)p)[c] = f32_to_bf16(v);
+}
+
+// dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy (of a single workgroup they are
+// dw and db): sixteen wavefronts take
 // 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them, and one
 // workgroup a CU leaves few parts to add.  us, 16384 x 4096: one row ahead of 16 elements a thread 93, two of eight 87, dx around the
 // caches 75, loads without branches 67.
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
       buf ^= 1;
     }
   }
-  if (!a.partial) return;
+  if (!a.partial && !a.dw && !a.db) return;
   // The groups' sums meet in LDS, the upper half of them added to the lower one until one is left.
   auto meet = [&](float* v) __attribute__((always_inline)) {
     if constexpr (ROWS > 1) {
@@ -235,15 +241,20 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   meet(dw);
   meet(db);
   if (group > 0) return;
-  float* out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
+  float* const out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = (c * G + t) * V;
     if (col >= a.width) continue;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      out[col + e] = dw[c * V + e];
-      out[a.width + col + e] = db[c * V + e];
+      if (a.partial) {
+        out[col + e] = dw[c * V + e];
+        out[a.width + col + e] = db[c * V + e];
+      } else {
+        if (a.dw) put(a.dw, a.w_dtype, col + e, dw[c * V + e]);
+        if (a.db) put(a.db, a.b_dtype, col + e, db[c * V + e]);
+      }
     }
   }
 }
@@ -291,15 +302,19 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a, int
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows fill.
+// Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows
+// fill; a single one for what it does in four turns, which saves the launch that adds the parts.
 static int norm_threads(int width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 2048 ? 256 : width <= 4096 ? 512 : 1024; }
 static int norm_parts(int rows, int width) {
   if (width > kNormWide) return rows < 128 ? rows : 128;
   const int at_once = 1024 / norm_threads(width);
   const int wgs = (rows + at_once - 1) / at_once;
-  return wgs < 256 ? wgs : 256;
+  return wgs <= 4 ? 1 : wgs < 256 ? wgs : 256;
 }
-size_t norm_partial_floats(int rows, int width) { return rows > 0 ? (size_t)norm_parts(rows, width) * 2 * width : 0; }
+size_t norm_partial_floats(int rows, int width) {
+  const int parts = rows > 0 ? norm_parts(rows, width) : 0;
+  return parts > 1 || width > kNormWide ? (size_t)parts * 2 * width : 0;
+}
 
 // Elements that one access can move: 8 (4 with fp32 on either side), 2 or 1, by what every row's start is a multiple of.
 static int norm_vec(const NormArgs& a, const void* other, int64_t ldo, int other_dtype) {
@@ -365,11 +380,13 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
-  if (a.rows <= 0 || a.width <= 0 || !a.x || !a.dy || !a.mean || !a.rstd || ((a.dw || a.db) && !a.partial)) return hipErrorInvalidValue;
+  if (a.rows <= 0 || a.width <= 0 || !a.x || !a.dy || !a.mean || !a.rstd) return hipErrorInvalidValue;
   NormArgs p = a;
   p.b = nullptr;  // (not read)
   const bool past = (int64_t)a.rows * a.width * (a.x_dtype ? 4 : 2) > kPast;
-  if (!a.dw && !a.db) p.partial = nullptr;
+  const bool sums = a.dw || a.db, joined = sums && norm_partial_floats(a.rows, a.width) > 0;
+  if (joined && !a.partial) return hipErrorInvalidValue;
+  if (!joined) p.partial = nullptr;
   const int parts = norm_parts(a.rows, a.width);
   hipError_t e = norm_types(p, [&](auto* tx, auto* ty) {
     typedef std::remove_pointer_t<decltype(tx)> TX;
@@ -402,7 +419,7 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
     else if (v == 2) sized(std::integral_constant<int, 2>());
     else sized(std::integral_constant<int, 1>());
   });
-  if (e != hipSuccess || !p.partial) return e;
+  if (e != hipSuccess || !joined) return e;
   return launch_lin_sum(p.partial, parts, a.width, p.dw, p.w_dtype, st, p.db, p.b_dtype);
 }
 

@@ -17,7 +17,7 @@ struct NormArgs {
   const void* dy;
   int64_t lddy;
   void* dx;
-  float* partial;  // norm_partial_floats(rows, width) where dw or db is asked for
+  float* partial;  // norm_partial_floats(rows, width), which may be none, where dw or db is asked for
   void *dw, *db;   // of w_dtype, b_dtype, or null
 };
 size_t norm_partial_floats(int rows, int width);
