@@ -122,8 +122,50 @@ static __device__ __forceinline__ void put(void* p, int dtype, int c, float v) {
   else ((bf16_t*)p)[c] = f32_to_bf16(v);
 }
 
-// dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy (of a single workgroup they are
-// dw and db): sixteen wavefronts take
+// dw and db of a.lanes (16, 64) columns from all rows, a column a lane: sixteen wavefronts take 1024 / a.lanes rows at a time, eight
+// times as many on their way.
+template <typename TX, typename TY>
+static __device__ __forceinline__ void few_rows_columns(const NormArgs& a, int block, float (*sums)[16][64]) {
+  constexpr int AHEAD = 8;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int of = lane & (a.lanes - 1), c = block * a.lanes + of, at = c < a.width ? c : 0, step = 1024 / a.lanes;
+  float dw = 0.f, db = 0.f;
+  for (int r0 = (int)threadIdx.x / a.lanes; r0 < a.rows; r0 += step * AHEAD) {
+    Piece<TX, 1> x[AHEAD];
+    Piece<TY, 1> d[AHEAD];
+    float mean[AHEAD], rstd[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t r = r0 + step * k < a.rows ? r0 + step * k : r0;
+      x[k].load((const TX*)a.x + r * a.ldx, at, true);
+      d[k].load((const TY*)a.dy + r * a.lddy, at, true);
+      mean[k] = a.mean[r];
+      rstd[k] = a.rstd[r];
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const bool in = r0 + step * k < a.rows;
+      const float v = d[k].get(0), w = fmaf(v, (x[k].get(0) - mean[k]) * rstd[k], dw);
+      dw = in ? w : dw;
+      db = in ? db + v : db;
+    }
+  }
+  for (int h = a.lanes; h < 64; h <<= 1) {
+    dw += __shfl_xor(dw, h, 64);
+    db += __shfl_xor(db, h, 64);
+  }
+  sums[0][wave][lane] = dw;
+  sums[1][wave][lane] = db;
+  __syncthreads();
+  if (wave > 1 || lane >= a.lanes || c >= a.width) return;
+  float s = sums[wave][0][lane];
+#pragma unroll
+  for (int k = 1; k < 16; ++k) s += sums[wave][k][lane];
+  if (wave == 0 && a.dw) put(a.dw, a.w_dtype, c, s);
+  if (wave == 1 && a.db) put(a.db, a.b_dtype, c, s);
+}
+
+// dx of every row and, in a.partial [workgroups][2][width], this workgroup's sums of dy xh and of dy: sixteen wavefronts take
 // 1024 / G rows at a time, the next ones' x and dy on their way meanwhile; a thread's columns are the same in all of them, and one
 // workgroup a CU leaves few parts to add.  us, 16384 x 4096: one row ahead of 16 elements a thread 93, two of eight 87, dx around the
 // caches 75, loads without branches 67.
@@ -131,9 +173,14 @@ template <typename TX, typename TY, int G, int E, int V, bool PAST>
 __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
   constexpr int NC = E / V, ROWS = 1024 / G;
   __shared__ float sums[2][16][2];
-  __shared__ float half[ROWS > 1 ? ROWS / 2 * G * E : 1];
+  constexpr int HALF = ROWS > 1 ? ROWS / 2 * G * E : 0;
+  __shared__ float half[HALF > 2048 ? HALF : 2048];
+  if ((int)blockIdx.x >= a.row_wgs) {
+    few_rows_columns<TX, TY>(a, blockIdx.x - a.row_wgs, (float(*)[16][64])half);
+    return;
+  }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave / (G / 64), t = threadIdx.x % G;
-  const int64_t step = (int64_t)gridDim.x * ROWS;
+  const int64_t step = (int64_t)a.row_wgs * ROWS;
   int64_t first = (int64_t)blockIdx.x * ROWS;
   const float n = 1.f / (float)a.width;
   // Rows on their way: two of eight elements a thread in one access; one in more; none of sixteen elements.
@@ -221,7 +268,7 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
       buf ^= 1;
     }
   }
-  if (!a.partial && !a.dw && !a.db) return;
+  if (!a.partial) return;
   // The groups' sums meet in LDS, the upper half of them added to the lower one until one is left.
   auto meet = [&](float* v) __attribute__((always_inline)) {
     if constexpr (ROWS > 1) {
@@ -248,13 +295,8 @@ __global__ __launch_bounds__(1024) void norm_backward_kernel(const NormArgs a) {
     if (col >= a.width) continue;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      if (a.partial) {
-        out[col + e] = dw[c * V + e];
-        out[a.width + col + e] = db[c * V + e];
-      } else {
-        if (a.dw) put(a.dw, a.w_dtype, col + e, dw[c * V + e]);
-        if (a.db) put(a.db, a.b_dtype, col + e, db[c * V + e]);
-      }
+      out[col + e] = dw[c * V + e];
+      out[a.width + col + e] = db[c * V + e];
     }
   }
 }
@@ -302,18 +344,20 @@ __global__ __launch_bounds__(256) void norm_columns_kernel(const NormArgs a, int
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows
-// fill; a single one for what it does in four turns, which saves the launch that adds the parts.
+// Threads of a row of the backward pass, eight elements each (sixteen of the widest), and its workgroups: one per CU, or what the rows fill.
 static int norm_threads(int width) { return width <= 512 ? 64 : width <= 1024 ? 128 : width <= 2048 ? 256 : width <= 4096 ? 512 : 1024; }
 static int norm_parts(int rows, int width) {
   if (width > kNormWide) return rows < 128 ? rows : 128;
   const int at_once = 1024 / norm_threads(width);
   const int wgs = (rows + at_once - 1) / at_once;
-  return wgs <= 4 ? 1 : wgs < 256 ? wgs : 256;
+  return wgs < 256 ? wgs : 256;
 }
+// Few rows: dw and db are other workgroups' of the same launch, which read x and dy again, from the caches, instead of parts that a second
+// launch adds; 64 columns each where eight loads fetch all rows of them, 16 otherwise.  us, so / in parts and their launch: 16 x 768
+// 4.6 / 9.0, 128 x 4096 5.6 / 14, 512 x 768 5.4 / 10, 777 x 1001 fp32 8.3 / 11.3, 1024 x 1024 8.6 / 11; 1024 x 2048 18 / 15.
+static bool norm_few(int rows, int width) { return rows <= 1024 && width <= kNormWide && (int64_t)rows * width <= 1 << 20; }
 size_t norm_partial_floats(int rows, int width) {
-  const int parts = rows > 0 ? norm_parts(rows, width) : 0;
-  return parts > 1 || width > kNormWide ? (size_t)parts * 2 * width : 0;
+  return rows <= 0 || norm_few(rows, width) ? 0 : (size_t)norm_parts(rows, width) * 2 * width;
 }
 
 // Elements that one access can move: 8 (4 with fp32 on either side), 2 or 1, by what every row's start is a multiple of.
@@ -402,7 +446,10 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
       constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value;
       constexpr bool WIDE = V >= 4;
       auto kernel = WIDE && past ? norm_backward_kernel<TX, TY, G, E, V, WIDE> : norm_backward_kernel<TX, TY, G, E, V, false>;
-      hipLaunchKernelGGL(kernel, dim3(parts), dim3(1024), 0, st, p);
+      p.row_wgs = p.dx || p.partial ? parts : 0;
+      p.lanes = a.rows <= 128 ? 64 : 16;
+      const int columns = sums && !joined ? (a.width + p.lanes - 1) / p.lanes : 0;
+      hipLaunchKernelGGL(kernel, dim3(p.row_wgs + columns), dim3(1024), 0, st, p);
     };
     auto sized = [&](auto vc) {
       typedef std::integral_constant<int, 8> eight;

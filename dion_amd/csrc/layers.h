@@ -19,6 +19,7 @@ struct NormArgs {
   void* dx;
   float* partial;  // norm_partial_floats(rows, width), which may be none, where dw or db is asked for
   void *dw, *db;   // of w_dtype, b_dtype, or null
+  int row_wgs, lanes;  // set by the launcher: workgroups that take rows, and columns of each of those behind them
 };
 size_t norm_partial_floats(int rows, int width);
 hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st);

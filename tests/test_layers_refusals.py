@@ -74,7 +74,7 @@ def test_workspaces_are_checked():
     for kw in ({}, {"ws": P, "nbytes": 100}, {"ws": P + 8, "nbytes": 1 << 20}):
         assert gated_forward(lib, k=63, ldx=63, ldg=63, ldu=63, **kw) == -2 and "workspace" in lib.dion_last_error().decode()
         assert gated_backward(lib, **kw) == -2
-        assert norm_backward(lib, **{"ws": None, "nbytes": 0, "rows": 100, **kw}) == -2
+        assert norm_backward(lib, **{"ws": None, "nbytes": 0, "rows": 2000, **kw}) == -2
         assert rows_backward(lib, **{"ws": None, "nbytes": 0, **kw}) == -2
     assert gated_forward(lib, t=0, x=None, h=None) == 0 and norm_forward(lib, rows=0, x=None, y=None) == 0
     assert rows_forward(lib, t=0, ids=None, y=None) == 0
@@ -86,8 +86,8 @@ def test_workspaces_are_checked():
             assert bytes_of(t, k, n, backward, 15) >= max(one) and all(b % 256 == 0 for b in one)
     assert lib.dion_gated_kept_bytes(3, 33, 24) == 3 * 64 * 6 and lib.dion_gated_kept_bytes(3, 32, 32) == 3 * 32 * 8
     assert lib.dion_gated_kept_bytes(-1, 8, 24) == 0 and lib.dion_gated_kept_bytes(3, 32, 16) == 0
-    assert lib.dion_layer_norm_workspace_bytes(0, 8) == 0 and lib.dion_layer_norm_workspace_bytes(64, 8) == 0
-    assert lib.dion_layer_norm_workspace_bytes(65, 8) >= 2 * 8 * 4 and lib.dion_layer_norm_workspace_bytes(1, 20000) >= 2 * 20000 * 4
+    assert lib.dion_layer_norm_workspace_bytes(0, 8) == 0 and lib.dion_layer_norm_workspace_bytes(1024, 8) == 0
+    assert lib.dion_layer_norm_workspace_bytes(1025, 8) >= 2 * 8 * 4 and lib.dion_layer_norm_workspace_bytes(1, 20000) >= 2 * 20000 * 4
     assert lib.dion_embedding_workspace_bytes(0, 8, 8) >= 9 * 4 + 8 * 4 and lib.dion_embedding_workspace_bytes(1, 0, 8) == 0
 
 
