@@ -1069,15 +1069,27 @@ def lion_step(X: List[Tensor], G: List[Tensor], M: List[Tensor], lr: Tensor, bet
 ACTIVATIONS = {None: 0, "relu": 1, "relu_squared": 2, "gelu": 3, "gelu_tanh": 4, "silu": 5}
 
 
+_MOST = (1 << 31) - 1  # what a C int holds
+
+
+def _refuse_long(*sizes: int) -> None:
+    if max(sizes) > _MOST:
+        raise ValueError(f"a tensor of {' x '.join(map(str, sizes))} passes the kernels' 2^31 - 1 rows and columns")
+
+
 def _rows(t: Optional[Tensor], copy: int = 0) -> Tuple[Optional[Tensor], Optional[int], int, int]:
     """A tensor (of any number of dimensions) as rows that are dense and do not overlap: itself, a view or a copy, which has to
     live as long as its address is used; their address; the elements between them; ``copy`` if they are not whole 16-byte
-    chunks, else 0."""
+    chunks, else 0.  ValueError where their number or length does not fit the C entries' int, which would lose its upper bits."""
     if t is None:
         return None, None, 0, 0
     if t.dim() != 2:
+        if t.numel() > _MOST:
+            _refuse_long(t.shape[:-1].numel(), t.shape[-1])
         t = t.reshape(-1, t.shape[-1])
     (rows, cols), (ld, inner) = t.shape, t.stride()
+    if rows > _MOST or cols > _MOST:
+        _refuse_long(rows, cols)
     if inner != 1 and cols > 1 or rows > 1 and ld < cols:
         t, ld = t.contiguous(), cols
     elif rows <= 1:
@@ -1459,6 +1471,7 @@ def embedding_forward(ids: Tensor, weight: Tensor, scale: float, dtype: Optional
     if dtype not in _FLOATS:
         raise TypeError(f"{op}: dtype must be torch.bfloat16 or torch.float32, got {dtype}")
     vocab, width = weight.shape
+    _refuse_long(ids.numel())
     with _device_of(weight):
         w, pw, ldw, _ = _rows(weight)
         t = ids.contiguous()
@@ -1480,6 +1493,7 @@ def embedding_backward(dy: Tensor, ids: Tensor, vocab: int, scale: float, paddin
     _check_operand(op, "dy", dy, ids.shape + (width,), index, _FLOATS)
     if dtype not in _FLOATS:
         raise TypeError(f"{op}: the gradient must be torch.bfloat16 or torch.float32, got {dtype}")
+    _refuse_long(vocab)
     return embedding_grad(dy, ids, vocab, scale, padding_idx, dtype)
 
 
