@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void embedding_join_kernel(const S
 }
 
 // ---------------------------------------------------------------------------------------------- host
-constexpr int64_t kMostUnits = int64_t(1) << 30;  // of wavefronts of a launch: room for the strides in 32 bits
+constexpr int64_t kMostUnits = int64_t(1) << 30;  // of the gradient's rows' slices: room for the strides in 32 bits
 
 struct EmbeddingSpace {
   size_t order, first, count, partial, total;
@@ -392,20 +392,20 @@ static bool embedding_fits(const void* p, int64_t ld, int dtype, int v) {  // wh
 hipError_t launch_embedding_forward(const EmbeddingArgs& a, hipStream_t st) {
   const bool past = (int64_t)a.tokens * a.width * (a.y_dtype ? 4 : 2) > kPast;
   if (a.tokens <= 0 || a.vocab <= 0 || a.width <= 0 || !a.ids || !a.w || !a.y) return hipErrorInvalidValue;
-  hipError_t err = hipSuccess;
   auto go = [&](auto* tw, auto* ty, auto vc) {
     typedef std::remove_pointer_t<decltype(tw)> TW;
     typedef std::remove_pointer_t<decltype(ty)> TY;
     constexpr int V = decltype(vc)::value;
-    const int64_t per_row = (a.width + 256 * V - 1) / (256 * V), units = per_row * a.tokens;
-    if (units > kMostUnits) {
-      err = hipErrorInvalidValue;
-      return;
-    }
+    const int64_t per_row = (a.width + 256 * V - 1) / (256 * V), at_once = kMostThreads / 256 * 4 / per_row;  // (tokens)
     constexpr bool WIDE = V == 8;
     auto kernel = WIDE && past ? embedding_rows_kernel<TW, TY, V, WIDE> : embedding_rows_kernel<TW, TY, V, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a, (uint32_t)per_row,
-                       (uint32_t)units);
+    for (int64_t t = 0; t < a.tokens; t += at_once) {
+      EmbeddingArgs p = a;
+      p.ids = (const char*)a.ids + t * (a.ids64 ? 8 : 4);
+      p.y = (TY*)a.y + t * a.width;
+      const int64_t units = per_row * (a.tokens - t < at_once ? a.tokens - t : at_once);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, p, (uint32_t)per_row, (uint32_t)units);
+    }
   };
   auto sized = [&](auto* tw, auto* ty) {
     auto fits = [&](int v) {
@@ -417,7 +417,7 @@ hipError_t launch_embedding_forward(const EmbeddingArgs& a, hipStream_t st) {
   };
   if (a.w_dtype) a.y_dtype ? sized((float*)nullptr, (float*)nullptr) : sized((float*)nullptr, (bf16_t*)nullptr);
   else a.y_dtype ? sized((bf16_t*)nullptr, (float*)nullptr) : sized((bf16_t*)nullptr, (bf16_t*)nullptr);
-  return err != hipSuccess ? err : hipGetLastError();
+  return hipGetLastError();
 }
 
 hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
@@ -470,7 +470,9 @@ hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st) {
   const bool longs = a.tokens > kRun;
   const int64_t units = (int64_t)a.vocab * p.slices, run_units = longs ? ((int64_t)a.tokens + kRun - 1) / kRun * p.slices : 0;
   const int64_t run_wgs = (run_units + 3) / 4, row_wgs = (units + 4 * kUnits - 1) / (4 * kUnits);
-  if (units > kMostUnits || run_units > kMostUnits || (a.width + kSlice - 1) / kSlice > 65535) return hipErrorInvalidValue;
+  if (units > kMostUnits || run_units > kMostUnits || (a.width + kSlice - 1) / kSlice > 65535 ||
+      (run_wgs + row_wgs) * 256 > kMostThreads)
+    return hipErrorInvalidValue;
   auto go = [&](auto* id, auto* ty, auto* tw, auto vc, auto sc) {
     typedef std::remove_pointer_t<decltype(id)> ID;
     typedef std::remove_pointer_t<decltype(ty)> TY;
