@@ -2324,7 +2324,8 @@ static int check_rows(const char* who, const char* arg, const void* p, int64_t l
 }
 
 static int check_norm(const char* who, int rows, int width) {
-  if (rows < 0 || width < 1 || width > kMostColumns) return fail(DION_E_INVALID, "%s: %d rows of %d", who, rows, width);
+  if (rows < 0 || width < 1) return fail(DION_E_INVALID, "%s: %d rows of %d", who, rows, width);
+  if (rows > (1 << 30) || width > kMostColumns) return fail(DION_E_INVALID, "%s: more than 2^30 rows or 2^24 columns", who);
   return DION_OK;
 }
 

@@ -374,6 +374,22 @@ static int norm_vec(const NormArgs& a, const void* other, int64_t ldo, int other
   return fits(most) ? most : fits(2) ? 2 : 1;
 }
 
+// go(its arguments) for every run of rows that a launch has threads for, so many a row.
+template <typename F>
+static void norm_runs(const NormArgs& a, int threads, F&& go) {
+  const int64_t at_once = kMostThreads / 1024 * (1024 / threads), x = a.x_dtype ? 4 : 2, y = a.y_dtype ? 4 : 2;
+  for (int64_t r = 0; r < a.rows; r += at_once) {
+    NormArgs p = a;
+    p.rows = (int)(a.rows - r < at_once ? a.rows - r : at_once);
+    p.x = (const char*)a.x + r * a.ldx * x;
+    if (a.y) p.y = (char*)a.y + r * a.width * y;
+    if (a.mean) p.mean += r, p.rstd += r;
+    if (a.dy) p.dy = (const char*)a.dy + r * a.lddy * y;
+    if (a.dx) p.dx = (char*)a.dx + r * a.width * x;
+    go(p);
+  }
+}
+
 template <typename F>
 static hipError_t norm_types(const NormArgs& a, F&& go) {
   if (a.x_dtype) {
@@ -393,14 +409,18 @@ hipError_t launch_norm_forward(const NormArgs& a, hipStream_t st) {
     typedef std::remove_pointer_t<decltype(tx)> TX;
     typedef std::remove_pointer_t<decltype(ty)> TY;
     if (a.width > 2 * kNormWide) {
-      hipLaunchKernelGGL((norm_forward_wide_kernel<TX, TY>), dim3(a.rows), dim3(1024), 0, st, a);
+      norm_runs(a, 1024, [&](const NormArgs& p) {
+        hipLaunchKernelGGL((norm_forward_wide_kernel<TX, TY>), dim3(p.rows), dim3(1024), 0, st, p);
+      });
       return;
     }
     auto run = [&](auto gc, auto ec, auto vc) {
       constexpr int G = decltype(gc)::value, E = decltype(ec)::value, V = decltype(vc)::value, T = G < 256 ? 256 : G;
       constexpr bool WIDE = V >= 4;
       auto kernel = WIDE && past ? norm_forward_kernel<TX, TY, G, E, V, WIDE> : norm_forward_kernel<TX, TY, G, E, V, false>;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.rows * G + T - 1) / T)), dim3(T), 0, st, a);
+      norm_runs(a, G, [&](const NormArgs& p) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)p.rows * G + T - 1) / T)), dim3(T), 0, st, p);
+      });
     };
     // Up to 64 elements a thread: rows of up to 4096 columns then need no barrier, and wider ones a workgroup of four wavefronts.  Not
     // where they are read one by one, and in the first case not in pairs.  us, 64 / 32 a thread: 16384 x 4096 56 / 66, 4096 x 16384
@@ -437,7 +457,10 @@ hipError_t launch_norm_backward(const NormArgs& a, hipStream_t st) {
     typedef std::remove_pointer_t<decltype(ty)> TY;
     if (a.width > kNormWide) {
       const int per = (a.rows + parts - 1) / parts;
-      if (p.dx) hipLaunchKernelGGL((norm_backward_wide_kernel<TX, TY>), dim3(a.rows), dim3(1024), 0, st, p);
+      if (p.dx)
+        norm_runs(p, 1024, [&](const NormArgs& q) {
+          hipLaunchKernelGGL((norm_backward_wide_kernel<TX, TY>), dim3(q.rows), dim3(1024), 0, st, q);
+        });
       if (p.partial)
         hipLaunchKernelGGL((norm_columns_kernel<TX, TY>), dim3((a.width + 255) / 256, parts), dim3(256), 0, st, p, per);
       return;

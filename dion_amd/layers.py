@@ -38,7 +38,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
     the backward pass it keeps ``x``, the weight and two float32 values a row.  Gradients are of their tensor's type, sums of
     the weight's and the bias's float32 until they are rounded, and repeat bit for bit.  Any strides (a last dimension that is not
-    contiguous is copied) and up to 2^24 columns.  Captures as for ``linear``."""
+    contiguous is copied), up to 2^30 rows and 2^24 columns.  Captures as for ``linear``."""
     if forward_ad._current_level >= 0:
         _refuse_tangents(x, weight, bias, op="layer_norm")
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or

@@ -480,7 +480,8 @@ int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kep
 /* --------------------------------------------------------------------------------------------
  * Layer norm of rows: m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), y = (x - m) r weight + bias, and its gradients.  x, y bf16
  * or fp32 each, `ld*` elements between the rows of x and dy, results dense; weight, bias [width] (null: 1, 0) bf16 or fp32
- * each.  Arithmetic and sums are fp32.  mean, rstd [rows] (both or neither): what the backward pass reads.  At most 2^24 columns.
+ * each.  Arithmetic and sums are fp32.  mean, rstd [rows] (both or neither): what the backward pass reads.  At most 2^30 rows
+ * and 2^24 columns.
  * ------------------------------------------------------------------------------------------ */
 int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* bias,
                             int bias_dtype, void* y, int y_dtype, float* mean, float* rstd, int rows, int width, float eps,

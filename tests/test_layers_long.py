@@ -33,3 +33,10 @@ def test_calls_refuse_them(rows):
             call()
     with pytest.raises(ValueError, match="passes the kernels'"):
         ops.embedding_backward(one, ids, rows, 1.0, None, BF)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_layer_norm_takes():
+    x = torch.ones(2 ** 30 + 1, 1, device="cuda", dtype=BF)
+    with pytest.raises(ValueError, match="more than 2\\^30 rows"):
+        layer_norm(x)
