@@ -8,6 +8,9 @@
 
 namespace dion {
 
+// Threads of a launch: HIP counts them modulo 2^32, and starts what is left of a larger number without an error.
+constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;
+
 typedef uint16_t bf16_t;  // raw bfloat16 bits in memory
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;

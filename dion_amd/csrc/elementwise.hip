@@ -777,13 +777,16 @@ __global__ __launch_bounds__(256) void scale_rows_kernel(const bf16_t* __restric
 hipError_t launch_scale_rows(const bf16_t* U, const float* scale, void* out, int out_dtype, int64_t n_rows,
                              int cols, hipStream_t st) {
   if (n_rows <= 0 || cols <= 0) return hipSuccess;
-  if (n_rows > 0x7fffffff) return hipErrorInvalidValue;
-  if (out_dtype == 0)
-    hipLaunchKernelGGL((scale_rows_kernel<bf16_t>), dim3((unsigned)n_rows), dim3(256), 0, st, U, scale,
-                       (bf16_t*)out, cols);
-  else
-    hipLaunchKernelGGL((scale_rows_kernel<float>), dim3((unsigned)n_rows), dim3(256), 0, st, U, scale,
-                       (float*)out, cols);
+  constexpr int64_t at_once = kMostThreads / 256;
+  for (int64_t r = 0; r < n_rows; r += at_once) {
+    const dim3 grid((unsigned)(n_rows - r < at_once ? n_rows - r : at_once));
+    if (out_dtype == 0)
+      hipLaunchKernelGGL((scale_rows_kernel<bf16_t>), grid, dim3(256), 0, st, U + r * cols, scale + r,
+                         (bf16_t*)out + r * cols, cols);
+    else
+      hipLaunchKernelGGL((scale_rows_kernel<float>), grid, dim3(256), 0, st, U + r * cols, scale + r,
+                         (float*)out + r * cols, cols);
+  }
   return hipGetLastError();
 }
 

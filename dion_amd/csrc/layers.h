@@ -45,9 +45,6 @@ size_t embedding_space_bytes(int tokens, int vocab, int width);
 hipError_t launch_embedding_forward(const EmbeddingArgs& a, hipStream_t st);
 hipError_t launch_embedding_backward(const EmbeddingArgs& a, hipStream_t st);
 
-// Threads of a launch: HIP counts them modulo 2^32, and starts what is left of a larger number without an error.
-constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;
-
 // A result of more bytes than the L2s of the eight XCDs hold is stored non-temporally.  us without / with: layer norm of 8192 x 2048
 // 13.9 / 12.2, 16384 x 2048 25.6 / 21.5, 16384 x 4096 53 / 54, forward and backward 146 / 137; rows of a table, 8192 x 4096 18.8 / 17.7,
 // 16384 x 4096 36.3 / 32.2.
