@@ -24,8 +24,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        grads = ops.layer_norm_grads if ops.plain_on_one_device(dy, x, weight, stats) else ops.layer_norm_backward
-        return (*grads(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
+        return (*ops.layer_norm_backward(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -60,8 +59,7 @@ class _Embedding(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         ids = ctx.saved_tensors[0]
-        grad = ops.embedding_grad if ops.plain_on_one_device(dy, ids) else ops.embedding_backward
-        return None, grad(dy, ids, *ctx.table), None, None, None
+        return None, ops.embedding_backward(dy, ids, *ctx.table), None, None, None
 
 
 def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None,

@@ -132,8 +132,7 @@ class _GatedLinear(torch.autograd.Function):
     def backward(ctx, dh):
         need = ctx.needs_input_grad
         x, weight_gate, weight_up, kept = ctx.saved_tensors
-        grads = ops.gated_grads if ops.plain_on_one_device(dh, x, weight_gate, weight_up, kept) else ops.gated_backward
-        return (*grads(dh, kept, ctx.keep, x, weight_gate, weight_up, *need[:3], *ctx.bias_dtypes), None)
+        return (*ops.gated_backward(dh, kept, ctx.keep, x, weight_gate, weight_up, *need[:3], *ctx.bias_dtypes), None)
 
 
 def gated_linear(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: Optional[Tensor] = None,

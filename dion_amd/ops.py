@@ -1161,7 +1161,8 @@ def _check_linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Opti
         raise ValueError(f"linear: activation {activation!r} goes with{'out' if activation is None else ''} slopes")
     if slope is not None:
         want = (ds[:-1].numel(), -(-fan_out // 8) * 8)
-        if slope.get_device() != index or slope.dtype != torch.int16 or tuple(slope.shape) != want or not slope.is_contiguous():
+        if type(slope) not in _PLAIN_SET or slope.get_device() != index or slope.dtype != torch.int16 or \
+                tuple(slope.shape) != want or not slope.is_contiguous():
             raise ValueError(f"linear: expected the slopes that the forward pass kept, int16 of shape {want} on device {index}")
     if need_dw:
         _check_linear("x", x, ds[:-1] + (fan_in,), index)
@@ -1260,18 +1261,6 @@ def _code(t: Optional[Tensor]) -> int:
     return DION_F32 if t is not None and t.dtype == torch.float32 else DION_BF16
 
 
-def plain_on_one_device(t: Tensor, *others: Optional[Tensor]) -> bool:
-    """Whether a gradient and what a forward pass kept can be read as they are: not where autograd, or a hook on what it saved, has given
-    back a wrapper or a tensor that lies elsewhere."""
-    index = t.get_device()
-    if index < 0 or type(t) not in _PLAIN_SET:
-        return False
-    for o in others:
-        if o is not None and (type(o) not in _PLAIN_SET or o.get_device() != index):
-            return False
-    return True
-
-
 def _viewed(t: Tensor, lead, cols: int) -> Tensor:
     return t if len(lead) == 1 else t.view(*lead, cols)
 
@@ -1341,19 +1330,13 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         if x is None:
             raise ValueError(f"{op}: the gradients of the weights need x")
         _check_operand(op, "x", x, lead + (fan_in,), index)
-    if kept is None or kept.get_device() != index or kept.dtype != torch.uint8 or not kept.is_contiguous() or \
+    if type(kept) not in _PLAIN_SET or kept.get_device() != index or kept.dtype != torch.uint8 or not kept.is_contiguous() or \
             keep not in (24, 32) or kept.numel() != _gated_kept(lead.numel(), fan_out, keep):
         raise ValueError(f"{op}: expected what the forward pass kept of {lead.numel()} x {fan_out} elements, in {keep} bits")
     for t in (bias_gate_dtype, bias_up_dtype):
         if t is not None and t not in _FLOATS:
             raise TypeError(f"{op}: a bias must be torch.bfloat16 or torch.float32, got {t}")
-    return gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, need_dup, bias_gate_dtype, bias_up_dtype)
-
-
-def gated_grads(dh, kept, keep, x, weight_gate, weight_up, need_dx, need_dgate, need_dup, bias_gate_dtype, bias_up_dtype):
-    """``gated_backward`` of what the forward pass kept, whose operands it has checked, and a gradient that autograd has."""
-    fan_out, fan_in = weight_gate.shape
-    lead, need_dw = dh.shape[:-1], need_dgate or need_dup
+    need_dw = need_dgate or need_dup
     with _device_of(dh):
         dh, pdh, lddh, _ = _rows(dh)
         x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
@@ -1415,6 +1398,11 @@ def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tenso
     return _viewed(y, lead, width), stats
 
 
+@functools.lru_cache(maxsize=4096)
+def _norm_bytes(rows: int, width: int) -> int:
+    return _lib.load().dion_layer_norm_workspace_bytes(rows, width)
+
+
 def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor, need_dx: bool, need_dw: bool,
                         bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients ``(dx, dweight, dbias)`` of ``layer_norm_forward``, None where not asked for (``bias_dtype`` None: no ``dbias``)."""
@@ -1422,22 +1410,13 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: 
     index = _check_norm(x, weight, None)
     _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
     rows = x.shape[:-1].numel()
-    if stats.get_device() != index or stats.dtype != torch.float32 or tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
+    if type(stats) not in _PLAIN_SET or stats.get_device() != index or stats.dtype != torch.float32 or \
+            tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
     if need_dw and weight is None:
         raise ValueError(f"{op}: the gradient of the weight needs the weight")
     if bias_dtype is not None and bias_dtype not in _FLOATS:
         raise TypeError(f"{op}: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
-    return layer_norm_grads(dy, x, weight, stats, need_dx, need_dw, bias_dtype)
-
-
-@functools.lru_cache(maxsize=4096)
-def _norm_bytes(rows: int, width: int) -> int:
-    return _lib.load().dion_layer_norm_workspace_bytes(rows, width)
-
-
-def layer_norm_grads(dy, x, weight, stats, need_dx, need_dw, bias_dtype):
-    """``layer_norm_backward`` of what the forward pass kept, whose operands it has checked, and a gradient that autograd has."""
     lead, width = x.shape[:-1], x.shape[-1]
     with _device_of(x):
         dy, pdy, lddy, _ = _rows(dy)
@@ -1481,6 +1460,11 @@ def embedding_forward(ids: Tensor, weight: Tensor, scale: float, dtype: Optional
     return y
 
 
+@functools.lru_cache(maxsize=4096)
+def _embedding_bytes(tokens: int, vocab: int, width: int) -> int:
+    return _lib.load().dion_embedding_workspace_bytes(tokens, vocab, width)
+
+
 def embedding_backward(dy: Tensor, ids: Tensor, vocab: int, scale: float, padding_idx: Optional[int], dtype: torch.dtype) -> Tensor:
     """The gradient ``[vocab, width]``, of ``dtype``, of the table of ``embedding_forward``: a row is ``scale`` times the sum of the
     rows of ``dy`` whose id it is, in their order."""
@@ -1494,17 +1478,6 @@ def embedding_backward(dy: Tensor, ids: Tensor, vocab: int, scale: float, paddin
     if dtype not in _FLOATS:
         raise TypeError(f"{op}: the gradient must be torch.bfloat16 or torch.float32, got {dtype}")
     _refuse_long(vocab)
-    return embedding_grad(dy, ids, vocab, scale, padding_idx, dtype)
-
-
-@functools.lru_cache(maxsize=4096)
-def _embedding_bytes(tokens: int, vocab: int, width: int) -> int:
-    return _lib.load().dion_embedding_workspace_bytes(tokens, vocab, width)
-
-
-def embedding_grad(dy, ids, vocab, scale, padding_idx, dtype):
-    """``embedding_backward`` of ids that the forward pass has checked and a gradient that autograd has."""
-    width = dy.shape[-1]
     with _device_of(dy):
         dy, pdy, lddy, _ = _rows(dy)
         t = ids.contiguous()
