@@ -1200,14 +1200,14 @@ def linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation
         r, pr, ldr, _ = _rows(residual)
         b = None if bias is None else bias.contiguous()
         tokens = x.shape[0]
-        y = x.new_empty((tokens, fan_out))
+        y = x.new_empty((*lead, fan_out))  # (no view: autograd refuses to change one that a custom function returns)
         # (in whole 16-byte chunks)
         slope = x.new_empty((tokens, -(-fan_out // 8) * 8), dtype=torch.int16) if keep_slope and act else None
         ws, nbytes = _linear_space(tokens, fan_in, fan_out, x.device, False, act, copy_x | copy_w)
         check(_lib.load().dion_linear_forward(px, ldx, pw, ldw, _ptr(b), DION_BF16 if b is None else _dtype_code(b, "bias"),
                                               act, pr, ldr, y.data_ptr(), _ptr(slope), tokens, fan_in, fan_out, _ptr(ws),
                                               nbytes, _stream_handle(x.device)), "linear")
-    return (y if len(lead) == 1 else y.view(*lead, fan_out)), slope
+    return y, slope
 
 
 def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[str], x: Optional[Tensor],
@@ -1223,14 +1223,12 @@ def linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Optional[st
         w, pw, ldw, copy_w = _rows(weight if need_dx else None, _lib.DION_LINEAR_COPY_W)
         tokens = dy.shape[0]
         ws, nbytes = _linear_space(tokens, fan_in, fan_out, dy.device, True, act, copy_x | copy_w | copy_dy)
-        dx = dy.new_empty((tokens, fan_in)) if need_dx else None
+        dx = dy.new_empty((*lead, fan_in)) if need_dx else None
         dw = dy.new_empty((fan_out, fan_in)) if need_dw else None
         db = dy.new_empty((fan_out,), dtype=bias_dtype) if bias_dtype is not None else None
         check(_lib.load().dion_linear_backward(pdy, lddy, _ptr(slope), act, px, ldx, pw, ldw, _ptr(dx), _ptr(dw), _ptr(db),
                                                DION_BF16 if db is None else _dtype_code(db, "bias"), tokens, fan_in, fan_out,
                                                _ptr(ws), nbytes, _stream_handle(dy.device)), "linear backward")
-    if need_dx and len(lead) != 1:
-        dx = dx.view(*lead, fan_in)
     return dx, dw, db
 
 
@@ -1259,10 +1257,6 @@ def _space(nbytes: int, device: torch.device) -> Optional[Tensor]:
 
 def _code(t: Optional[Tensor]) -> int:
     return DION_F32 if t is not None and t.dtype == torch.float32 else DION_BF16
-
-
-def _viewed(t: Tensor, lead, cols: int) -> Tensor:
-    return t if len(lead) == 1 else t.view(*lead, cols)
 
 
 def _check_gated_weights(op: str, t: Tensor, name: str, gate: Tensor, up: Tensor, side: int) -> int:
@@ -1308,14 +1302,14 @@ def gated_forward(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: 
         bg = None if bias_gate is None else bias_gate.contiguous()
         bu = None if bias_up is None else bias_up.contiguous()
         tokens = x.shape[0]
-        h = x.new_empty((tokens, fan_out))
+        h = x.new_empty((*lead, fan_out))
         kept = x.new_empty((_gated_kept(tokens, fan_out, keep),), dtype=torch.uint8) if keep else None
         nbytes = _gated_bytes(tokens, fan_in, fan_out, False, copy_x | copy_g | copy_u)
         ws = _space(nbytes, x.device)
         check(_lib.load().dion_gated_forward(px, ldx, pg, ldg, pu, ldu, _ptr(bg), _code(bg), _ptr(bu), _code(bu),
                                              ACTIVATIONS[activation], h.data_ptr(), _ptr(kept), keep, tokens, fan_in, fan_out,
                                              _ptr(ws), nbytes, _stream_handle(x.device)), op)
-    return _viewed(h, lead, fan_out), kept
+    return h, kept
 
 
 def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], weight_gate: Tensor, weight_up: Tensor, need_dx: bool,
@@ -1345,7 +1339,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         tokens = dh.shape[0]
         nbytes = _gated_bytes(tokens, fan_in, fan_out, True, copy_x | copy_g | copy_u)
         ws = _space(nbytes, dh.device)
-        dx = dh.new_empty((tokens, fan_in)) if need_dx else None
+        dx = dh.new_empty((*lead, fan_in)) if need_dx else None
         dgate = dup = None
         behind = need_dgate and need_dup
         if behind:  # (one product: the second behind the first, which starts on a multiple of 8 rows)
@@ -1360,7 +1354,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         check(_lib.load().dion_gated_backward(pdh, lddh, kept.data_ptr(), keep, px, ldx, pg, ldg, pu, ldu, _ptr(dx),
                                               _ptr(dgate), _ptr(dup), behind, _ptr(dbg), _code(dbg), _ptr(dbu), _code(dbu), tokens, fan_in,
                                               fan_out, _ptr(ws), nbytes, _stream_handle(dh.device)), "gated_linear backward")
-    return (_viewed(dx, lead, fan_in) if need_dx else None), dgate, dup, dbg, dbu
+    return dx, dgate, dup, dbg, dbu
 
 
 def _check_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> int:
@@ -1389,13 +1383,13 @@ def layer_norm_forward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tenso
         w = None if weight is None else weight.contiguous()
         b = None if bias is None else bias.contiguous()
         rows = x.shape[0]
-        y = x.new_empty((rows, width), dtype=dtype)
+        y = x.new_empty((*lead, width), dtype=dtype)
         stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
         at = None if stats is None else stats.data_ptr()
         check(_lib.load().dion_layer_norm_forward(px, ldx, _code(x), _ptr(w), _code(w), _ptr(b), _code(b), y.data_ptr(), _code(y),
                                                   at, None if at is None else at + 4 * rows, rows, width, eps,
                                                   _stream_handle(x.device)), "layer_norm")
-    return _viewed(y, lead, width), stats
+    return y, stats
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1423,7 +1417,7 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: 
         x, px, ldx, _ = _rows(x)
         rows = x.shape[0]
         w = None if weight is None else weight.contiguous()
-        dx = x.new_empty((rows, width)) if need_dx else None
+        dx = x.new_empty((*lead, width)) if need_dx else None
         dw = w.new_empty((width,)) if need_dw else None
         db = x.new_empty((width,), dtype=bias_dtype) if bias_dtype is not None else None
         nbytes = _norm_bytes(rows, width) if need_dw or db is not None else 0
@@ -1431,7 +1425,7 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: 
         check(_lib.load().dion_layer_norm_backward(pdy, lddy, _code(dy), px, ldx, _code(x), _ptr(w), _code(w), at, at + 4 * rows,
                                                    _ptr(dx), _ptr(dw), _ptr(db), _code(db), rows, width, _ptr(ws), nbytes,
                                                    _stream_handle(x.device)), "layer_norm backward")
-    return (_viewed(dx, lead, width) if need_dx else None), dw, db
+    return dx, dw, db
 
 
 def _check_ids(op: str, ids: Tensor, index: int) -> None:
