@@ -124,7 +124,8 @@ class _GatedLinear(torch.autograd.Function):
         # (sums that are stored as float32 are worth it; whether one is asked for does not change the other gradients)
         ctx.keep = 32 if any(b is not None and b.dtype == torch.float32 for b, _ in biases) else 24
         h, kept = ops.gated_forward(x, weight_gate, weight_up, bias_gate, bias_up, activation, ctx.keep)
-        ctx.save_for_backward(x if need[1] or need[2] else None, weight_gate, weight_up, kept)
+        weights = (weight_gate, weight_up) if need[0] else (None, None)
+        ctx.save_for_backward(x if need[1] or need[2] else None, *weights, kept)
         return h
 
     @staticmethod
@@ -143,8 +144,8 @@ def gated_linear(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: O
     float32, and the result is rounded once.
 
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
-    the backward pass it keeps ``x``, the weights and ``act(g)`` and ``act'(g) u`` in 24 bits each (32 beside a float32
-    bias); the gradients that reach the two projections are rounded to bfloat16 for the products, not for the biases.  The gradients of the two
+    the backward pass it keeps ``x`` where a weight needs a gradient, the weights where ``x`` does, and ``act(g)`` and ``act'(g) u`` in
+    24 bits each (32 beside a float32 bias); the gradients that reach the two projections are rounded to bfloat16 for the products, not for the biases.  The gradients of the two
     weights, where both are asked for, share an allocation.  Sizes, strides and captures as for ``linear``, up to 2^20 - 8
     columns of the result."""
     operands = (x, weight_gate, weight_up, bias_gate, bias_up)

@@ -1312,17 +1312,28 @@ def gated_forward(x: Tensor, weight_gate: Tensor, weight_up: Tensor, bias_gate: 
     return h, kept
 
 
-def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], weight_gate: Tensor, weight_up: Tensor, need_dx: bool,
-                   need_dgate: bool, need_dup: bool, bias_gate_dtype: Optional[torch.dtype],
+def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], weight_gate: Optional[Tensor], weight_up: Optional[Tensor],
+                   need_dx: bool, need_dgate: bool, need_dup: bool, bias_gate_dtype: Optional[torch.dtype],
                    bias_up_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], ...]:
     """Gradients ``(dx, dWg, dWu, dbg, dbu)`` of ``gated_forward``, None where not asked for.  ``x`` is read for ``dWg`` and
-    ``dWu``, and may be None without.  Both asked for, they are the two ends of one allocation."""
+    ``dWu``, the weights for ``dx``; ``x``, or both weights, may be None without.  ``dWg`` and ``dWu`` both asked for, they are the two
+    ends of one allocation."""
     op = "gated_linear"
-    index = _check_gated_weights(op, dh, "dh", weight_gate, weight_up, 0)
-    (fan_out, fan_in), lead = weight_gate.shape, dh.shape[:-1]
-    if need_dgate or need_dup:
-        if x is None:
-            raise ValueError(f"{op}: the gradients of the weights need x")
+    need_dw, lead = need_dgate or need_dup, dh.shape[:-1]
+    if need_dw and x is None:
+        raise ValueError(f"{op}: the gradients of the weights need x")
+    if weight_gate is not None and weight_up is not None:
+        index = _check_gated_weights(op, dh, "dh", weight_gate, weight_up, 0)
+        fan_out, fan_in = weight_gate.shape
+    else:  # (without weights their rows' length is that of x, and 1 where only biases are asked for)
+        if need_dx or weight_gate is not None or weight_up is not None:
+            raise ValueError(f"{op}: the gradient of x needs both weights")
+        index = dh.get_device()
+        _check_operand(op, "dh", dh, dh.shape, index)
+        if dh.dim() < 1 or dh.shape[-1] == 0 or need_dw and (x.dim() < 1 or x.shape[-1] == 0):
+            raise ValueError(f"{op}: dh of shape {tuple(dh.shape)} belongs to no weights")
+        fan_out, fan_in = dh.shape[-1], x.shape[-1] if need_dw else 1
+    if need_dw:
         _check_operand(op, "x", x, lead + (fan_in,), index)
     if type(kept) not in _PLAIN_SET or kept.get_device() != index or kept.dtype != torch.uint8 or not kept.is_contiguous() or \
             keep not in (24, 32) or kept.numel() != _gated_kept(lead.numel(), fan_out, keep):
@@ -1330,7 +1341,6 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
     for t in (bias_gate_dtype, bias_up_dtype):
         if t is not None and t not in _FLOATS:
             raise TypeError(f"{op}: a bias must be torch.bfloat16 or torch.float32, got {t}")
-    need_dw = need_dgate or need_dup
     with _device_of(dh):
         dh, pdh, lddh, _ = _rows(dh)
         x, px, ldx, copy_x = _rows(x if need_dw else None, _lib.DION_LINEAR_COPY_X)
