@@ -2374,6 +2374,7 @@ extern "C" int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtyp
                                         size_t workspace_bytes, void* stream) {
   const char* who = "dion_layer_norm_backward";
   if (int rc = check_norm(who, rows, width)) return rc;
+  if (!dx && !dweight) x = dy, ldx = lddy, x_dtype = y_dtype;  // (x is then read for nothing that is stored)
   if (int rc = check_rows(who, "dy", dy, lddy, y_dtype, rows, width)) return rc;
   if (int rc = check_rows(who, "x", x, ldx, x_dtype, rows, width)) return rc;
   if (int rc = check_vector(who, "weight", weight, weight_dtype)) return rc;

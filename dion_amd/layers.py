@@ -15,8 +15,9 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, dtype):
         y, stats = ops.layer_norm_forward(x, weight, bias, eps, dtype, True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = bias.dtype if bias is not None and ctx.needs_input_grad[2] else None
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(x if need[0] or need[1] else None, weight if need[0] else None, stats)
+        ctx.dtypes = bias.dtype if bias is not None and need[2] else None, weight.dtype if weight is not None else None
         return y
 
     @staticmethod
@@ -24,7 +25,7 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*ops.layer_norm_backward(dy, x, weight, stats, need[0], need[1], ctx.bias_dtype), None, None)
+        return (*ops.layer_norm_backward(dy, x, weight, stats, need[0], need[1], *ctx.dtypes), None, None)
 
 
 def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5,
@@ -35,7 +36,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     comes out as the bias).
 
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
-    the backward pass it keeps ``x``, the weight and two float32 values a row.  Gradients are of their tensor's type, sums of
+    the backward pass it keeps two float32 values a row, ``x`` where it or the weight needs a gradient, and the weight where ``x`` does.  Gradients are of their tensor's type, sums of
     the weight's and the bias's float32 until they are rounded, and repeat bit for bit.  Any strides (a last dimension that is not
     contiguous is copied), up to 2^30 rows and 2^24 columns.  Captures as for ``linear``."""
     if forward_ad._current_level >= 0:

@@ -1407,20 +1407,30 @@ def _norm_bytes(rows: int, width: int) -> int:
     return _lib.load().dion_layer_norm_workspace_bytes(rows, width)
 
 
-def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: Tensor, need_dx: bool, need_dw: bool,
-                        bias_dtype: Optional[torch.dtype]) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
-    """Gradients ``(dx, dweight, dbias)`` of ``layer_norm_forward``, None where not asked for (``bias_dtype`` None: no ``dbias``)."""
+def layer_norm_backward(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor], stats: Tensor, need_dx: bool, need_dw: bool,
+                        bias_dtype: Optional[torch.dtype],
+                        weight_dtype: Optional[torch.dtype] = None) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients ``(dx, dweight, dbias)`` of ``layer_norm_forward``, None where not asked for (``bias_dtype`` None: no ``dbias``).  ``x`` is
+    read for ``dx`` and ``dweight``, the weight for ``dx``: either may be None without (``dweight`` is then of ``weight_dtype``)."""
     op = "layer_norm"
+    if need_dx or need_dw:
+        if x is None:
+            raise ValueError(f"{op}: the gradients of x and the weight need x")
+    else:  # (dy stands for x, of which nothing is read)
+        x, weight = dy, None
     index = _check_norm(x, weight, None)
     _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
     rows = x.shape[:-1].numel()
     if type(stats) not in _PLAIN_SET or stats.get_device() != index or stats.dtype != torch.float32 or \
             tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
-    if need_dw and weight is None:
-        raise ValueError(f"{op}: the gradient of the weight needs the weight")
-    if bias_dtype is not None and bias_dtype not in _FLOATS:
-        raise TypeError(f"{op}: bias must be torch.bfloat16 or torch.float32, got {bias_dtype}")
+    if need_dw and weight is None and weight_dtype is None:
+        raise ValueError(f"{op}: the gradient of the weight needs the weight or its type")
+    for name, t in (("bias", bias_dtype), ("weight", weight_dtype)):
+        if t is not None and t not in _FLOATS:
+            raise TypeError(f"{op}: {name} must be torch.bfloat16 or torch.float32, got {t}")
+    if weight is not None:
+        weight_dtype = weight.dtype
     lead, width = x.shape[:-1], x.shape[-1]
     with _device_of(x):
         dy, pdy, lddy, _ = _rows(dy)
@@ -1428,13 +1438,13 @@ def layer_norm_backward(dy: Tensor, x: Tensor, weight: Optional[Tensor], stats: 
         rows = x.shape[0]
         w = None if weight is None else weight.contiguous()
         dx = x.new_empty((*lead, width)) if need_dx else None
-        dw = w.new_empty((width,)) if need_dw else None
+        dw = x.new_empty((width,), dtype=weight_dtype) if need_dw else None
         db = x.new_empty((width,), dtype=bias_dtype) if bias_dtype is not None else None
         nbytes = _norm_bytes(rows, width) if need_dw or db is not None else 0
         ws, at = _space(nbytes, x.device), stats.data_ptr()
-        check(_lib.load().dion_layer_norm_backward(pdy, lddy, _code(dy), px, ldx, _code(x), _ptr(w), _code(w), at, at + 4 * rows,
-                                                   _ptr(dx), _ptr(dw), _ptr(db), _code(db), rows, width, _ptr(ws), nbytes,
-                                                   _stream_handle(x.device)), "layer_norm backward")
+        check(_lib.load().dion_layer_norm_backward(pdy, lddy, _code(dy), px, ldx, _code(x), _ptr(w), _code(dw if w is None else w), at,
+                                                   at + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db), _code(db), rows, width, _ptr(ws),
+                                                   nbytes, _stream_handle(x.device)), "layer_norm backward")
     return dx, dw, db
 
 

@@ -486,7 +486,8 @@ int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kep
 int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* bias,
                             int bias_dtype, void* y, int y_dtype, float* mean, float* rstd, int rows, int width, float eps,
                             void* stream);
-/* dy of y_dtype; dx of x_dtype, dweight of weight_dtype, dbias of bias_dtype; each may be null.  The workspace is read and written where
+/* dy of y_dtype; dx of x_dtype, dweight of weight_dtype, dbias of bias_dtype; each may be null.  x is read for dx and dweight, and may be
+ * null without.  The workspace is read and written where
  * dweight or dbias is asked for. */
 size_t dion_layer_norm_workspace_bytes(int rows, int width);
 int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight,
