@@ -2393,6 +2393,12 @@ extern "C" int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtyp
   if (dweight || dbias)
     if (int rc = check_space(who, workspace, workspace_bytes, norm_partial_floats(rows, width) * sizeof(float))) return rc;
   if (!dx && !dweight && !dbias) return DION_OK;
+  if (dx) {  // (other workgroups may read a row, for the sums, when its dx is written)
+    auto bytes = [&](int64_t ld, int dtype) { return ((size_t)(rows - 1) * ld + width) * (dtype == DION_F32 ? 4 : 2); };
+    const size_t all = bytes(width, x_dtype);
+    if (overlap(dx, all, x, bytes(rows > 1 ? ldx : width, x_dtype)) || overlap(dx, all, dy, bytes(rows > 1 ? lddy : width, y_dtype)))
+      return fail(DION_E_INVALID, "%s: dx overlaps x or dy", who);
+  }
   NormArgs a;
   memset(&a, 0, sizeof(a));
   a.x = x;

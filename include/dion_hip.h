@@ -450,7 +450,8 @@ int dion_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, 
                         int fan_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* dz = dy act' (rounded to bf16 for the products, not for db):  dx = dz w,  dw = dz^T x,  db = sum of dz over the tokens.
- * dx, dw, db may be null; x is read for dw, w for dx, slope with an activation.  (The residual's gradient is dy.) */
+ * dx, dw, db may be null; x is read for dw, w for dx, slope with an activation.  No result may overlap an operand.  (The
+ * residual's gradient is dy.) */
 int dion_linear_backward(const void* dy, int64_t lddy, const void* slope, int activation, const void* x, int64_t ldx,
                          const void* w, int64_t ldw, void* dx, void* dw, void* db, int db_dtype, int tokens, int fan_in,
                          int fan_out, void* workspace, size_t workspace_bytes, void* stream);
@@ -458,8 +459,8 @@ int dion_linear_backward(const void* dy, int64_t lddy, const void* slope, int ac
 /* Both projections of a gated feed-forward block: h = act(x w_gate^T + bias_gate) * (x w_up^T + bias_up), [tokens][fan_out], and
  * its gradients.  Operands and results as above, fan_out at most 2^20 - 8; the biases may be null and of different types.
  * kept (null, or dion_gated_kept_bytes(...) of them, 16-byte aligned): act'(g) u and act(g) of every element, for
- * dion_gated_backward, rounded to kept_bits = 24 bits of fp32, or all 32, which sums for an fp32 bias are worth.  Neither h nor kept may overlap an operand.  copies: DION_LINEAR_COPY_X, _W (w_gate), _DY (dh) and
- * DION_GATED_COPY_UP (w_up). */
+ * dion_gated_backward, rounded to kept_bits = 24 bits of fp32, or all 32, which sums for an fp32 bias are worth.  Neither h nor
+ * kept may overlap an operand.  copies: DION_LINEAR_COPY_X, _W (w_gate), _DY (dh) and DION_GATED_COPY_UP (w_up). */
 #define DION_GATED_COPY_UP 8
 size_t dion_gated_kept_bytes(int tokens, int fan_out, int kept_bits);
 size_t dion_gated_workspace_bytes(int tokens, int fan_in, int fan_out, int backward, int copies);
@@ -471,7 +472,7 @@ int dion_gated_forward(const void* x, int64_t ldx, const void* w_gate, int64_t l
 /* dg = dh act'(g) u, du = dh act(g) (rounded to bf16 for the products, not for the biases):  dx = dg w_gate + du w_up,
  * dw_gate = dg^T x,  dw_up = du^T x,  db_gate, db_up = sums over the tokens.  Any of them may be null; x is read for dw_*, the weights
  * for dx.  dw_behind: dw_up lies fan_out rounded up to 8 rows behind dw_gate, and the rows between them, which are written (zeros),
- * belong to the same buffer: one product instead of two. */
+ * belong to the same buffer: one product instead of two.  No result may overlap an operand. */
 int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kept_bits, const void* x, int64_t ldx,
                         const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up, void* dx, void* dw_gate, void* dw_up,
                         int dw_behind, void* db_gate, int db_gate_dtype, void* db_up, int db_up_dtype, int tokens, int fan_in, int fan_out, void* workspace,
@@ -481,13 +482,13 @@ int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kep
  * Layer norm of rows: m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), y = (x - m) r weight + bias, and its gradients.  x, y bf16
  * or fp32 each, `ld*` elements between the rows of x and dy, results dense; weight, bias [width] (null: 1, 0) bf16 or fp32
  * each.  Arithmetic and sums are fp32.  mean, rstd [rows] (both or neither): what the backward pass reads.  At most 2^30 rows
- * and 2^24 columns.
+ * and 2^24 columns.  y may be x, of the same type, where its rows are dense; no other result may overlap an operand.
  * ------------------------------------------------------------------------------------------ */
 int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* bias,
                             int bias_dtype, void* y, int y_dtype, float* mean, float* rstd, int rows, int width, float eps,
                             void* stream);
 /* dy of y_dtype; dx of x_dtype, dweight of weight_dtype, dbias of bias_dtype; each may be null.  x is read for dx and dweight, and may be
- * null without.  The workspace is read and written where
+ * null without.  No result may overlap an operand: dx over x or dy (the addresses from their first to their last element) is refused.  The workspace is read and written where
  * dweight or dbias is asked for. */
 size_t dion_layer_norm_workspace_bytes(int rows, int width);
 int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight,
@@ -498,7 +499,7 @@ int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtype, const vo
  * Rows of a table: y[t] = scale w[ids[t]], w [vocab][width] bf16 or fp32, ldw elements between its rows, y dense, bf16 or fp32;
  * ids int64 (ids_bits 64) or int32 (32).  An id outside 0 .. vocab - 1 reads nothing and gives a row of NaN.
  * dw[v] = scale times the sum of dy[t] over the tokens t with ids[t] = v, in the order of t, in fp32, rounded once; zeros where there are
- * none and in row `padding` (negative: none).  dw is written whole.  At most 2^24 rows, 2^24 columns, 2^30 tokens.
+ * none and in row `padding` (negative: none).  dw is written whole.  No result may overlap an operand.  At most 2^24 rows, 2^24 columns, 2^30 tokens.
  * ------------------------------------------------------------------------------------------ */
 int dion_embedding_forward(const void* ids, int ids_bits, int tokens, const void* w, int64_t ldw, int w_dtype, int vocab, int width,
                            float scale, void* y, int y_dtype, void* stream);
