@@ -1354,7 +1354,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         behind = need_dgate and need_dup
         if behind:  # (one product: the second behind the first, which starts on a multiple of 8 rows)
             both = dh.new_empty((-(-fan_out // 8) * 8 + fan_out, fan_in))
-            dgate, dup = both[:fan_out], both[-fan_out:]
+            dgate, dup = both[:fan_out], both[-fan_out:].data  # (with a version counter each: either may be changed in place alone)
         elif need_dgate:
             dgate = dh.new_empty((fan_out, fan_in))
         elif need_dup:

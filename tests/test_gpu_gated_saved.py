@@ -57,3 +57,16 @@ def test_operator_call_without_weights():
             ops.gated_backward(**{**good, **bad})
     with pytest.raises(TypeError, match="gated_linear"):
         ops.gated_backward(**{**good, "weight_gate": None, "weight_up": None, "dh": dh.float()})
+
+
+def test_either_weights_gradient_may_be_changed_in_place():
+    """... while a graph keeps the other one, though both lie in one allocation."""
+    (x, wg, wu, _bg, _bu), dh = tensors(24, 40, 56)
+    wg.requires_grad_(), wu.requires_grad_()
+    scale = torch.ones(56, 40, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    for kept in (0, 1):
+        grads = torch.autograd.grad(gated_linear(x, wg, wu), [wg, wu], dh)
+        want = grads[kept].clone()
+        penalty = (grads[kept] * scale).sum()
+        grads[1 - kept].zero_()
+        assert torch.equal(torch.autograd.grad(penalty, scale)[0], want)
