@@ -32,8 +32,9 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
                dtype: Optional[torch.dtype] = None) -> Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension: ``x [..., width]``, ``weight`` and ``bias``
     ``[width]``, bfloat16 or float32 each; the result is of ``dtype`` (None: that of ``x``).  ``var`` is the mean square of the centred
-    values; arithmetic and sums are float32, and the result is rounded once (a row whose squares leave float32, with values past 1.8e19,
-    comes out as the bias).
+    values; arithmetic and sums are float32, and the result is rounded once.  A row whose squared distances from its mean add up past float32
+    (values past about 1.8e19 / sqrt(width)) comes out as the bias, with a gradient of zero; one whose values do (past 3.4e38 / width, of
+    one sign) as NaN.
 
     Differentiable once with respect to every tensor, in reverse mode (a forward-mode tangent is refused: NotImplementedError).  For
     the backward pass it keeps two float32 values a row, ``x`` where it or the weight needs a gradient, and the weight where ``x`` does.  Gradients are of their tensor's type, sums of

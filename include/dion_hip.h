@@ -481,15 +481,15 @@ int dion_gated_backward(const void* dh, int64_t ld_dh, const void* kept, int kep
 /* --------------------------------------------------------------------------------------------
  * Layer norm of rows: m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), y = (x - m) r weight + bias, and its gradients.  x, y bf16
  * or fp32 each, `ld*` elements between the rows of x and dy, results dense; weight, bias [width] (null: 1, 0) bf16 or fp32
- * each.  Arithmetic and sums are fp32.  mean, rstd [rows] (both or neither): what the backward pass reads.  At most 2^30 rows
- * and 2^24 columns.  y may be x, of the same type, where its rows are dense; no other result may overlap an operand.
+ * each.  Arithmetic and sums are fp32 (a row whose sum of (x - m)^2 leaves it comes out as the bias, one whose sum of x does as
+ * NaN).  mean, rstd [rows] (both or neither): what the backward pass reads.  At most 2^30 rows and 2^24 columns.  y may be x, of the same type, where its rows are dense; no other result may overlap an operand.
  * ------------------------------------------------------------------------------------------ */
 int dion_layer_norm_forward(const void* x, int64_t ldx, int x_dtype, const void* weight, int weight_dtype, const void* bias,
                             int bias_dtype, void* y, int y_dtype, float* mean, float* rstd, int rows, int width, float eps,
                             void* stream);
 /* dy of y_dtype; dx of x_dtype, dweight of weight_dtype, dbias of bias_dtype; each may be null.  x is read for dx and dweight, and may be
- * null without.  No result may overlap an operand: dx over x or dy (the addresses from their first to their last element) is refused.  The workspace is read and written where
- * dweight or dbias is asked for. */
+ * null without.  No result may overlap an operand: dx over x or dy (the addresses from their first to their last element) is refused.
+ * The workspace is read and written where dweight or dbias is asked for. */
 size_t dion_layer_norm_workspace_bytes(int rows, int width);
 int dion_layer_norm_backward(const void* dy, int64_t lddy, int y_dtype, const void* x, int64_t ldx, int x_dtype, const void* weight,
                              int weight_dtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
