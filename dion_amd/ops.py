@@ -1239,12 +1239,13 @@ _BF16, _FLOATS, _IDS = (torch.bfloat16,), (torch.bfloat16, torch.float32), (torc
 
 
 def _check_operand(op: str, name: str, t: Tensor, shape, index: int, dtypes=_BF16) -> None:
-    if type(t) in _PLAIN_SET and t.get_device() == index >= 0 and t.shape == shape and t.dtype in dtypes:
+    """(``shape`` None: any.)"""
+    if type(t) in _PLAIN_SET and t.get_device() == index >= 0 and (shape is None or t.shape == shape) and t.dtype in dtypes:
         return
     _require_gpu(t, f"{op}: {name}")
     if t.dtype not in dtypes:
         raise TypeError(f"{op}: {name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
-    if t.shape != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{op}: expected {name} of shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.get_device() != index:
         raise ValueError(f"{op}: {name} is on {t.device}, another tensor on device {index}")
@@ -1266,8 +1267,8 @@ def _check_gated_weights(op: str, t: Tensor, name: str, gate: Tensor, up: Tensor
     if ws[0] == 0 or ws[1] == 0:
         raise ValueError(f"{op}: empty weights of shape {tuple(ws)}")
     index = t.get_device()
-    _check_operand(op, name, t, ts, index)
-    _check_operand(op, "weight_gate", gate, ws, index)
+    _check_operand(op, name, t, None, index)
+    _check_operand(op, "weight_gate", gate, None, index)
     _check_operand(op, "weight_up", up, ws, index)
     return index
 
@@ -1329,7 +1330,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         if need_dx or weight_gate is not None or weight_up is not None:
             raise ValueError(f"{op}: the gradient of x needs both weights")
         index = dh.get_device()
-        _check_operand(op, "dh", dh, dh.shape, index)
+        _check_operand(op, "dh", dh, None, index)
         if dh.dim() < 1 or dh.shape[-1] == 0 or need_dw and (x.dim() < 1 or x.shape[-1] == 0):
             raise ValueError(f"{op}: dh of shape {tuple(dh.shape)} belongs to no weights")
         fan_out, fan_in = dh.shape[-1], x.shape[-1] if need_dw else 1
@@ -1372,10 +1373,12 @@ def _check_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor]) -> 
     if len(xs) < 1 or xs[-1] == 0:
         raise ValueError(f"layer_norm: x of shape {tuple(xs)} has no last dimension to normalise")
     index = x.get_device()
-    _check_operand("layer_norm", "x", x, xs, index, _FLOATS)
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _check_operand("layer_norm", name, t, xs[-1:], index, _FLOATS)
+    _check_operand("layer_norm", "x", x, None, index, _FLOATS)
+    if weight is not None or bias is not None:
+        row = xs[-1:]
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None:
+                _check_operand("layer_norm", name, t, row, index, _FLOATS)
     return index
 
 
@@ -1419,10 +1422,12 @@ def layer_norm_backward(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor
     else:  # (dy stands for x, of which nothing is read)
         x, weight = dy, None
     index = _check_norm(x, weight, None)
-    _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
-    rows = x.shape[:-1].numel()
+    if dy is not x:
+        _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
+    *lead, width = x.shape
+    rows = x.numel() // width
     if type(stats) not in _PLAIN_SET or stats.get_device() != index or stats.dtype != torch.float32 or \
-            tuple(stats.shape) != (2, rows) or not stats.is_contiguous():
+            stats.shape != (2, rows) or not stats.is_contiguous():
         raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
     if need_dw and weight is None and weight_dtype is None:
         raise ValueError(f"{op}: the gradient of the weight needs the weight or its type")
@@ -1431,11 +1436,9 @@ def layer_norm_backward(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor
             raise TypeError(f"{op}: {name} must be torch.bfloat16 or torch.float32, got {t}")
     if weight is not None:
         weight_dtype = weight.dtype
-    lead, width = x.shape[:-1], x.shape[-1]
     with _device_of(x):
         dy, pdy, lddy, _ = _rows(dy)
         x, px, ldx, _ = _rows(x)
-        rows = x.shape[0]
         w = None if weight is None else weight.contiguous()
         dx = x.new_empty((*lead, width)) if need_dx else None
         dw = x.new_empty((width,), dtype=weight_dtype) if need_dw else None
@@ -1449,7 +1452,7 @@ def layer_norm_backward(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor
 
 
 def _check_ids(op: str, ids: Tensor, index: int) -> None:
-    _check_operand(op, "ids", ids, ids.shape, index, _IDS)
+    _check_operand(op, "ids", ids, None, index, _IDS)
 
 
 def embedding_forward(ids: Tensor, weight: Tensor, scale: float, dtype: Optional[torch.dtype]) -> Tensor:
@@ -1458,7 +1461,7 @@ def embedding_forward(ids: Tensor, weight: Tensor, scale: float, dtype: Optional
     if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"{op}: expected a table of two dimensions that is not empty, got {tuple(weight.shape)}")
     index = weight.get_device()
-    _check_operand(op, "weight", weight, weight.shape, index, _FLOATS)
+    _check_operand(op, "weight", weight, None, index, _FLOATS)
     _check_ids(op, ids, index)
     dtype = weight.dtype if dtype is None else dtype
     if dtype not in _FLOATS:
