@@ -65,7 +65,8 @@ struct IndexArgs {
 // wavefront has a run of consecutive tokens; it lists those of the workgroup's rows in LDS, in order, and counts and places from
 // there, 64 at a time, equal ones together; so the tokens of a row stay in order.  Where the list is full it reads the ids again
 // instead.  Bound by the instructions that look at an id that is another workgroup's (255 of 256): 8192 tokens 9 us, 32768 14,
-// 131072 42.  Without lists, every match counted and placed where it is found, 32768 tokens took 33.
+// 131072 42.  Without lists, every match counted and placed where it is found, 32768 tokens took 33.  Tables past 131072 rows have more
+// workgroups, which all read all ids: 8192 tokens of 300000 rows 28.
 template <typename ID>
 __global__ __launch_bounds__(kIndexWaves * 64) void embedding_index_kernel(const IndexArgs a, int rows, int capacity) {
   constexpr int AHEAD = 16;  // ids of a lane on their way

@@ -5,10 +5,11 @@
 //   dWg = dg^T x,  dWu = du^T x          one product of linear.hip where the results lie behind one another
 // Operands bf16, sums fp32.  Tiles, ring and epilogue are lin_tile.h's; like linear.hip's products, large ones are bound by the matrix
 // units at the clock the power limit leaves, and by what all CUs store when a round of tiles ends.
-// us: 8192 x 4096 x 14336 (tokens, fan-in, fan-out) forward 1360, 1.41 PFLOP/s; 8192 x 2048 x 5632 forward with what is kept 351 (277 MB
-// of it; 1408 tiles of 256 x 256, 5.5 rounds of the CUs), dz 108, dx 279, dW 322 (704 tiles of 256 x 128, 2.75 rounds); 8192 x 2048
-// x 8192 480, 180, 418, 409, forward without keeping 424 (1.30 PFLOP/s).  Two workgroups a CU of 128 x 128 tiles in a ring of two slots, so
-// that one stores while the other multiplies, take 452 instead of 351 and 571 instead of 424: their operands come twice as often.
+// us, medians of kernel traces (from card to card 4 % apart): 8192 x 4096 x 14336 (tokens, fan-in, fan-out) forward 1371 to 1435, 1.34 to 1.40
+// PFLOP/s; 8192 x 2048 x 5632 forward with what is kept 369 to 380 (277 MB of it; 1408 tiles of 256 x 256, 5.5 rounds of the CUs), dz
+// 110, dx 289 to 295, dW 334 to 345 (704 tiles of 256 x 128, 2.75 rounds); 8192 x 2048 x 8192 507, 175, 437, 441, forward without keeping 431
+// (1.28 PFLOP/s).  Two workgroups a CU of 128 x 128 tiles in a ring of two slots, so that one stores while the other multiplies, took 452
+// where these took 351, and 571 where 424: their operands come twice as often.
 #include "lin_tile.h"
 
 namespace dion {
@@ -266,6 +267,9 @@ static hipError_t launch_act(const LinTwoParams& tp, bool wide, hipStream_t st) 
 template <class Cfg>
 static hipError_t launch_tiles(const GatedProduct& p, LinTwoParams tp, hipStream_t st) {
   if (!lin_tile_list<Cfg>(p.M, ((int64_t)p.N * 2 + Cfg::BN - 1) / Cfg::BN * Cfg::BN, tp)) return hipErrorInvalidValue;
+  // As in linear.hip, with half its bound on a weight: there are two.  us, a run for each XCD / interleaved, with 24 bits kept: 16384 x 8192 x
+  // 4096 1699 / 1579, 65536 x 2048 x 8192 3871 / 3708, but 32768 x 4096 x 8192 3420 / 3469; larger weights 16384 x 4096 x 14336 2951 / 3054
+  // (16384 x 8192 x 8192 3399 / 3251 the other way), a smaller x 32768 x 2048 x 16384 3773 / 3983, 16384 x 4096 x 4096 837 / 834.
   tp.interleave = Cfg::BM == 256 && Cfg::BN == 256 && (int64_t)p.M * p.K >= (int64_t(128) << 20) &&
                   (int64_t)p.N * p.K <= (int64_t(48) << 20);
   if (tp.splits > 1) return launch_tile<Cfg, false, false, kActNone, false, true, kLinGated>(tp, st);
@@ -371,6 +375,9 @@ size_t pair_product_scratch(int M, int N, int K) {
 template <class Cfg>
 static hipError_t launch_pair_tiles(const PairProduct& p, LinTwoParams tp, hipStream_t st) {
   if (!lin_tile_list<Cfg>(p.M, p.N, tp)) return hipErrorInvalidValue;
+  // Two of each operand: half of linear.hip's bounds.  us with dz, a run for each XCD / interleaved: 16384 x 4096 x 4096 (tokens, fan-in,
+  // fan-out) 956 / 929, 32768 x 4096 x 8192 3946 / 3833, 65536 x 4096 x 8192 7993 / 7751, but 65536 x 1024 x 8192 3068 / 3140; smaller dg
+  // and du 8192 x 2048 x 5632 370 / 367, larger weights 8192 x 4096 x 14336 1643 / 1644 (16384 x 4096 x 14336 3397 / 3304).
   tp.interleave = Cfg::BM == 256 && Cfg::BN == 256 && (int64_t)p.M * p.K >= (int64_t(64) << 20) &&
                   (int64_t)p.N * p.K <= (int64_t(48) << 20);
   return tp.splits > 1 ? launch_tile<Cfg, false, true, kActNone, false, true, kLinPair>(tp, st)

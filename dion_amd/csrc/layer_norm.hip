@@ -2,8 +2,10 @@
 // and its gradients, with g = dy w:  dx = r (g - mean g - xh mean(g xh)),  dw = sum over the rows of dy xh,  db = of dy.
 // Rows stay in registers between the two sums of a pass (the variance is that of the centred values: no difference of large
 // numbers), so x and dy are read once.  Sums fp32, in an order that depends on the sizes alone.  Bound by HBM.  us, bf16: 16384 x 4096
-// forward 55 (4.9 TB/s), backward 67 (6.0) and 4 for the sums over the workgroups; 4096 x 16384 64 and 114, 65536 x 768 41 and 54;
-// one row of 768 2.4, a launch and one way to memory.
+// forward 56 (4.8 TB/s), backward 69 (5.8) and 4 for the sums over the workgroups; 65536 x 768 43 and 53; one row of 768 2.3, a launch
+// and one way to memory.  Not at both ends: the backward pass of 8193 to 16384 columns, with sixteen elements of five arrays a thread,
+// sends 23 to 97 of its registers through scratch memory (52 to 172 bytes a lane), 4096 x 16384 66 and 109 where its bytes take 56 and 84; and
+// rows of 64 or 128 columns leave most of a wavefront idle, 2^20 of 64 286 and 258 where their bytes take 56 and 84.
 #include "layers.h"
 #include "linear.h"
 

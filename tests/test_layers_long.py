@@ -1,8 +1,10 @@
 """Rows and columns past what the C entries' int holds are refused, not counted modulo 2^32."""
+import os
+
 import pytest
 import torch
 
-from dion_amd import embedding, gated_linear, layer_norm, linear, ops
+from dion_amd import _lib, embedding, gated_linear, layer_norm, linear, ops
 
 BF = torch.bfloat16
 LONG = 2 ** 32 + 5  # five, to an int
@@ -18,6 +20,16 @@ def test_rows_that_an_int_does_not_count(shape):
 def test_rows_that_an_int_counts(shape, rows):
     t, _address, ld, _copy = ops._rows(torch.empty(shape, dtype=BF, device="meta"))
     assert t.shape == (rows, shape[-1]) and ld == shape[-1]
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libdion_hip.so not built in this checkout")
+def test_c_entries_refuse_more_rows_than_layer_norm_takes():
+    from test_layers_refusals import norm_backward, norm_forward
+
+    lib = _lib.load()
+    for call in (norm_forward, norm_backward):
+        assert call(lib, rows=2 ** 30 + 1) == -1 and "2^30 rows" in lib.dion_last_error().decode()
+    assert lib.dion_layer_norm_workspace_bytes(2 ** 30 + 1, 8) == 0 and lib.dion_layer_norm_workspace_bytes(2 ** 30, 8) > 0
 
 
 @pytest.mark.gpu
