@@ -1130,6 +1130,12 @@ def _check_weight(t: Tensor, name: str, weight: Tensor, side: int, activation: O
     return index
 
 
+def _is_kept(t: Optional[Tensor], dtype: torch.dtype, shape: Tuple[int, ...], index: int) -> bool:
+    """Whether ``t`` can be what a forward pass has kept for its backward pass, whose address that reads."""
+    return (t is not None and t.get_device() == index and t.dtype == dtype and t.shape == shape and t.is_contiguous() and
+            (type(t) in _PLAIN_SET or not is_traceable_wrapper_subclass(t)))
+
+
 def _check_linear_forward(x: Tensor, weight: Tensor, bias: Optional[Tensor], activation: Optional[str],
                           residual: Optional[Tensor]) -> None:
     index, xs, ws = _check_weight(x, "x", weight, 1, activation), x.shape, weight.shape
@@ -1161,8 +1167,7 @@ def _check_linear_backward(dy: Tensor, slope: Optional[Tensor], activation: Opti
         raise ValueError(f"linear: activation {activation!r} goes with{'out' if activation is None else ''} slopes")
     if slope is not None:
         want = (ds[:-1].numel(), -(-fan_out // 8) * 8)
-        if type(slope) not in _PLAIN_SET or slope.get_device() != index or slope.dtype != torch.int16 or \
-                tuple(slope.shape) != want or not slope.is_contiguous():
+        if not _is_kept(slope, torch.int16, want, index):
             raise ValueError(f"linear: expected the slopes that the forward pass kept, int16 of shape {want} on device {index}")
     if need_dw:
         _check_linear("x", x, ds[:-1] + (fan_in,), index)
@@ -1336,8 +1341,7 @@ def gated_backward(dh: Tensor, kept: Tensor, keep: int, x: Optional[Tensor], wei
         fan_out, fan_in = dh.shape[-1], x.shape[-1] if need_dw else 1
     if need_dw:
         _check_operand(op, "x", x, lead + (fan_in,), index)
-    if type(kept) not in _PLAIN_SET or kept.get_device() != index or kept.dtype != torch.uint8 or not kept.is_contiguous() or \
-            keep not in (24, 32) or kept.numel() != _gated_kept(lead.numel(), fan_out, keep):
+    if keep not in (24, 32) or not _is_kept(kept, torch.uint8, (_gated_kept(lead.numel(), fan_out, keep),), index):
         raise ValueError(f"{op}: expected what the forward pass kept of {lead.numel()} x {fan_out} elements, in {keep} bits")
     for t in (bias_gate_dtype, bias_up_dtype):
         if t is not None and t not in _FLOATS:
@@ -1426,8 +1430,7 @@ def layer_norm_backward(dy: Tensor, x: Optional[Tensor], weight: Optional[Tensor
         _check_operand(op, "dy", dy, x.shape, index, _FLOATS)
     *lead, width = x.shape
     rows = x.numel() // width
-    if type(stats) not in _PLAIN_SET or stats.get_device() != index or stats.dtype != torch.float32 or \
-            stats.shape != (2, rows) or not stats.is_contiguous():
+    if not _is_kept(stats, torch.float32, (2, rows), index):
         raise ValueError(f"{op}: expected the statistics that the forward pass kept, float32 of shape {(2, rows)} on device {index}")
     if need_dw and weight is None and weight_dtype is None:
         raise ValueError(f"{op}: the gradient of the weight needs the weight or its type")
